@@ -30,7 +30,9 @@ CFLAGS = [
     "-Wall", "-Wno-unused-result", "-Wno-unused-value", "-Wno-unused-function",
 ]
 SOURCES = ["moddown.hip", "ntt.hip", "convert.hip", "rescale.hip", "small_ring.hip",
-           "poly_ops.hip", "keyswitch.hip", "encode.hip", "keygen.hip", "context.cpp", "capi.cpp"]
+           "poly_ops.hip", "keyswitch.hip", "encode.hip", "keygen.hip", "clear_scan.hip",
+           "clear_scan_value.hip", "clear_scan_query.hip", "clear_step.hip", "clear_conv.hip",
+           "clear_logprob.hip", "context.cpp", "capi.cpp", "clear_capi.cpp"]
 
 
 def _compile(src: str) -> tuple[str, int, str]:

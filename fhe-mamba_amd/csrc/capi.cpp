@@ -13,6 +13,7 @@
 #include "ops.hpp"
 #include "params.hpp"
 #include "sampling.hpp"
+#include "status.hpp"
 
 // Every handle shares ownership of its context, so handles may be released
 // in any order (a garbage collector may finalise a context before its polys).
@@ -38,37 +39,8 @@ struct fhe_key {
 
 namespace {
 
-thread_local std::string g_err;
-
-template <typename F>
-int guard(F&& f) {
-  try {
-    f();
-    return FHE_OK;
-  } catch (const fhe::ArgError& e) {
-    g_err = e.what();
-    return FHE_ERR_ARG;
-  } catch (const fhe::HipError& e) {
-    g_err = e.what();
-    return FHE_ERR_HIP;
-  } catch (const fhe::StateError& e) {
-    g_err = e.what();
-    return FHE_ERR_STATE;
-  } catch (const std::out_of_range& e) {
-    g_err = e.what();
-    return FHE_ERR_RANGE;
-  } catch (const std::exception& e) {
-    g_err = e.what();
-    return FHE_ERR_INTERNAL;
-  } catch (...) {
-    g_err = "unknown error";
-    return FHE_ERR_INTERNAL;
-  }
-}
-
-void need(bool ok, const char* msg) {
-  if (!ok) throw fhe::ArgError(msg);
-}
+using fhe::guard;
+using fhe::need;
 
 size_t words(const fhe::Context& c, uint32_t npoly, uint32_t nlimb) {
   return (size_t)npoly * nlimb * c.n;
@@ -138,7 +110,7 @@ fhe_key* new_key(const std::shared_ptr<fhe::Context>& own) {
 
 extern "C" {
 
-const char* fhe_last_error(void) { return g_err.c_str(); }
+const char* fhe_last_error(void) { return fhe::last_error.c_str(); }
 int fhe_abi_version(void) { return 1; }
 
 int fhe_gen_moduli(uint32_t log_n, uint32_t depth, uint32_t scale_bits, uint32_t first_bits,

@@ -1,0 +1,423 @@
+// The selective scan over whole sequences and its gradients.
+//
+//   h_t = exp(g_t) h_{t-1} + w_t x_t B_t^T,   y_t = h_t C_t + D x_t
+//
+// In chunks of 64 tokens everything is a matrix product: the pairs of a chunk
+// (C B^T under a triangle of decays) with its x, the state before it with C,
+// and the state that it adds.  A wavefront keeps the state of 32 channels in
+// registers and walks its segment's chunks, so that x, B and C are read once
+// and y is written once.  A segment is a whole sequence where there are enough
+// of them to fill the chip; else a first sweep makes the state that each
+// segment adds, and a small kernel carries them along the sequence.
+//
+// Backwards the adjoint state A_t = exp(g_{t+1}) A_{t+1} + dy_t C_t^T is the
+// same recurrence in reversed time with B and C, x and dy in each other's
+// place, so the same sweeps give V_t = A_t B_t (dx = w V + D dy, dw = x . V),
+// dB and dC.  With M_ts the part of the loss in source s and target t,
+// dg_r is the sum of M over t >= r > s: what crosses the segment's end,
+// <A, h> there, plus the sums over t >= r of what enters at t less what leaves.
+// Terms with s = t are in neither, and the sums restart in every segment.
+#pragma clang fp contract(fast)
+#include "clear_scan.hpp"
+
+#include <algorithm>
+
+#include "context.hpp"
+
+namespace fhe::clear {
+namespace {
+
+// ---- segments of packed sequences ----
+// first[s]: sequence s's first item, first[seqs] the end.  Offsets are taken as
+// a partition whatever they hold: clamped to the tokens and made to rise.  The
+// tokens before the first and after the last sequence are items without one;
+// entries past the last item are empty.
+__global__ __launch_bounds__(256) void k_items(const int* offsets, int seqs, int tokens, int length,
+                                               bool keep_empty, int items, Item* table, int* first) {
+  __shared__ int most[256], sum[256];
+  __shared__ int carry_most, carry_sum;
+  const int i = threadIdx.x;
+  if (i == 0) {
+    carry_most = 0;
+    carry_sum = 0;
+  }
+  __syncthreads();
+  const int start0 = min(max(offsets[0], 0), tokens);
+  for (int s0 = 0; s0 < seqs; s0 += 256) {
+    const int s = s0 + i;
+    // ends of the sequences, rising
+    most[i] = s < seqs ? min(max(offsets[s + 1], start0), tokens) : 0;
+    __syncthreads();
+    for (int d = 1; d < 256; d *= 2) {
+      const int v = i >= d ? most[i - d] : 0;
+      __syncthreads();
+      most[i] = max(most[i], v);
+      __syncthreads();
+    }
+    const int before = max(carry_most, start0);
+    const int begin = i ? max(most[i - 1], before) : before, end = max(most[i], before);
+    int mine = 0;
+    if (s < seqs) mine = keep_empty ? max(1, (end - begin + length - 1) / length) : (end - begin + length - 1) / length;
+    sum[i] = mine;
+    __syncthreads();
+    for (int d = 1; d < 256; d *= 2) {
+      const int v = i >= d ? sum[i - d] : 0;
+      __syncthreads();
+      sum[i] += v;
+      __syncthreads();
+    }
+    const int at = carry_sum + sum[i] - mine;
+    if (s < seqs) {
+      first[s] = at;
+      for (int k = 0; k < mine; ++k)
+        table[at + k] = {s, begin + k * length, min(length, end - begin - k * length), 1};
+    }
+    __syncthreads();
+    if (i == 255) {
+      carry_most = end;
+      carry_sum += sum[255];
+    }
+    __syncthreads();
+  }
+  const int last = carry_most, count = carry_sum;
+  if (i == 0) first[seqs] = count;
+  // outside of the sequences
+  const int head = (start0 + length - 1) / length, tail = (tokens - last + length - 1) / length;
+  for (int k = i; k < items - count; k += 256) {
+    Item it = {-1, 0, 0, 0};
+    if (k < head) it = {-1, k * length, min(length, start0 - k * length), 0};
+    else if (k < head + tail)
+      it = {-1, last + (k - head) * length, min(length, tokens - last - (k - head) * length), 0};
+    table[count + k] = it;
+  }
+}
+
+// ---- states carried from segment to segment ----
+// In: the state that each item adds.  Out: the state before it (behind it in
+// reverse), and the sequence's last.  A thread an element; eight items are read
+// at a time, since only the sums depend on each other.
+__global__ __launch_bounds__(256) void k_join(float* states, const float* decay, const int* first,
+                                              int segments, int size, int per_head, int heads, bool rev,
+                                              const float* initial, float* last) {
+  const int e = blockIdx.x * 256 + threadIdx.x, seq = blockIdx.y;
+  if (e >= size) return;
+  const int head = e / per_head;
+  const int from = first ? first[seq] : seq * segments;
+  const int count = first ? first[seq + 1] - from : segments;
+  float run = initial ? initial[(int64_t)seq * size + e] : 0.0f;
+  for (int i0 = 0; i0 < count; i0 += 8) {
+    float add[8], keep[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = min(i0 + u, count - 1), item = from + (rev ? count - 1 - i : i);
+      add[u] = states[(int64_t)item * size + e];
+      keep[u] = decay[(int64_t)item * heads + head];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u < count) {
+        const int item = from + (rev ? count - 1 - i0 - u : i0 + u);
+        states[(int64_t)item * size + e] = run;
+        run = run * keep[u] + add[u];
+      }
+  }
+  if (last) last[(int64_t)seq * size + e] = run;
+}
+
+// ---- the ends of the gradients ----
+template <class T>
+__global__ __launch_bounds__(256) void k_sum_parts(const float* parts, int count, int64_t size, T* out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= size) return;
+  if (i + 4 <= size && size % 4 == 0) {
+    f32x4 sum = *reinterpret_cast<const f32x4*>(parts + i);
+    for (int p = 1; p < count; ++p) sum += *reinterpret_cast<const f32x4*>(parts + p * size + i);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[i + r] = (T)sum[r];
+    return;
+  }
+  for (int64_t k = i; k < min(i + 4, size); ++k) {
+    float sum = parts[k];
+    for (int p = 1; p < count; ++p) sum += parts[p * size + k];
+    out[k] = (T)sum;
+  }
+}
+
+__device__ __forceinline__ double block_sum(double v, double* scratch) {
+#pragma unroll
+  for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
+}
+
+// Gradients of write and log_decay of one item and head: the first summed over
+// the head's channels, the second from the segment's end backwards.
+__global__ __launch_bounds__(256) void k_gate_grads(SweepArgs a, const int* first, const float* entering,
+                                                    const float* leaving, const float* adjoint,
+                                                    const float* states, const float* last, float* dwrite,
+                                                    float* ddecay) {
+  __shared__ double scratch[4];
+  const int item_i = blockIdx.x, head = blockIdx.y;
+  const Item it = find_item(a, item_i);
+  if (it.count <= 0) return;
+  const int64_t token0 = item_token(a, it);
+  const int64_t size = (int64_t)a.head_dim * a.states, all = size * a.heads;
+  double carry = 0.0;
+  if (adjoint && it.live) {
+    const float* A = adjoint + (a.by_item ? item_i : it.seq) * all + head * size;
+    const bool more = a.by_item && (a.table ? item_i + 1 < first[it.seq + 1] : (item_i + 1) % a.segments != 0);
+    const float* h = (more ? states + (item_i + 1) * all : last + it.seq * all) + head * size;
+    for (int64_t e = threadIdx.x; e < size; e += 256) carry += (double)A[e] * h[e];
+    carry = block_sum(carry, scratch);
+  }
+  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  for (int end = it.count; end > 0; end -= 256) {
+    const int t = end - 1 - (int)threadIdx.x;  // the last token first
+    double v = 0.0;
+    if (t >= 0) {
+      float dw = 0.0f;
+      for (int p = 0; p < a.col_tiles; ++p) {
+        const int64_t at = ((int64_t)head * a.col_tiles + p) * a.all_tokens + token0 + t;
+        v += (double)entering[at] + (double)leaving[at];
+        dw += a.dwrite_part[at];
+      }
+      dwrite[(token0 + t) * a.heads + head] = dw;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const double up = __shfl_up(v, d);
+      if (lane >= d) v += up;
+    }
+    __syncthreads();
+    if (lane == 63) scratch[wave] = v;
+    __syncthreads();
+    double before = carry;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += scratch[w];
+      carry += scratch[w];
+    }
+    if (t >= 0) ddecay[(token0 + t) * a.heads + head] = (float)(before + v);
+  }
+}
+
+__global__ __launch_bounds__(256) void k_skip_grad(SweepArgs a, int items, float* dd) {
+  __shared__ double scratch[4];
+  const int head = blockIdx.x;
+  double v = 0.0;
+  for (int i = threadIdx.x; i < items; i += 256) {
+    const Item it = find_item(a, i);
+    if (!it.live) continue;
+    for (int p = 0; p < a.col_tiles; ++p)
+      v += a.dd_part[((int64_t)i * a.heads + head) * a.col_tiles + p];
+  }
+  v = block_sum(v, scratch);
+  if (threadIdx.x == 0) dd[head] = (float)v;
+}
+
+// ---- plan ----
+struct Plan {
+  int col_tiles, blocks, length, segments, items;
+  bool by_item;
+  // workspace, in bytes
+  size_t table, first, decays, states, adjoints, last, dwrite, gate_out, gate_in, dd, parts, total;
+};
+
+// Tokens of a segment: a whole sequence where the sequences alone give each CU
+// a workgroup or more, else as many chunks as leave about two a CU.
+int segment_length(int64_t all, int64_t longest, int seqs, int64_t per_item, bool packed) {
+  constexpr int64_t WANT = 512;
+  if (!packed && seqs * per_item >= WANT / 2) return (int)std::max<int64_t>(longest, 1);
+  const int64_t items = std::max<int64_t>(1, WANT / per_item);
+  const int64_t chunks = (all + CHUNK - 1) / CHUNK;
+  const int64_t len = std::max<int64_t>(1, (chunks + items - 1) / items) * CHUNK;
+  return (int)std::min<int64_t>(len, std::max<int64_t>(longest, 1));
+}
+
+Plan make_plan(const Scan& s, bool backward) {
+  Plan p{};
+  const bool packed = s.offsets != nullptr;
+  p.col_tiles = (s.head_dim + COLS - 1) / COLS;
+  p.blocks = (s.heads / s.groups * p.col_tiles + WAVES - 1) / WAVES;
+  const int64_t all = s.all_tokens();
+  p.length = segment_length(all, s.tokens, s.seqs, (int64_t)p.blocks * s.groups, packed);
+  p.segments = packed ? 0 : std::max<int>(1, (int)((s.tokens + p.length - 1) / p.length));
+  p.by_item = p.length < s.tokens;
+  p.items = packed ? (int)(s.tokens / p.length) + s.seqs + 2 : s.seqs * p.segments;
+  const size_t state = (size_t)s.heads * s.head_dim * s.states * 4;
+  const size_t rows = (size_t)s.heads * p.col_tiles;
+  auto take = [&](size_t bytes) {
+    const size_t at = p.total;
+    p.total += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  if (packed) {
+    p.table = take(sizeof(Item) * p.items);
+    p.first = take(4 * ((size_t)s.seqs + 1));
+  }
+  if (p.by_item) {
+    p.decays = take((size_t)p.items * s.heads * 4);
+    p.states = take(p.items * state);
+  }
+  if (backward) {
+    if (p.by_item) p.adjoints = take(p.items * state);
+    p.last = take(s.seqs * state);
+    p.dwrite = take(rows * all * 4);
+    p.gate_out = take(rows * all * 4);
+    p.gate_in = take(rows * all * 4);
+    p.dd = take(rows * p.items * 4);
+    p.parts = take((size_t)p.blocks * all * s.groups * s.states * 4);
+  }
+  return p;
+}
+
+// Whether every row of 16-byte pieces starts at a multiple of 16 bytes.
+bool is_wide(const Strided& t, int vec, bool packed) {
+  return reinterpret_cast<uintptr_t>(t.p) % 16 == 0 && (packed || t.seq % vec == 0) && t.tok % vec == 0 &&
+         t.head % vec == 0;
+}
+
+struct Sweep {
+  const Scan& s;
+  const Plan& p;
+  char* ws;
+  SweepArgs a{};
+
+  Sweep(const Scan& s_, const Plan& p_, char* ws_) : s(s_), p(p_), ws(ws_) {
+    a.heads = s.heads;
+    a.head_dim = s.head_dim;
+    a.states = s.states;
+    a.groups = s.groups;
+    a.col_tiles = p.col_tiles;
+    a.blocks = p.blocks;
+    a.tokens = s.offsets ? 0 : s.tokens;
+    a.all_tokens = s.all_tokens();
+    a.table = s.offsets ? at<const Item>(p.table) : nullptr;
+    a.segments = p.segments;
+    a.length = p.length;
+    a.write = s.write;
+    a.decay = s.decay;
+    a.by_item = p.by_item;
+    // 32-channel pieces of a head begin at multiples of 32
+    a.wide_out = (s.head_dim * elem()) % 16 == 0;
+  }
+  template <class T>
+  T* at(size_t offset) const {
+    return reinterpret_cast<T*>(ws + offset);
+  }
+  int elem() const { return s.dtype == BF16 ? 2 : 4; }
+  bool wide(const Strided& t) const { return is_wide(t, 16 / elem(), s.offsets != nullptr); }
+  SweepArgs with(const Strided& key, const Strided& query, const Strided& value,
+                 const Strided& other) const {
+    SweepArgs b = a;
+    b.key = key;
+    b.query = query;
+    b.value = value;
+    b.other = other;
+    b.wide_key = wide(key);
+    b.wide_query = wide(query);
+    b.wide_value = wide(value);
+    b.wide_other = wide(other);
+    return b;
+  }
+  const int* first() const { return s.offsets ? at<const int>(p.first) : nullptr; }
+
+  void make_items(hipStream_t stream) const {
+    if (!s.offsets) return;
+    k_items<<<1, 256, 0, stream>>>(s.offsets, s.seqs, (int)s.tokens, p.length, !p.by_item, p.items,
+                                   at<Item>(p.table), at<int>(p.first));
+    hip_check(hipGetLastError(), "scan segments");
+  }
+  // The states before (in reverse, behind) each segment at `states`, and each
+  // sequence's last at `last`.
+  void carry(const Strided& key, const Strided& value, bool rev, size_t states, const float* initial,
+             float* last, hipStream_t stream) const {
+    SweepArgs b = with(key, key, value, value);
+    b.state_out = at<float>(states);
+    b.decay_out = at<float>(p.decays);
+    launch_state_sweep(s.dtype, b, p.items, rev, stream);
+    const int size = s.heads * s.head_dim * s.states;
+    k_join<<<dim3((size + 255) / 256, s.seqs), 256, 0, stream>>>(
+        at<float>(states), at<float>(p.decays), first(), p.segments, size, s.head_dim * s.states, s.heads,
+        rev, initial, last);
+    hip_check(hipGetLastError(), "scan state join");
+  }
+  void sum_parts(void* out, hipStream_t stream) const {
+    const int64_t size = s.all_tokens() * s.groups * s.states;
+    if (!size) return;
+    const uint32_t grid = (uint32_t)((size + 1023) / 1024);
+    if (s.dtype == BF16)
+      k_sum_parts<<<grid, 256, 0, stream>>>(at<float>(p.parts), p.blocks, size, (bf16*)out);
+    else
+      k_sum_parts<<<grid, 256, 0, stream>>>(at<float>(p.parts), p.blocks, size, (float*)out);
+    hip_check(hipGetLastError(), "scan gradient sums");
+  }
+};
+
+}  // namespace
+
+size_t scan_workspace(const Scan& s, bool backward) { return make_plan(s, backward).total; }
+
+void scan(const Scan& s, void* y, float* final_state, void* workspace, hipStream_t stream) {
+  const Plan p = make_plan(s, false);
+  const Sweep sweep(s, p, (char*)workspace);
+  sweep.make_items(stream);
+  if (p.by_item) sweep.carry(s.b, s.x, false, p.states, s.initial, final_state, stream);
+  SweepArgs a = sweep.with(s.b, s.c, s.x, s.x);
+  a.wide_out = a.wide_out && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  a.d = s.d;
+  a.state_in = p.by_item ? sweep.at<float>(p.states) : s.initial;
+  a.state_out = p.by_item ? nullptr : final_state;
+  a.out = y;
+  launch_value_sweep(s.dtype, a, p.items, false, stream);
+}
+
+void scan_backward(const Scan& s, const ScanGrads& g, void* workspace, hipStream_t stream) {
+  const Plan p = make_plan(s, true);
+  const Sweep sweep(s, p, (char*)workspace);
+  float* last = g.dfinal ? sweep.at<float>(p.last) : nullptr;
+  sweep.make_items(stream);
+  if (p.by_item) {
+    sweep.carry(s.b, s.x, false, p.states, s.initial, sweep.at<float>(p.last), stream);
+    sweep.carry(s.c, g.dy, true, p.adjoints, g.dfinal, g.dinitial, stream);
+  }
+  const float* states = p.by_item ? sweep.at<float>(p.states) : s.initial;
+  const float* adjoints = p.by_item ? sweep.at<float>(p.adjoints) : g.dfinal;
+
+  SweepArgs a = sweep.with(s.c, s.b, g.dy, s.x);
+  a.wide_out = a.wide_out && reinterpret_cast<uintptr_t>(g.dx) % 16 == 0;
+  a.d = s.d;
+  a.state_in = adjoints;
+  a.state_out = p.by_item ? nullptr : g.dinitial;
+  a.out = g.dx;
+  a.dwrite_part = sweep.at<float>(p.dwrite);
+  a.gate_part = sweep.at<float>(p.gate_out);
+  a.dd_part = sweep.at<float>(p.dd);
+  launch_value_sweep(s.dtype, a, p.items, true, stream);
+
+  SweepArgs c = sweep.with(s.b, s.c, s.x, g.dy);
+  c.state_in = states;
+  c.state_out = p.by_item ? nullptr : last;
+  c.out = sweep.at<float>(p.parts);
+  c.gate_part = sweep.at<float>(p.gate_in);
+  launch_query_sweep(s.dtype, c, p.items, false, stream);
+  sweep.sum_parts(g.dc, stream);
+
+  SweepArgs b = sweep.with(s.c, s.b, g.dy, s.x);
+  b.state_in = adjoints;
+  b.out = sweep.at<float>(p.parts);
+  launch_query_sweep(s.dtype, b, p.items, true, stream);
+  sweep.sum_parts(g.db, stream);
+
+  k_gate_grads<<<dim3(p.items, s.heads), 256, 0, stream>>>(
+      a, sweep.first(), sweep.at<float>(p.gate_in), sweep.at<float>(p.gate_out), adjoints, states,
+      sweep.at<float>(p.last), g.dwrite, g.ddecay);
+  hip_check(hipGetLastError(), "scan gate gradients");
+  if (g.dd) {
+    k_skip_grad<<<s.heads, 256, 0, stream>>>(a, p.items, g.dd);
+    hip_check(hipGetLastError(), "scan skip gradient");
+  }
+}
+
+}  // namespace fhe::clear

@@ -97,6 +97,18 @@ SIGNATURES = {
     "fhe_keygen_galois": [_p, _p, _u32, _u64, _pp],
     "fhe_encrypt": [_p, _p, _p, _u64],
     "fhe_decrypt": [_p, _p, _p],
+    # structures go over as their packed bytes (clear.py)
+    "fhe_ssm_scan_workspace": [_p, _int, _p],
+    "fhe_ssm_scan": [_p, _p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_ssm_scan_backward": [_p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_ssm_step": [_p, _p, _p],
+    "fhe_causal_conv": [_p, _p, _p, _p],
+    "fhe_causal_conv_workspace": [_p, _p],
+    "fhe_causal_conv_backward": [_p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_causal_conv_step": [_p, _p, _p],
+    "fhe_token_logprobs_workspace": [_p, _p],
+    "fhe_token_logprobs": [_p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_token_logprobs_backward": [_p, _p, _p, _p, _p, _p, _p, _p],
 }
 
 

@@ -346,6 +346,151 @@ int fhe_encrypt(fhe_poly *ct, const fhe_poly *pk, const fhe_poly *pt,
                 uint64_t seed);
 int fhe_decrypt(fhe_poly *pt, const fhe_poly *ct, const int64_t *s_coef);
 
+/* ---- Mamba-2 in the clear ------------------------------------------------
+ * The layer's operators on plain device memory: what the client runs on its
+ * own prompt, and what fits and checks the polynomials (the reference does both
+ * in PyTorch on the host, src/fhemamba/reference.py:182-339).  No context:
+ * every call takes a hipStream_t of the current device (NULL: its null stream),
+ * enqueues there and returns; nothing is allocated and nothing is waited for,
+ * so calls may be captured into a graph.  Workspaces are the caller's, of at
+ * least the size the *_workspace call gives, 256-byte aligned, and free again
+ * when the call's work is done.  Outputs are contiguous and must not overlap
+ * inputs; *_step updates its state in place.  Activations are FHE_F32 or
+ * FHE_BF16; gates, states, weights and their gradients are 32-bit floats. */
+enum { FHE_F32 = 0, FHE_BF16 = 1 };
+enum { FHE_MAX_STATES = 128, FHE_MAX_TAPS = 8, FHE_MAX_TOP = 32 };
+
+/* [sequence][token][head or group] of contiguous runs, strides in elements.
+ * Where sequences are packed, stride[0] is not used. */
+typedef struct {
+  const void *data;
+  int64_t stride[3];
+} fhe_strided;
+
+/* h_t = exp(log_decay_t) h_{t-1} + (write_t x_t) b_t^T,  y_t = h_t c_t + d x_t
+ * for every head, h [head_dim][states]; group g of b and c serves heads
+ * g * heads / groups and up.  log_decay <= 0 is meant; -infinity forgets the
+ * state.  offsets NULL: `seqs` sequences of `tokens` each.  Else the tokens
+ * [offsets[i], offsets[i+1]) are sequence i of `tokens` in all; tokens outside
+ * of every sequence give zeros.  tokens < 2^31, states <= FHE_MAX_STATES. */
+typedef struct {
+  uint32_t dtype, seqs, heads, head_dim, states, groups;
+  int64_t tokens;
+  const int32_t *offsets; /* device, [seqs + 1], or NULL */
+  fhe_strided x, b, c;    /* dtype */
+  fhe_strided write, log_decay;
+  const float *d;       /* [heads] or NULL */
+  const float *initial; /* [seqs][heads][head_dim][states], or NULL: zeros */
+} fhe_scan_args;
+
+int fhe_ssm_scan_workspace(const fhe_scan_args *args, int backward,
+                           size_t *bytes);
+/* y [tokens][heads][head_dim] (for each sequence), final_state as `initial`
+ * or NULL. */
+int fhe_ssm_scan(const fhe_scan_args *args, void *y, float *final_state,
+                 void *workspace, size_t bytes, void *hip_stream);
+/* From dy (strided as x) and dfinal (as `initial`, or NULL: zeros).  dx as y;
+ * dwrite and dlog_decay [tokens][heads]; db and dc [tokens][groups][states] in
+ * dtype; dd [heads] or NULL; dinitial as `initial` or NULL.  Sums have a fixed
+ * order: the same inputs give the same bits. */
+typedef struct {
+  fhe_strided dy;
+  const float *dfinal;
+  void *dx;
+  float *dwrite, *dlog_decay;
+  void *db, *dc;
+  float *dd, *dinitial;
+} fhe_scan_grads;
+int fhe_ssm_scan_backward(const fhe_scan_args *args,
+                          const fhe_scan_grads *grads, void *workspace,
+                          size_t bytes, void *hip_stream);
+
+/* One token of each of `requests` requests.  slots [requests] (device, or NULL:
+ * 0, 1, ...) names its row of the state [cache][heads][head_dim][states], which
+ * is updated in place; no two requests may name one row.  A slot outside of
+ * [0, cache) is padding: y is zero and no state changes.  The token strides are
+ * the requests'; stride[0] is not used. */
+typedef struct {
+  uint32_t dtype, requests, cache, heads, head_dim, states, groups;
+  const int32_t *slots;
+  fhe_strided x, b, c;
+  fhe_strided write, log_decay;
+  const float *d;
+  float *state;
+} fhe_ssm_step_args;
+int fhe_ssm_step(const fhe_ssm_step_args *args, void *y, void *hip_stream);
+
+/* y_t = act(bias + sum_k weight_k x_{t - taps + 1 + k}) for every channel, act
+ * silu or nothing; weight [channels][taps], 2 <= taps <= FHE_MAX_TAPS.  Before a
+ * sequence's first token lie its initial inputs [taps - 1][channels], oldest
+ * first (NULL: zeros).  Sequences as in fhe_scan_args; stride[2] is not used. */
+typedef struct {
+  uint32_t dtype, seqs, channels, taps;
+  int64_t tokens;
+  const int32_t *offsets;
+  fhe_strided x;
+  const float *weight, *bias; /* bias may be NULL */
+  const void *initial;        /* dtype */
+  int silu;
+} fhe_conv_args;
+/* final_state: each sequence's last taps - 1 inputs, as `initial`, or NULL. */
+int fhe_causal_conv(const fhe_conv_args *args, void *y, void *final_state,
+                    void *hip_stream);
+int fhe_causal_conv_workspace(const fhe_conv_args *args, size_t *bytes);
+/* dx as y, dweight as weight, dbias [channels] or NULL, dinitial as `initial`
+ * or NULL; dfinal is the gradient of final_state, or NULL: zeros. */
+typedef struct {
+  fhe_strided dy;
+  const void *dfinal;
+  void *dx;
+  float *dweight, *dbias;
+  void *dinitial;
+} fhe_conv_grads;
+int fhe_causal_conv_backward(const fhe_conv_args *args,
+                             const fhe_conv_grads *grads, void *workspace,
+                             size_t bytes, void *hip_stream);
+/* The single-token form on state [cache][taps - 1][channels], slots as in
+ * fhe_ssm_step_args. */
+typedef struct {
+  uint32_t dtype, requests, cache, channels, taps;
+  const int32_t *slots;
+  fhe_strided x;
+  const float *weight, *bias;
+  void *state;
+  int silu;
+} fhe_conv_step_args;
+int fhe_causal_conv_step(const fhe_conv_step_args *args, void *y,
+                         void *hip_stream);
+
+/* Rows of logits [rows][vocab] (row_stride elements apart): the log probability
+ * of each row's target, the entropy of its distribution, its largest logit and
+ * the logarithm of the sum of exponentials relative to that, and the `top` <= FHE_MAX_TOP likeliest tokens with their log probabilities, the lower
+ * index first among equals.  A logit of -infinity is a token that is not
+ * allowed; a row of nothing else has log probability -infinity and entropy 0.
+ * targets (NULL: none) below 0 are left out (log probability 0); one of vocab or
+ * more gives NaN. */
+typedef struct {
+  uint32_t dtype, top;
+  int64_t rows, vocab, row_stride;
+  const void *logits;
+  const int64_t *targets;
+} fhe_logprob_args;
+typedef struct {
+  float *logprob, *entropy, *peak, *log_sum; /* [rows] */
+  float *top_logprob;             /* [rows][top] */
+  int32_t *top_index;
+} fhe_logprob_out;
+int fhe_token_logprobs_workspace(const fhe_logprob_args *args, size_t *bytes);
+int fhe_token_logprobs(const fhe_logprob_args *args, const fhe_logprob_out *out,
+                       void *workspace, size_t bytes, void *hip_stream);
+/* dlogits [rows][vocab] in dtype from the gradients of logprob and entropy
+ * [rows] (either may be NULL: zeros) and what the forward call gave. */
+int fhe_token_logprobs_backward(const fhe_logprob_args *args,
+                                const float *peak, const float *log_sum,
+                                const float *entropy, const float *dlogprob,
+                                const float *dentropy, void *dlogits,
+                                void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif
