@@ -155,7 +155,7 @@ __device__ __forceinline__ double block_sum(double v, double* scratch) {
 // Gradients of write and log_decay of one item and head: the first summed over
 // the head's channels, the second from the segment's end backwards.
 __global__ __launch_bounds__(256) void k_gate_grads(SweepArgs a, const int* first, const float* entering,
-                                                    const float* leaving, const float* adjoint,
+                                                    int entering_tiles, const float* leaving, const float* adjoint,
                                                     const float* states, const float* last, float* dwrite,
                                                     float* ddecay) {
   __shared__ double scratch[4];
@@ -180,9 +180,11 @@ __global__ __launch_bounds__(256) void k_gate_grads(SweepArgs a, const int* firs
       float dw = 0.0f;
       for (int p = 0; p < a.col_tiles; ++p) {
         const int64_t at = ((int64_t)head * a.col_tiles + p) * a.all_tokens + token0 + t;
-        v += (double)entering[at] + (double)leaving[at];
+        v += (double)leaving[at];
         dw += a.dwrite_part[at];
       }
+      for (int p = 0; p < entering_tiles; ++p)
+        v += (double)entering[((int64_t)head * entering_tiles + p) * a.all_tokens + token0 + t];
       dwrite[(token0 + t) * a.heads + head] = dw;
     }
 #pragma unroll
@@ -217,18 +219,34 @@ __global__ __launch_bounds__(256) void k_skip_grad(SweepArgs a, int items, float
 }
 
 // ---- plan ----
+// How a sweep cuts heads into wavefronts and workgroups.
+struct Cut {
+  int cols, col_tiles, blocks;
+  Cut() = default;
+  Cut(const Scan& s, int cols_) : cols(cols_) {
+    col_tiles = (s.head_dim + cols - 1) / cols;
+    blocks = (s.heads / s.groups * col_tiles + WAVES - 1) / WAVES;
+  }
+};
+
 struct Plan {
-  int col_tiles, blocks, length, segments, items;
+  Cut value, query;
+  int length, segments, items;
   bool by_item;
   // workspace, in bytes
   size_t table, first, decays, states, adjoints, last, dwrite, gate_out, gate_in, dd, parts, total;
 };
 
-// Tokens of a segment: a whole sequence where the sequences alone give each CU
-// a workgroup or more, else as many chunks as leave about two a CU.
+// Tokens of a segment: a whole sequence where the sequences alone fill half of
+// the chip's places for workgroups (two a CU), else as many chunks as leave
+// about three workgroups a CU: lengths are whole chunks and sequences ragged, and
+// with fewer the last round is half empty.  Each segment's states are written
+// and read twice, which holds the number down.  us of all launches, two / three /
+// four a CU: 30011 packed tokens of 24 heads 314 / 265 / 265, the gradients of
+// 4 x 2048 349 / 313 / 314.
 int segment_length(int64_t all, int64_t longest, int seqs, int64_t per_item, bool packed) {
-  constexpr int64_t WANT = 512;
-  if (!packed && seqs * per_item >= WANT / 2) return (int)std::max<int64_t>(longest, 1);
+  constexpr int64_t WANT = 768, ENOUGH = 256;
+  if (!packed && seqs * per_item >= ENOUGH) return (int)std::max<int64_t>(longest, 1);
   const int64_t items = std::max<int64_t>(1, WANT / per_item);
   const int64_t chunks = (all + CHUNK - 1) / CHUNK;
   const int64_t len = std::max<int64_t>(1, (chunks + items - 1) / items) * CHUNK;
@@ -238,15 +256,18 @@ int segment_length(int64_t all, int64_t longest, int seqs, int64_t per_item, boo
 Plan make_plan(const Scan& s, bool backward) {
   Plan p{};
   const bool packed = s.offsets != nullptr;
-  p.col_tiles = (s.head_dim + COLS - 1) / COLS;
-  p.blocks = (s.heads / s.groups * p.col_tiles + WAVES - 1) / WAVES;
+  p.value = Cut(s, VALUE_COLS);
+  // 64 channels take all of a head's registers there are, and halve the sums
+  // over wavefronts and the parts: 146 us for both sweeps and their sums at
+  // 4 x 2048 tokens of 24 heads of 64, 32 channels 183
+  p.query = Cut(s, s.head_dim <= 32 ? 32 : 64);
   const int64_t all = s.all_tokens();
-  p.length = segment_length(all, s.tokens, s.seqs, (int64_t)p.blocks * s.groups, packed);
+  p.length = segment_length(all, s.tokens, s.seqs, (int64_t)p.value.blocks * s.groups, packed);
   p.segments = packed ? 0 : std::max<int>(1, (int)((s.tokens + p.length - 1) / p.length));
   p.by_item = p.length < s.tokens;
   p.items = packed ? (int)(s.tokens / p.length) + s.seqs + 2 : s.seqs * p.segments;
   const size_t state = (size_t)s.heads * s.head_dim * s.states * 4;
-  const size_t rows = (size_t)s.heads * p.col_tiles;
+  const size_t rows = (size_t)s.heads * p.value.col_tiles;
   auto take = [&](size_t bytes) {
     const size_t at = p.total;
     p.total += (bytes + 255) / 256 * 256;
@@ -265,9 +286,9 @@ Plan make_plan(const Scan& s, bool backward) {
     p.last = take(s.seqs * state);
     p.dwrite = take(rows * all * 4);
     p.gate_out = take(rows * all * 4);
-    p.gate_in = take(rows * all * 4);
+    p.gate_in = take((size_t)s.heads * p.query.col_tiles * all * 4);
     p.dd = take(rows * p.items * 4);
-    p.parts = take((size_t)p.blocks * all * s.groups * s.states * 4);
+    p.parts = take((size_t)p.query.blocks * all * s.groups * s.states * 4);
   }
   return p;
 }
@@ -289,8 +310,6 @@ struct Sweep {
     a.head_dim = s.head_dim;
     a.states = s.states;
     a.groups = s.groups;
-    a.col_tiles = p.col_tiles;
-    a.blocks = p.blocks;
     a.tokens = s.offsets ? 0 : s.tokens;
     a.all_tokens = s.all_tokens();
     a.table = s.offsets ? at<const Item>(p.table) : nullptr;
@@ -299,8 +318,6 @@ struct Sweep {
     a.write = s.write;
     a.decay = s.decay;
     a.by_item = p.by_item;
-    // 32-channel pieces of a head begin at multiples of 32
-    a.wide_out = (s.head_dim * elem()) % 16 == 0;
   }
   template <class T>
   T* at(size_t offset) const {
@@ -308,9 +325,12 @@ struct Sweep {
   }
   int elem() const { return s.dtype == BF16 ? 2 : 4; }
   bool wide(const Strided& t) const { return is_wide(t, 16 / elem(), s.offsets != nullptr); }
-  SweepArgs with(const Strided& key, const Strided& query, const Strided& value,
+  SweepArgs with(const Cut& cut, const Strided& key, const Strided& query, const Strided& value,
                  const Strided& other) const {
     SweepArgs b = a;
+    b.cols = cut.cols;
+    b.col_tiles = cut.col_tiles;
+    b.blocks = cut.blocks;
     b.key = key;
     b.query = query;
     b.value = value;
@@ -333,7 +353,8 @@ struct Sweep {
   // sequence's last at `last`.
   void carry(const Strided& key, const Strided& value, bool rev, size_t states, const float* initial,
              float* last, hipStream_t stream) const {
-    SweepArgs b = with(key, key, value, value);
+    SweepArgs b = with(p.value, key, key, value, value);
+    b.wide_out = true;
     b.state_out = at<float>(states);
     b.decay_out = at<float>(p.decays);
     launch_state_sweep(s.dtype, b, p.items, rev, stream);
@@ -348,9 +369,9 @@ struct Sweep {
     if (!size) return;
     const uint32_t grid = (uint32_t)((size + 1023) / 1024);
     if (s.dtype == BF16)
-      k_sum_parts<<<grid, 256, 0, stream>>>(at<float>(p.parts), p.blocks, size, (bf16*)out);
+      k_sum_parts<<<grid, 256, 0, stream>>>(at<float>(p.parts), p.query.blocks, size, (bf16*)out);
     else
-      k_sum_parts<<<grid, 256, 0, stream>>>(at<float>(p.parts), p.blocks, size, (float*)out);
+      k_sum_parts<<<grid, 256, 0, stream>>>(at<float>(p.parts), p.query.blocks, size, (float*)out);
     hip_check(hipGetLastError(), "scan gradient sums");
   }
 };
@@ -364,8 +385,8 @@ void scan(const Scan& s, void* y, float* final_state, void* workspace, hipStream
   const Sweep sweep(s, p, (char*)workspace);
   sweep.make_items(stream);
   if (p.by_item) sweep.carry(s.b, s.x, false, p.states, s.initial, final_state, stream);
-  SweepArgs a = sweep.with(s.b, s.c, s.x, s.x);
-  a.wide_out = a.wide_out && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  SweepArgs a = sweep.with(p.value, s.b, s.c, s.x, s.x);
+  a.wide_out = s.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
   a.d = s.d;
   a.state_in = p.by_item ? sweep.at<float>(p.states) : s.initial;
   a.state_out = p.by_item ? nullptr : final_state;
@@ -385,8 +406,8 @@ void scan_backward(const Scan& s, const ScanGrads& g, void* workspace, hipStream
   const float* states = p.by_item ? sweep.at<float>(p.states) : s.initial;
   const float* adjoints = p.by_item ? sweep.at<float>(p.adjoints) : g.dfinal;
 
-  SweepArgs a = sweep.with(s.c, s.b, g.dy, s.x);
-  a.wide_out = a.wide_out && reinterpret_cast<uintptr_t>(g.dx) % 16 == 0;
+  SweepArgs a = sweep.with(p.value, s.c, s.b, g.dy, s.x);
+  a.wide_out = s.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(g.dx) % 16 == 0;
   a.d = s.d;
   a.state_in = adjoints;
   a.state_out = p.by_item ? nullptr : g.dinitial;
@@ -396,22 +417,24 @@ void scan_backward(const Scan& s, const ScanGrads& g, void* workspace, hipStream
   a.dd_part = sweep.at<float>(p.dd);
   launch_value_sweep(s.dtype, a, p.items, true, stream);
 
-  SweepArgs c = sweep.with(s.b, s.c, s.x, g.dy);
+  SweepArgs c = sweep.with(p.query, s.b, s.c, s.x, g.dy);
   c.state_in = states;
   c.state_out = p.by_item ? nullptr : last;
   c.out = sweep.at<float>(p.parts);
+  c.wide_out = s.states % 4 == 0;
   c.gate_part = sweep.at<float>(p.gate_in);
   launch_query_sweep(s.dtype, c, p.items, false, stream);
   sweep.sum_parts(g.dc, stream);
 
-  SweepArgs b = sweep.with(s.c, s.b, g.dy, s.x);
+  SweepArgs b = sweep.with(p.query, s.c, s.b, g.dy, s.x);
   b.state_in = adjoints;
   b.out = sweep.at<float>(p.parts);
+  b.wide_out = s.states % 4 == 0;
   launch_query_sweep(s.dtype, b, p.items, true, stream);
   sweep.sum_parts(g.db, stream);
 
   k_gate_grads<<<dim3(p.items, s.heads), 256, 0, stream>>>(
-      a, sweep.first(), sweep.at<float>(p.gate_in), sweep.at<float>(p.gate_out), adjoints, states,
+      a, sweep.first(), sweep.at<float>(p.gate_in), p.query.col_tiles, sweep.at<float>(p.gate_out), adjoints, states,
       sweep.at<float>(p.last), g.dwrite, g.ddecay);
   hip_check(hipGetLastError(), "scan gate gradients");
   if (g.dd) {

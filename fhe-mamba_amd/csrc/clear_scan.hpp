@@ -9,8 +9,8 @@
 namespace fhe::clear {
 
 constexpr int CHUNK = 64, TILES = CHUNK / 16;  // tokens of a chunk, its tiles
-constexpr int COLS = 32;                       // head channels of a wavefront
 constexpr int WAVES = 4;                       // wavefronts of a workgroup
+constexpr int VALUE_COLS = 32;                 // head channels of a value sweep's wavefront
 
 // Consecutive tokens of one sequence.  `live` is 0 for tokens outside of every
 // sequence, whose results are zeros; such an item has no sequence.
@@ -20,7 +20,8 @@ struct Item {
 
 struct SweepArgs {
   int heads, head_dim, states, groups;
-  int col_tiles;        // wavefronts a head: ceil(head_dim / COLS)
+  int cols;             // head channels of a wavefront: 32 or 64
+  int col_tiles;        // wavefronts a head: ceil(head_dim / cols)
   int blocks;           // workgroups a group
   int64_t tokens;       // per sequence (0: packed)
   int64_t all_tokens;
@@ -62,64 +63,86 @@ __device__ __forceinline__ float exp2d(double d) { return __builtin_amdgcn_exp2f
 // product does not.  Forward, source s reaches target t >= s; in reverse the
 // targets are the earlier ones.
 struct Gates {
-  double g[CHUNK], e[TILES];
-  float src[CHUNK], dst[CHUNK], w[CHUNK];
-  float cross[TILES][TILES];  // [i][j], i > j: start of tile i from the end of tile j
-  float src_out[TILES];       // from a source's tile to the state behind the chunk
-  float dst_in[TILES];        // from the state before the chunk to a target's tile
-  float total;
-  float pad[3];
+  double g[CHUNK];
+  float src[CHUNK], w[CHUNK];
+  float steps[26];
+  double ends[TILES + 1];  // of the tiles, after 0
+
+  // start of tile i from the end of tile j < i
+  __device__ __forceinline__ float cross(int i, int j) const { return steps[4 * i + j]; }
+  // a tile's start from the chunk's, the chunk's end from that of the tile
+  __device__ __forceinline__ float first(int i) const { return steps[16 + i]; }
+  __device__ __forceinline__ float last(int i) const { return steps[20 + i]; }
+  __device__ __forceinline__ float total() const { return steps[24]; }
+  // to token `tok` of tile i from its tile's end on the sources' side
+  template <bool REV>
+  __device__ __forceinline__ float inside(int i, int tok) const {
+    return exp2d(REV ? ends[i + 1] - g[tok] : g[tok] - ends[i]);
+  }
+  // from the state before the chunk to that end of tile i
+  template <bool REV>
+  __device__ __forceinline__ float into(int i) const {
+    return REV ? last(i) : first(i);
+  }
 };
 
-// Fills `t` for tokens [first, first + n) (n <= CHUNK; the rest decay by
-// nothing and write nothing).  One wavefront, a lane a token.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Sums over the lanes up to each, without LDS.
+__device__ __forceinline__ double wave_scan(double v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: within sixteen lanes
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // row_bcast 15: of lanes 0 and 32 up to the next sixteen
+  return dpp_add<0x143, 0xc>(v);  // row_bcast 31
+}
+
+__device__ __forceinline__ double read_lane(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Fills `t` from one token's gates in each lane (tokens that are not there decay
+// by nothing and write nothing).
 template <bool REV>
-__device__ __forceinline__ void make_gates(Gates& t, const float* write, int64_t write_tok,
-                                           const float* decay, int64_t decay_tok, int n) {
-  const int lane = lane_id();
-  float g = 0.0f, w = 0.0f;
-  if (lane < n) {
-    g = decay[lane * decay_tok];
-    w = write[lane * write_tok];
-  }
+__device__ __forceinline__ void make_gates(Gates& t, float g, float w) {
+  const int lane = lane_id(), tile = lane >> 4;
   // A decay of exp(-1e4) is 0 in 32 bits as exp(-inf) is, and its sums are finite.
-  double sum = (double)(g < -1e4f ? -1e4f : g) * 1.4426950408889634;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const double up = __shfl_up(sum, d);
-    if (lane >= d) sum += up;
-  }
+  const double sum = wave_scan((double)(g < -1e4f ? -1e4f : g) * 1.4426950408889634);
+  // the sum at the end of each tile, 0 before the first
+  const double e0 = read_lane(sum, 15), e1 = read_lane(sum, 31), e2 = read_lane(sum, 47), e3 = read_lane(sum, 63);
+  auto before = [&](int i) { return i == 0 ? 0.0 : i == 1 ? e0 : i == 2 ? e1 : i == 3 ? e2 : e3; };
   t.g[lane] = sum;
   t.w[lane] = w;
-  if ((lane & 15) == 15) t.e[lane >> 4] = sum;
-  wave_sync();
-  const int tile = lane >> 4;
-  const double start = tile ? t.e[tile - 1] : 0.0, end = t.e[tile], all = t.e[TILES - 1];
-  const float in = exp2d(sum - start), out = exp2d(end - sum);
-  t.src[lane] = REV ? in : out * w;
-  t.dst[lane] = REV ? out : in;
-  if (lane < TILES * TILES) {
-    const int i = lane / TILES, j = lane % TILES;
-    t.cross[i][j] = i > j ? exp2d(t.e[i - 1] - t.e[j]) : 0.0f;
-  } else if (lane < TILES * TILES + TILES) {
-    const int i = lane - TILES * TILES;
-    const float first = exp2d(i ? t.e[i - 1] : 0.0), last = exp2d(all - t.e[i]);
-    t.src_out[i] = REV ? first : last;
-    t.dst_in[i] = REV ? last : first;
-  } else if (lane == TILES * TILES + TILES) {
-    t.total = exp2d(all);
-  }
+  t.src[lane] = REV ? exp2d(sum - before(tile)) : exp2d(before(tile + 1) - sum) * w;
+  // lanes 0 .. 15: start of tile i from the end of tile j; 16 .. 19: start of
+  // tile i from the chunk's; 20 .. 23: the chunk's end from that of tile i; 24: all
+  const int i = lane < 16 ? lane >> 2 : lane & 3, j = lane & 3;
+  const double to = lane < 20 ? before(i) : e3;
+  const double from = lane < 16 ? before(j + 1) : lane < 20 || lane >= 24 ? 0.0 : before(i + 1);
+  const float f = exp2d(to - from);
+  if (lane < 25) t.steps[lane] = f;
+  if (lane <= TILES) t.ends[lane] = before(lane);
   wave_sync();
 }
 
 // A tile of products, rows the sources 16 j + 4 q + r and columns the targets
 // 16 i + l, times their decays and the sources' weights; zeros where the
 // target does not see the source.
+// `inside`: Gates::inside of the lane's target.
 template <bool REV>
-__device__ __forceinline__ f32x4 decayed(const Gates& t, f32x4 s, int i, int j) {
+__device__ __forceinline__ f32x4 decayed(const Gates& t, f32x4 s, int i, int j, float inside) {
   const int q = lane_id() >> 4, l = lane_id() & 15;
   if (i != j) {
-    const float m = t.dst[16 * i + l] * (REV ? t.cross[j][i] : t.cross[i][j]);
+    const float m = inside * (REV ? t.cross(j, i) : t.cross(i, j));
     const f32x4 v = *reinterpret_cast<const f32x4*>(&t.src[16 * j + 4 * q]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) s[r] *= m * v[r];
@@ -138,11 +161,12 @@ __device__ __forceinline__ f32x4 decayed(const Gates& t, f32x4 s, int i, int j) 
 
 // The factors from the sources of tiles 2 m and 2 m + 1 to the state behind the
 // chunk, in the order of a fragment.
+template <bool REV>
 __device__ __forceinline__ f32x8 to_state(const Gates& t, int m) {
   const int q = lane_id() >> 4;
   f32x4 a = *reinterpret_cast<const f32x4*>(&t.src[32 * m + 4 * q]);
   f32x4 b = *reinterpret_cast<const f32x4*>(&t.src[32 * m + 16 + 4 * q]);
-  const float fa = t.src_out[2 * m], fb = t.src_out[2 * m + 1];
+  const float fa = REV ? t.first(2 * m) : t.last(2 * m), fb = REV ? t.first(2 * m + 1) : t.last(2 * m + 1);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     a[r] *= fa;
@@ -151,20 +175,46 @@ __device__ __forceinline__ f32x8 to_state(const Gates& t, int m) {
   return join(a, b);
 }
 
-// Copies tokens [0, n) of `width` contiguous elements into rows of an LDS tile
-// of 64 rows and PITCH elements, `span` of them filled: zeros past the width and
-// the count.  `threads` threads, this one the `thread`-th.
-template <class T, int PITCH>
-__device__ __forceinline__ void stage(T* tile, const T* src, int64_t tok, int n, int width,
-                                      int span, bool wide, int thread, int threads) {
-  constexpr int VEC = Num<T>::VEC;
-  const int per = span / VEC;
-  for (int i = thread; i < CHUNK * per; i += threads) {
-    const int row = i / per, col = i % per * VEC;
-    const u32x4 v = load16(src + row * tok + col, row < n ? width - col : 0, wide);
-    *reinterpret_cast<u32x4*>(tile + row * PITCH + col) = v;
+// Tokens [0, n) of `width` contiguous elements on their way into the rows of an LDS
+// tile of 64 rows and SPAN columns: zeros past the width and the count.  THREADS threads; loading and storing are apart so that a
+// chunk's loads are all in flight at once.
+//
+// FULL: every row has SPAN elements and is wide, and there is a row 0.
+template <class T, int SPAN, int THREADS, bool FULL>
+struct Stage {
+  static constexpr int VEC = Num<T>::VEC, PER = SPAN / VEC, PIECES = CHUNK * PER / THREADS;
+  static_assert(CHUNK * PER % THREADS == 0);
+  u32x4 v[PIECES];
+
+  __device__ __forceinline__ void load(const T* src, int64_t tok, int n, int width, bool wide, int thread) {
+    const int row = thread / PER, col = thread % PER * VEC;
+    constexpr int STEP = THREADS / PER;
+    if constexpr (FULL) {
+      // no branches: rows past the last are that one again, and then zeros.  A
+      // chunk's offsets take 32 bits (is_full).
+      const uint32_t pitch = (uint32_t)(tok * sizeof(T));
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        const uint32_t at = (uint32_t)max(min(row + k * STEP, n - 1), 0) * pitch + col * (uint32_t)sizeof(T);
+        v[k] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(src) + at);
+      }
+      if (n < CHUNK) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k)
+          if (row + k * STEP >= n) v[k] = u32x4{0, 0, 0, 0};
+      }
+    } else {
+      const T* p = src + row * tok + col;
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) v[k] = load16(p + k * STEP * tok, row + k * STEP < n ? width - col : 0, wide);
+    }
   }
-}
+  __device__ __forceinline__ void store(T* tile, int thread) const {
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+      *reinterpret_cast<u32x4*>(tile + Tile<T, SPAN>::at(thread / PER + k * (THREADS / PER), thread % PER)) = v[k];
+  }
+};
 
 // Sum over the sixteen lanes of one lane group, in each of them.
 __device__ __forceinline__ float sum16(float v) {
@@ -183,10 +233,46 @@ __device__ __forceinline__ float sum_groups(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-template <class T, int NB>
-struct Pitch {
-  static constexpr int KEY = 32 * NB + Num<T>::PAD, VALUE = COLS + Num<T>::PAD;
+// What every sweep derives from its workgroup and wavefront.
+struct Place {
+  Item it;
+  int item, block, group, wave, head, p0, width;
+  bool active;        // whether the wavefront has channels
+  int64_t token0;     // of all tokens
+  int64_t state_at;   // of its head in the states
+  int64_t part;       // its row in per-wavefront results
+
+  // Workgroups are dealt to the eight dies in turn: each die takes a run of
+  // consecutive ones, so that those which share keys and queries share an L2.
+  __device__ __forceinline__ explicit Place(const SweepArgs& a) {
+    const uint32_t n = gridDim.x, b = blockIdx.x;
+    const uint32_t id = b < n / 8 * 8 ? b % 8 * (n / 8) + b / 8 : b;
+    item = (int)(id / (uint32_t)(a.groups * a.blocks));
+    block = (int)(id % (uint32_t)(a.groups * a.blocks));
+    it = find_item(a, item);
+    group = block / a.blocks;
+    block %= a.blocks;
+    const int per_group = a.heads / a.groups;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // one for all lanes: in scalar registers
+    const int unit = block * WAVES + wave;
+    active = unit < per_group * a.col_tiles;
+    head = group * per_group + (active ? unit / a.col_tiles : 0);
+    p0 = active ? unit % a.col_tiles * a.cols : 0;
+    width = active ? min(a.cols, a.head_dim - p0) : 0;
+    token0 = item_token(a, it);
+    state_at = ((int64_t)(a.by_item ? item : it.seq) * a.heads + head) * a.head_dim * a.states;
+    part = (int64_t)head * a.col_tiles + p0 / a.cols;
+  }
 };
+
+// Whether a sweep's rows are all of whole 16-byte pieces and fill its tiles.
+inline bool is_full(const SweepArgs& a, int nb) {
+  for (const Strided& t : {a.key, a.query, a.value, a.other})
+    if (t.tok >= (1 << 24)) return false;
+  if (reinterpret_cast<uintptr_t>(a.state_in) % 16 || reinterpret_cast<uintptr_t>(a.state_out) % 16) return false;
+  return a.head_dim % a.cols == 0 && a.states == 32 * nb && a.wide_key && a.wide_query && a.wide_value &&
+         a.wide_other && a.wide_out;
+}
 
 inline uint32_t workgroups(const SweepArgs& a, int items) {
   const int64_t n = (int64_t)items * a.groups * a.blocks;

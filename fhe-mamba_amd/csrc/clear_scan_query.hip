@@ -2,29 +2,30 @@
 // in reverse, where keys and queries change places, those of B.
 #pragma clang fp contract(fast)
 #include "clear_scan.hpp"
-#include "context.hpp"
 
 namespace fhe::clear {
 namespace {
 
-template <class T, int NB>
+template <class T, int NB, int PT>
 struct QueryLds {
-  static constexpr int SUM = 32 * NB + 4;
-  alignas(16) T key[CHUNK * Pitch<T, NB>::KEY];
-  alignas(16) T value[WAVES][CHUNK * Pitch<T, NB>::VALUE];
-  alignas(16) T other[WAVES][CHUNK * Pitch<T, NB>::VALUE];
+  using Key = Tile<T, 32 * NB>;
+  using Value = Tile<T, 16 * PT>;
+  static constexpr int ROUND = NB < 2 ? 2 * NB : 4;  // tiles of states summed over the wavefronts at a time
+  static constexpr int SUM = 16 * ROUND + 4;
+  alignas(16) T key[CHUNK * Key::PITCH];
+  alignas(16) T value[WAVES][CHUNK * Value::PITCH];
   alignas(16) float sum[WAVES][16 * SUM];
   alignas(16) Gates gates[WAVES];
 };
 
 // State tiles (rows 4 q + r the channel, column l the state) from and to
 // [head_dim][states].
-template <int NB>
-__device__ __forceinline__ void state_io(f32x4 (&h)[2][2 * NB], const float* from, float* to, int p0,
+template <int NB, int PT>
+__device__ __forceinline__ void state_io(f32x4 (&h)[PT][2 * NB], const float* from, float* to, int p0,
                                          int head_dim, int states) {
   const int q = lane_id() >> 4, l = lane_id() & 15;
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
+  for (int p = 0; p < PT; ++p)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = p0 + 16 * p + 4 * q + r;
@@ -39,105 +40,106 @@ __device__ __forceinline__ void state_io(f32x4 (&h)[2][2 * NB], const float* fro
     }
 }
 
-// Target t's gradient from 32 channels of one head,
+// Target t's gradient from 16 PT channels of one head,
 //   in_t sum_p other[t][p] h[p] + sum_s decay(t, s) (other_t . value_s) key_s,
 // summed over a workgroup's wavefronts and written for each workgroup of a
 // group; forward also the part of the gates' gradient that the state before the
 // chunk has in it.
-template <class T, int NB, bool REV>
-__global__ __launch_bounds__(64 * WAVES, 1) void k_query_sweep(SweepArgs a) {
+template <class T, int NB, int PT, bool REV, bool FULL>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_query_sweep(SweepArgs a) {
   using N = Num<T>;
   using Frag = typename N::Frag;
-  using Lds = QueryLds<T, NB>;
-  constexpr int KP = Pitch<T, NB>::KEY, VP = Pitch<T, NB>::VALUE;
+  using Lds = QueryLds<T, NB, PT>;
+  using Key = typename Lds::Key;
+  using Value = typename Lds::Value;
   extern __shared__ __align__(16) char lds_raw[];
   Lds& lds = *reinterpret_cast<Lds*>(lds_raw);
 
-  const int item_i = blockIdx.x / (a.groups * a.blocks);
-  const int block = blockIdx.x % (a.groups * a.blocks);
-  const Item it = find_item(a, item_i);
+  const Place at(a);
+  const Item it = at.it;
   if (it.count <= 0 && it.seq < 0) return;
-  const int group = block / a.blocks, per_group = a.heads / a.groups;
-  const int wave = threadIdx.x >> 6, lane = lane_id(), q = lane >> 4, l = lane & 15;
-  const int unit = block % a.blocks * WAVES + wave;
-  const bool active = unit < per_group * a.col_tiles;
-  const int head = group * per_group + (active ? unit / a.col_tiles : 0);
-  const int p0 = active ? unit % a.col_tiles * COLS : 0;
-  const int width = active ? min(COLS, a.head_dim - p0) : 0;
-  const int64_t part = (int64_t)head * a.col_tiles + p0 / COLS;
-  const int64_t token0 = item_token(a, it);
-  const int64_t state_at =
-      ((int64_t)(a.by_item ? item_i : it.seq) * a.heads + head) * a.head_dim * a.states;
-
-  const T* key = (const T*)a.key.p + item_at(a, a.key, it) + group * a.key.head;
-  const T* query = REV ? nullptr : (const T*)a.query.p + item_at(a, a.query, it) + group * a.query.head;
-  const T* value = (const T*)a.value.p + item_at(a, a.value, it) + head * a.value.head + p0;
-  const T* other = (const T*)a.other.p + item_at(a, a.other, it) + head * a.other.head + p0;
-  const float* write = (const float*)a.write.p + item_at(a, a.write, it) + head * a.write.head;
-  const float* decay = (const float*)a.decay.p + item_at(a, a.decay, it) + head * a.decay.head;
-  float* out = (float*)a.out +
-               (((int64_t)(block % a.blocks) * a.all_tokens + token0) * a.groups + group) * a.states;
+  const int lane = lane_id(), q = lane >> 4, l = lane & 15;
+  const T* key = (const T*)a.key.p + item_at(a, a.key, it) + at.group * a.key.head;
+  const T* query = REV ? nullptr : (const T*)a.query.p + item_at(a, a.query, it) + at.group * a.query.head;
+  const T* value = (const T*)a.value.p + item_at(a, a.value, it) + at.head * a.value.head + at.p0;
+  const T* other = (const T*)a.other.p + item_at(a, a.other, it) + at.head * a.other.head + at.p0;
+  const float* write = (const float*)a.write.p + item_at(a, a.write, it) + at.head * a.write.head;
+  const float* decay = (const float*)a.decay.p + item_at(a, a.decay, it) + at.head * a.decay.head;
+  float* out =
+      (float*)a.out + (((int64_t)at.block * a.all_tokens + at.token0) * a.groups + at.group) * a.states;
   const int64_t out_tok = (int64_t)a.groups * a.states;
+  float* gate_grad = REV ? nullptr : a.gate_part + at.part * a.all_tokens + at.token0;
 
-  f32x4 h[2][2 * NB] = {};
-  if (a.state_in && active && it.live)
-    state_io<NB>(h, a.state_in + state_at, nullptr, p0, a.head_dim, a.states);
+  f32x4 h[PT][2 * NB] = {};
+  if (a.state_in && at.active && it.live)
+    state_io<NB, PT>(h, a.state_in + at.state_at, nullptr, at.p0, a.head_dim, a.states);
 
-  T* vt = lds.value[wave];
-  T* ot = lds.other[wave];
-  Gates& t = lds.gates[wave];
+  T* vt = lds.value[at.wave];
+  Gates& t = lds.gates[at.wave];
   const int chunks = (it.count + CHUNK - 1) / CHUNK;
   for (int c = 0; c < chunks; ++c) {
     const int first = (REV ? chunks - 1 - c : c) * CHUNK;
     const int n = min(CHUNK, it.count - first), live = it.live ? n : 0;
-    __syncthreads();
-    stage<T, KP>(lds.key, key + first * a.key.tok, a.key.tok, live, a.states, 32 * NB, a.wide_key,
-                 threadIdx.x, 64 * WAVES);
-    if (active) {
-      stage<T, VP>(vt, value + first * a.value.tok, a.value.tok, live, width, COLS, a.wide_value,
-                   lane, 64);
-      stage<T, VP>(ot, other + first * a.other.tok, a.other.tok, live, width, COLS, a.wide_other,
-                   lane, 64);
-      make_gates<REV>(t, write + first * a.write.tok, a.write.tok, decay + first * a.decay.tok,
-                      a.decay.tok, live);
+    {
+      Stage<T, 32 * NB, 64 * WAVES, FULL> sk;
+      Stage<T, 16 * PT, 64, FULL> sv;
+      float g = 0.0f, w = 0.0f;
+      if (at.active && lane < live) {
+        g = decay[(int64_t)(first + lane) * a.decay.tok];
+        w = write[(int64_t)(first + lane) * a.write.tok];
+      }
+      sk.load(key + first * a.key.tok, a.key.tok, live, a.states, a.wide_key, threadIdx.x);
+      sv.load(value + first * a.value.tok, a.value.tok, live, at.width, a.wide_value, lane);
+      __syncthreads();
+      if (at.active) make_gates<REV>(t, g, w);
+      sk.store(lds.key, threadIdx.x);
+      sv.store(vt, lane);
+      __syncthreads();
     }
-    __syncthreads();
-
-    Split<T, N::FAIR> state[2 * NB];
-#pragma unroll
-    for (int nt = 0; nt < 2 * NB; ++nt) state[nt] = split<T, N::FAIR>(join(h[0][nt], h[1][nt]));
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       if (16 * i >= n) break;
+      step_end();
+      const int tok = 16 * i + l;
       f32x4 got[2 * NB] = {};
-      if (active) {
-        const Frag of = N::rows(ot + 16 * i * VP, VP);
-        const float in = t.dst[16 * i + l] * t.dst_in[i];
+      if (at.active) {
+        Frag of[PT / 2];
+#pragma unroll
+        for (int k = 0; k < PT / 2; ++k)
+          of[k] = row_frag<T, FULL>(other + (int64_t)(first + 16 * i) * a.other.tok + 32 * k, a.other.tok,
+                                    live - 16 * i, at.width - 32 * k, a.wide_other);
+        const float inside = t.template inside<REV>(i, tok), in = inside * t.template into<REV>(i);
 #pragma unroll
         for (int nt = 0; nt < 2 * NB; ++nt) {
-          got[nt] = mma<T, N::FAIR>(state[nt], of, got[nt]);
+#pragma unroll
+          for (int k = 0; k < PT / 2; ++k)
+            got[nt] = mma<T, N::FAIR>(split<T, N::FAIR>(join(h[2 * k][nt], h[2 * k + 1][nt])), of[k], got[nt]);
           got[nt] *= in;
         }
         if constexpr (!REV) {
           float sum = 0.0f;
-          if (16 * i + l < live) {
-            const T* row = query + (first + 16 * i + l) * a.query.tok + 4 * q;
 #pragma unroll
-            for (int nt = 0; nt < 2 * NB; ++nt)
+          for (int k = 0; k < NB; ++k) {
+            const Frag qf = row_frag<T, FULL>(query + (int64_t)(first + 16 * i) * a.query.tok + 32 * k, a.query.tok,
+                                              live - 16 * i, a.states - 32 * k, a.wide_query);
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (16 * nt + 4 * q + r < a.states) sum += got[nt][r] * (float)row[16 * nt + r];
+            for (int half = 0; half < 2; ++half) {
+              const f32x4 v = half_of(qf, half);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sum += got[2 * k + half][r] * v[r];
+            }
           }
           sum = sum_groups(sum);
-          if (q == 0 && 16 * i + l < n) a.gate_part[part * a.all_tokens + token0 + first + 16 * i + l] = sum;
+          if (q == 0 && tok < n) (gate_grad + first + 16 * i)[l] = sum;
         }
         f32x4 pairs[TILES] = {};
 #pragma unroll
         for (int j = 0; j < TILES; ++j) {
           if (REV ? j < i : j > i) continue;
           f32x4 z = {};
-          z = N::mma(N::rows(vt + 16 * j * VP, VP), of, z);
-          pairs[j] = decayed<REV>(t, z, i, j);
+#pragma unroll
+          for (int k = 0; k < PT / 2; ++k) z = N::mma(Value::rows(vt, 16 * j, 32 * k), of[k], z);
+          pairs[j] = decayed<REV>(t, z, i, j, inside);
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -145,64 +147,70 @@ __global__ __launch_bounds__(64 * WAVES, 1) void k_query_sweep(SweepArgs a) {
           const auto s = split<T, N::FAIR>(join(pairs[2 * m], pairs[2 * m + 1]));
 #pragma unroll
           for (int nt = 0; nt < 2 * NB; ++nt)
-            got[nt] = mma<T, N::FAIR>(N::cols(lds.key + 32 * m * KP + 16 * nt, KP), s, got[nt]);
+            got[nt] = mma<T, N::FAIR>(Key::cols(lds.key, 32 * m, 16 * nt), s, got[nt]);
         }
         if constexpr (REV) {
-          const float w = t.w[16 * i + l];
+          const float w = t.w[tok];
 #pragma unroll
           for (int nt = 0; nt < 2 * NB; ++nt) got[nt] *= w;
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < 2 * NB; ++nt)
-        *reinterpret_cast<f32x4*>(&lds.sum[wave][l * Lds::SUM + 16 * nt + 4 * q]) = got[nt];
-      __syncthreads();
-      for (int e = threadIdx.x; e < 16 * 32 * NB; e += 64 * WAVES) {
-        const int row = e / (32 * NB), col = e % (32 * NB);
-        float sum = 0.0f;
+      for (int n0 = 0; n0 < 2 * NB; n0 += Lds::ROUND) {
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) sum += lds.sum[w][row * Lds::SUM + col];
-        if (16 * i + row < n && col < a.states) out[(first + 16 * i + row) * out_tok + col] = sum;
+        for (int nt = 0; nt < Lds::ROUND; ++nt)
+          *reinterpret_cast<f32x4*>(&lds.sum[at.wave][l * Lds::SUM + 16 * nt + 4 * q]) = got[n0 + nt];
+        __syncthreads();
+        const int row = threadIdx.x / (4 * Lds::ROUND), col = threadIdx.x % (4 * Lds::ROUND) * 4;
+        if (row < 16 && 16 * i + row < n) {
+          f32x4 sum = {};
+#pragma unroll
+          for (int w = 0; w < WAVES; ++w) sum += *reinterpret_cast<const f32x4*>(&lds.sum[w][row * Lds::SUM + col]);
+          const int at_n = 16 * n0 + col;
+          store4(out + (first + 16 * i + row) * out_tok + at_n, sum, (FULL ? 32 * NB : a.states) - at_n,
+                 FULL || a.wide_out);
+        }
+        __syncthreads();
       }
-      __syncthreads();
     }
-    if (!active) continue;
+    if (!at.active) continue;
     // h <- total h + sum_s (factor_s value_s) key_s
-    const float total = t.total;
+    const float total = t.total();
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
+    for (int p = 0; p < PT; ++p)
 #pragma unroll
       for (int nt = 0; nt < 2 * NB; ++nt) h[p][nt] *= total;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       if (32 * m >= n) break;
-      const f32x8 f = to_state(t, m);
-      Split<T, N::FINE> s[2];
+      const f32x8 f = to_state<REV>(t, m);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const Frag v = N::cols(vt + 32 * m * VP + 16 * p, VP);
-        f32x8 x;
+      for (int p2 = 0; p2 < PT; p2 += 2) {
+        step_end();
+        Split<T, N::FINE> s[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)v[j] * f[j];
-        s[p] = split<T, N::FINE>(x);
-      }
+        for (int p = 0; p < 2; ++p) {
+          const Frag v = Value::cols(vt, 32 * m, 16 * (p2 + p));
+          s[p] = split<T, N::FINE>(widen(v) * f);
+        }
 #pragma unroll
-      for (int nt = 0; nt < 2 * NB; ++nt) {
-        const auto k = N::cols(lds.key + 32 * m * KP + 16 * nt, KP);
+        for (int nt = 0; nt < 2 * NB; ++nt) {
+          const auto k = Key::cols(lds.key, 32 * m, 16 * nt);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) h[p][nt] = mma<T, N::FINE>(s[p], k, h[p][nt]);
+          for (int p = 0; p < 2; ++p) h[p2 + p][nt] = mma<T, N::FINE>(s[p], k, h[p2 + p][nt]);
+        }
       }
     }
   }
-  if (a.state_out && active && it.live)
-    state_io<NB>(h, nullptr, a.state_out + state_at, p0, a.head_dim, a.states);
+  if (a.state_out && at.active && it.live)
+    state_io<NB, PT>(h, nullptr, a.state_out + at.state_at, at.p0, a.head_dim, a.states);
 }
 
-template <class T, int NB, bool REV>
+template <class T, int NB, int PT, bool REV>
 void launch(const SweepArgs& a, int items, hipStream_t s) {
-  constexpr size_t bytes = sizeof(QueryLds<T, NB>);
+  constexpr size_t bytes = sizeof(QueryLds<T, NB, PT>);
   static_assert(bytes <= 160 * 1024);
-  auto* kernel = &k_query_sweep<T, NB, REV>;
+  auto* kernel = is_full(a, NB) ? &k_query_sweep<T, NB, PT, REV, true> : &k_query_sweep<T, NB, PT, REV, false>;
   hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
             "scan gradient sweep");
   kernel<<<workgroups(a, items), 64 * WAVES, bytes, s>>>(a);
@@ -211,14 +219,19 @@ void launch(const SweepArgs& a, int items, hipStream_t s) {
 
 template <bool REV>
 void dispatch(uint32_t dtype, const SweepArgs& a, int items, hipStream_t s) {
-  auto by_size = [&](auto zero) {
+  auto by_size = [&](auto zero, auto cols) {
     using T = decltype(zero);
-    if (a.states <= 32) launch<T, 1, REV>(a, items, s);
-    else if (a.states <= 64) launch<T, 2, REV>(a, items, s);
-    else launch<T, 4, REV>(a, items, s);
+    constexpr int PT = decltype(cols)::value / 16;
+    if (a.states <= 32) launch<T, 1, PT, REV>(a, items, s);
+    else if (a.states <= 64) launch<T, 2, PT, REV>(a, items, s);
+    else launch<T, 4, PT, REV>(a, items, s);
   };
-  if (dtype == BF16) by_size(bf16{});
-  else by_size(float{});
+  auto by_cols = [&](auto zero) {
+    if (a.cols == 32) by_size(zero, std::integral_constant<int, 32>{});
+    else by_size(zero, std::integral_constant<int, 64>{});
+  };
+  if (dtype == BF16) by_cols(bf16{});
+  else by_cols(float{});
 }
 
 }  // namespace

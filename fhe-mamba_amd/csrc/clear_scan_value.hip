@@ -2,203 +2,196 @@
 // results, and the state that a segment leaves.
 #pragma clang fp contract(fast)
 #include "clear_scan.hpp"
-#include "context.hpp"
 
 namespace fhe::clear {
 namespace {
 
-template <class T, int NB, bool REV, bool VALUES>
+template <class T, int NB, int PT, bool VALUES>
 struct ValueLds {
+  using Key = Tile<T, 32 * NB>;
+  using Value = Tile<T, 16 * PT>;
   // 16-byte rows: a tile that a kernel does not have must not shift the others
-  alignas(16) T key[CHUNK * Pitch<T, NB>::KEY];
-  alignas(16) T query[VALUES ? CHUNK * Pitch<T, NB>::KEY : 1];
-  alignas(16) T value[WAVES][CHUNK * Pitch<T, NB>::VALUE];
-  alignas(16) T other[VALUES && REV ? WAVES : 1][VALUES && REV ? CHUNK * Pitch<T, NB>::VALUE : 1];
+  alignas(16) T key[CHUNK * Key::PITCH];
+  alignas(16) T query[VALUES ? CHUNK * Key::PITCH : 1];
+  alignas(16) T value[WAVES][CHUNK * Value::PITCH];
   alignas(16) Gates gates[WAVES];
 };
 
-// Adds a chunk to a wavefront's state [states][32 channels]:
+// Adds a chunk to a wavefront's state [states][channels]:
 // h <- total h + sum_s key_s (factor_s value_s).
-template <class T, int NB>
-__device__ __forceinline__ void add_chunk(f32x4 (&h)[2 * NB][2], const T* key, const Gates& t,
-                                          const typename Num<T>::Frag (&v)[2][2], int n) {
+template <class T, int NB, int PT, bool REV>
+__device__ __forceinline__ void add_chunk(f32x4 (&h)[2 * NB][PT], const T* key, const T* value, const Gates& t,
+                                          int n) {
   using N = Num<T>;
-  const float total = t.total;
+  const float total = t.total();
 #pragma unroll
   for (int nt = 0; nt < 2 * NB; ++nt)
 #pragma unroll
-    for (int p = 0; p < 2; ++p) h[nt][p] *= total;
+    for (int p = 0; p < PT; ++p) h[nt][p] *= total;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     if (32 * m >= n) break;
-    const f32x8 f = to_state(t, m);
-    Split<T, N::FINE> s[2];
+    const f32x8 f = to_state<REV>(t, m);
+    Split<T, N::FINE> s[PT];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      f32x8 x;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = (float)v[m][p][j] * f[j];
-      s[p] = split<T, N::FINE>(x);
-    }
+    for (int p = 0; p < PT; ++p)
+      s[p] = split<T, N::FINE>(widen(Tile<T, 16 * PT>::cols(value, 32 * m, 16 * p)) * f);
 #pragma unroll
     for (int nt = 0; nt < 2 * NB; ++nt) {
-      const auto k = N::cols(key + 32 * m * Pitch<T, NB>::KEY + 16 * nt, Pitch<T, NB>::KEY);
+      const auto k = Tile<T, 32 * NB>::cols(key, 32 * m, 16 * nt);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) h[nt][p] = mma<T, N::FINE>(k, s[p], h[nt][p]);
+      for (int p = 0; p < PT; ++p) h[nt][p] = mma<T, N::FINE>(k, s[p], h[nt][p]);
     }
   }
 }
 
 // State tiles (rows 4 q + r the states, column l the channel) to and from
 // [head_dim][states].
-template <int NB>
-__device__ __forceinline__ void state_io(f32x4 (&h)[2 * NB][2], const float* from, float* to, int p0,
+template <int NB, int PT, bool FULL>
+__device__ __forceinline__ void state_io(f32x4 (&h)[2 * NB][PT], const float* from, float* to, int p0,
                                          int head_dim, int states) {
   const int q = lane_id() >> 4, l = lane_id() & 15;
+  const bool wide = FULL || (states % 4 == 0 && reinterpret_cast<uintptr_t>(to ? to : from) % 16 == 0);
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
+  for (int p = 0; p < PT; ++p) {
     const int row = p0 + 16 * p + l;
+    if (!FULL && row >= head_dim) continue;
 #pragma unroll
-    for (int nt = 0; nt < 2 * NB; ++nt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = 16 * nt + 4 * q + r;
-        if (row < head_dim && n < states) {
-          if (to) to[(int64_t)row * states + n] = h[nt][p][r];
-          else h[nt][p][r] = from[(int64_t)row * states + n];
-        }
-      }
+    for (int nt = 0; nt < 2 * NB; ++nt) {
+      const int n = 16 * nt + 4 * q;
+      const int64_t at = (int64_t)row * states + n;
+      const int left = FULL ? 4 : states - n;
+      if (to) store4(to + at, h[nt][p], left, wide);
+      else h[nt][p] = load4(from + at, left, wide);
+    }
   }
 }
 
-// y (or, in reverse, the gradient of x) of a segment, 32 channels of one head a
-// wavefront, four wavefronts of one group on shared keys and queries.
-template <class T, int NB, bool REV, bool VALUES>
-__global__ __launch_bounds__(64 * WAVES, VALUES && REV ? 1 : 2) void k_value_sweep(SweepArgs a) {
+// y (or, in reverse, the gradient of x) of a segment, 16 PT channels of one head
+// a wavefront, four wavefronts of one group on shared keys and queries.
+template <class T, int NB, int PT, bool REV, bool VALUES, bool FULL>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_value_sweep(SweepArgs a) {
   using N = Num<T>;
   using Frag = typename N::Frag;
-  using Lds = ValueLds<T, NB, REV, VALUES>;
-  constexpr int KP = Pitch<T, NB>::KEY, VP = Pitch<T, NB>::VALUE;
+  using Lds = ValueLds<T, NB, PT, VALUES>;
+  using Key = typename Lds::Key;
+  using Value = typename Lds::Value;
   extern __shared__ __align__(16) char lds_raw[];
   Lds& lds = *reinterpret_cast<Lds*>(lds_raw);
 
-  const int item_i = blockIdx.x / (a.groups * a.blocks);
-  const int block = blockIdx.x % (a.groups * a.blocks);
-  const Item it = find_item(a, item_i);
+  const Place at(a);
+  const Item it = at.it;
   if (it.count <= 0 && it.seq < 0) return;
-  const int group = block / a.blocks, per_group = a.heads / a.groups;
-  const int wave = threadIdx.x >> 6, lane = lane_id(), q = lane >> 4, l = lane & 15;
-  const int unit = block % a.blocks * WAVES + wave;
-  const bool active = unit < per_group * a.col_tiles;
-  const int head = group * per_group + (active ? unit / a.col_tiles : 0);
-  const int p0 = active ? unit % a.col_tiles * COLS : 0;
-  const int width = active ? min(COLS, a.head_dim - p0) : 0;
-  const int64_t part = (int64_t)head * a.col_tiles + p0 / COLS;  // row of the per-unit results
-  const int64_t token0 = item_token(a, it);
-  const int64_t state_at =
-      ((int64_t)(a.by_item ? item_i : it.seq) * a.heads + head) * a.head_dim * a.states;
-
-  const T* key = (const T*)a.key.p + item_at(a, a.key, it) + group * a.key.head;
-  const T* query = VALUES ? (const T*)a.query.p + item_at(a, a.query, it) + group * a.query.head : nullptr;
-  const T* value = (const T*)a.value.p + item_at(a, a.value, it) + head * a.value.head + p0;
+  const int lane = lane_id(), q = lane >> 4, l = lane & 15;
+  const T* key = (const T*)a.key.p + item_at(a, a.key, it) + at.group * a.key.head;
+  const T* query = VALUES ? (const T*)a.query.p + item_at(a, a.query, it) + at.group * a.query.head : nullptr;
+  const T* value = (const T*)a.value.p + item_at(a, a.value, it) + at.head * a.value.head + at.p0;
   const T* other =
-      VALUES && REV ? (const T*)a.other.p + item_at(a, a.other, it) + head * a.other.head + p0 : nullptr;
-  const float* write = (const float*)a.write.p + item_at(a, a.write, it) + head * a.write.head;
-  const float* decay = (const float*)a.decay.p + item_at(a, a.decay, it) + head * a.decay.head;
-  T* out = VALUES ? (T*)a.out + (token0 * a.heads + head) * a.head_dim + p0 : nullptr;
+      VALUES && REV ? (const T*)a.other.p + item_at(a, a.other, it) + at.head * a.other.head + at.p0 : nullptr;
+  const float* write = (const float*)a.write.p + item_at(a, a.write, it) + at.head * a.write.head;
+  const float* decay = (const float*)a.decay.p + item_at(a, a.decay, it) + at.head * a.decay.head;
+  T* out = VALUES ? (T*)a.out + (at.token0 * a.heads + at.head) * a.head_dim + at.p0 : nullptr;
   const int64_t out_tok = (int64_t)a.heads * a.head_dim;
-  const float skip = VALUES && a.d && active ? a.d[head] : 0.0f;
+  const uint32_t out_at = (uint32_t)(l * out_tok + 4 * q) * (uint32_t)sizeof(T);  // a lane's place in 16 rows
+  float* dwrite = VALUES && REV ? a.dwrite_part + at.part * a.all_tokens + at.token0 : nullptr;
+  float* gate_grad = VALUES && REV ? a.gate_part + at.part * a.all_tokens + at.token0 : nullptr;
+  const int width = FULL ? 16 * PT : at.width;
+  const float skip = VALUES && a.d && at.active ? a.d[at.head] : 0.0f;
 
-  f32x4 h[2 * NB][2] = {};
-  const bool seeded = VALUES && a.state_in && active && it.live;
-  if (seeded) state_io<NB>(h, a.state_in + state_at, nullptr, p0, a.head_dim, a.states);
+  f32x4 h[2 * NB][PT] = {};
+  if (VALUES && a.state_in && at.active && it.live)
+    state_io<NB, PT, FULL>(h, a.state_in + at.state_at, nullptr, at.p0, a.head_dim, a.states);
 
-  T* vt = lds.value[wave];
-  T* ot = lds.other[VALUES && REV ? wave : 0];
-  Gates& t = lds.gates[wave];
+  T* vt = lds.value[at.wave];
+  Gates& t = lds.gates[at.wave];
   float dd = 0.0f;
   double log_total = 0.0;
   const int chunks = (it.count + CHUNK - 1) / CHUNK;
   for (int c = 0; c < chunks; ++c) {
     const int first = (REV ? chunks - 1 - c : c) * CHUNK;
     const int n = min(CHUNK, it.count - first), live = it.live ? n : 0;
-    __syncthreads();
-    stage<T, KP>(lds.key, key + first * a.key.tok, a.key.tok, live, a.states, 32 * NB, a.wide_key,
-                 threadIdx.x, 64 * WAVES);
-    if constexpr (VALUES)
-      stage<T, KP>(lds.query, query + first * a.query.tok, a.query.tok, live, a.states, 32 * NB,
-                   a.wide_query, threadIdx.x, 64 * WAVES);
-    if (active) {
-      stage<T, VP>(vt, value + first * a.value.tok, a.value.tok, live, width, COLS, a.wide_value,
-                   lane, 64);
-      if constexpr (VALUES && REV)
-        stage<T, VP>(ot, other + first * a.other.tok, a.other.tok, live, width, COLS, a.wide_other,
-                     lane, 64);
-      make_gates<REV>(t, write + first * a.write.tok, a.write.tok, decay + first * a.decay.tok,
-                      a.decay.tok, live);
+    {
+      Stage<T, 32 * NB, 64 * WAVES, FULL> sk, sq;
+      Stage<T, 16 * PT, 64, FULL> sv;
+      float g = 0.0f, w = 0.0f;
+      if (at.active && lane < live) {
+        g = decay[(int64_t)(first + lane) * a.decay.tok];
+        w = write[(int64_t)(first + lane) * a.write.tok];
+      }
+      sk.load(key + first * a.key.tok, a.key.tok, live, a.states, a.wide_key, threadIdx.x);
+      if constexpr (VALUES)
+        sq.load(query + first * a.query.tok, a.query.tok, live, a.states, a.wide_query, threadIdx.x);
+      sv.load(value + first * a.value.tok, a.value.tok, live, at.width, a.wide_value, lane);
+      __syncthreads();
+      if (at.active) make_gates<REV>(t, g, w);
+      sk.store(lds.key, threadIdx.x);
+      if constexpr (VALUES) sq.store(lds.query, threadIdx.x);
+      sv.store(vt, lane);
+      __syncthreads();
     }
-    __syncthreads();
-    if (!active) continue;
-
-    Frag v[2][2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) v[m][p] = N::cols(vt + 32 * m * VP + 16 * p, VP);
+    if (!at.active) continue;
 
     if constexpr (VALUES) {
-      Split<T, N::FAIR> state[NB][2];
+      // what the state before the chunk gives: rows 4 q + r the channels, columns
+      // l the tokens, so that a lane has four neighbouring channels of its token
+      f32x4 y[TILES][PT] = {};
 #pragma unroll
-      for (int k = 0; k < NB; ++k)
+      for (int k = 0; k < NB; ++k) {
+        Split<T, N::FAIR> state[PT];
 #pragma unroll
-        for (int p = 0; p < 2; ++p) state[k][p] = split<T, N::FAIR>(join(h[2 * k][p], h[2 * k + 1][p]));
-      float row_sum[TILES][4] = {}, col_sum[TILES] = {};
+        for (int p = 0; p < PT; ++p) state[p] = split<T, N::FAIR>(join(h[2 * k][p], h[2 * k + 1][p]));
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+          const Frag qf = Key::rows(lds.query, 16 * i, 32 * k);
+#pragma unroll
+          for (int p = 0; p < PT; ++p) y[i][p] = mma<T, N::FAIR>(state[p], qf, y[i][p]);
+        }
+      }
+      f32x4 row_sum[REV ? TILES : 1] = {};
+      float gate[REV ? TILES : 1] = {};
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
         if (16 * i >= n) break;
-        Frag qf[NB];
+        if constexpr (REV) step_end();
+        const int tok = 16 * i + l;
+        const float inside = t.template inside<REV>(i, tok), in = inside * t.template into<REV>(i), w = t.w[tok];
+        Frag of[REV ? PT / 2 : 1];
+        if constexpr (REV) {
 #pragma unroll
-        for (int k = 0; k < NB; ++k) qf[k] = N::rows(lds.query + 16 * i * KP + 32 * k, KP);
-        // what the state before the chunk gives
-        f32x4 y[2] = {};
+          for (int k = 0; k < PT / 2; ++k)
+            of[k] = row_frag<T, FULL>(other + (int64_t)(first + 16 * i) * a.other.tok + 32 * k, a.other.tok,
+                                      live - 16 * i, width - 32 * k, a.wide_other);
+        }
 #pragma unroll
-        for (int k = 0; k < NB; ++k)
-#pragma unroll
-          for (int p = 0; p < 2; ++p) y[p] = mma<T, N::FAIR>(qf[k], state[k][p], y[p]);
-        f32x4 din = *reinterpret_cast<const f32x4*>(&t.dst[16 * i + 4 * q]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) din[r] *= t.dst_in[i];
-        f32x4 from_state = {};
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          y[p] *= din;
+        for (int p = 0; p < PT; ++p) {
+          y[i][p] *= in;
           if constexpr (REV) {
+            const f32x4 x = half_of(of[p / 2], p % 2);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              from_state[r] += y[p][r] * (float)ot[(16 * i + 4 * q + r) * VP + 16 * p + l];
+            for (int r = 0; r < 4; ++r) gate[i] -= w * (y[i][p][r] * x[r]);
           }
         }
         // and the tokens of the chunk
+        Frag qf[NB];
+#pragma unroll
+        for (int k = 0; k < NB; ++k) qf[k] = Key::rows(lds.query, 16 * i, 32 * k);
         f32x4 pairs[TILES] = {};
-        Frag of;
-        if constexpr (REV) of = N::rows(ot + 16 * i * VP, VP);
 #pragma unroll
         for (int j = 0; j < TILES; ++j) {
           if (REV ? j < i : j > i) continue;
           f32x4 s = {};
 #pragma unroll
-          for (int k = 0; k < NB; ++k)
-            s = N::mma(N::rows(lds.key + 16 * j * KP + 32 * k, KP), qf[k], s);
-          pairs[j] = decayed<REV>(t, s, i, j);
+          for (int k = 0; k < NB; ++k) s = N::mma(Key::rows(lds.key, 16 * j, 32 * k), qf[k], s);
+          pairs[j] = decayed<REV>(t, s, i, j, inside);
           if constexpr (REV) {  // the pairs' own parts of the loss, off the diagonal
             f32x4 z = {};
-            z = N::mma(N::rows(vt + 16 * j * VP, VP), of, z);
-            const float w = t.w[16 * i + l];
+#pragma unroll
+            for (int k = 0; k < PT / 2; ++k) z = N::mma(Value::rows(vt, 16 * j, 32 * k), of[k], z);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float m = i == j && 4 * q + r == l ? 0.0f : pairs[j][r] * z[r] * w;
               row_sum[j][r] += m;
-              col_sum[i] += m;
+              gate[i] -= m;
             }
           }
         }
@@ -207,84 +200,79 @@ __global__ __launch_bounds__(64 * WAVES, VALUES && REV ? 1 : 2) void k_value_swe
           if (REV ? 2 * m + 1 < i : 2 * m > i) continue;
           const auto s = split<T, N::FAIR>(join(pairs[2 * m], pairs[2 * m + 1]));
 #pragma unroll
-          for (int p = 0; p < 2; ++p) y[p] = mma<T, N::FAIR>(s, v[m][p], y[p]);
+          for (int p = 0; p < PT; ++p)
+            y[i][p] = mma<T, N::FAIR>(Value::cols(vt, 32 * m, 16 * p), s, y[i][p]);
         }
-        f32x4 against = {};
+        Frag vf[PT / 2];
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
+        for (int k = 0; k < PT / 2; ++k) vf[k] = Value::rows(vt, 16 * i, 32 * k);
+        float against = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int at = (16 * i + 4 * q + r) * VP + 16 * p + l;
-            const float mine = (float)vt[at];
-            float got = y[p][r];
-            if constexpr (REV) {
-              const float x = (float)ot[at];
-              against[r] += got * x;
-              dd += mine * x;
-              got *= t.w[16 * i + 4 * q + r];
+        for (int p = 0; p < PT; ++p) {
+          const f32x4 mine = half_of(vf[p / 2], p % 2);
+          if constexpr (REV) {
+            const f32x4 x = half_of(of[p / 2], p % 2);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              against += y[i][p][r] * x[r];
+              dd += mine[r] * x[r];
+              y[i][p][r] *= w;
             }
-            vt[at] = (T)(got + skip * mine);
           }
-        if constexpr (REV) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int at = first + 16 * i + 4 * q + r;
-            const float dw = sum16(against[r]), k = sum16(from_state[r]);
-            if (l == 0 && 16 * i + 4 * q + r < n) {
-              a.dwrite_part[part * a.all_tokens + token0 + at] = dw;
-              // kept until the row sums are whole; the same lane adds them
-              t.g[16 * i + 4 * q + r] = -(double)(t.w[16 * i + 4 * q + r] * k);
-            }
+          for (int r = 0; r < 4; ++r) y[i][p][r] += skip * mine[r];
+        }
+        if constexpr (REV) against = sum_groups(against);
+        if (tok < n) {
+          T* rows = out + (int64_t)(first + 16 * i) * out_tok;
+          T* to = FULL ? reinterpret_cast<T*>(reinterpret_cast<char*>(rows) + out_at) : rows + l * out_tok + 4 * q;
+#pragma unroll
+          for (int p = 0; p < PT; ++p) store4(to + 16 * p, y[i][p], width - 16 * p - 4 * q, FULL || a.wide_out);
+          if constexpr (REV) {
+            if (q == 0) (dwrite + first + 16 * i)[l] = against;
           }
         }
       }
       if constexpr (REV) {
+        wave_sync();  // the sums of logarithms are read for the last time: their place is free
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float sum = sum16(row_sum[i][r]);
+            if (l == 0) t.g[16 * i + 4 * q + r] = sum;
+          }
+        }
         wave_sync();
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
-          const float cs = sum_groups(col_sum[i]);
-          f32x4 rs;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) rs[r] = sum16(row_sum[i][r]);
-          if (l == 0) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) t.g[16 * i + 4 * q + r] += rs[r];
-          }
-          wave_sync();
-          if (q == 0 && 16 * i + l < n)
-            a.gate_part[part * a.all_tokens + token0 + first + 16 * i + l] =
-                (float)(t.g[16 * i + l] - cs);
+          const float sum = sum_groups(gate[i]) + (float)t.g[16 * i + l];
+          if (q == 0 && 16 * i + l < n) (gate_grad + first + 16 * i)[l] = sum;
         }
       }
-      wave_sync();
-      for (int i = lane; i < CHUNK * (COLS / N::VEC); i += 64) {
-        const int row = i / (COLS / N::VEC), col = i % (COLS / N::VEC) * N::VEC;
-        if (row < n)
-          store16(out + (first + row) * out_tok + col,
-                  *reinterpret_cast<const u32x4*>(vt + row * VP + col), width - col, a.wide_out);
-      }
     } else {
-      log_total += t.e[TILES - 1];
+      log_total += t.ends[TILES];
     }
-    add_chunk<T, NB>(h, lds.key, t, v, n);
+    add_chunk<T, NB, PT, REV>(h, lds.key, vt, t, n);
   }
-  if (!active) return;
+  if (!at.active) return;
   if (a.state_out && (a.by_item || it.live))
-    state_io<NB>(h, nullptr, a.state_out + state_at, p0, a.head_dim, a.states);
+    state_io<NB, PT, FULL>(h, nullptr, a.state_out + at.state_at, at.p0, a.head_dim, a.states);
   if constexpr (!VALUES) {
-    if (lane == 0 && p0 == 0) a.decay_out[(int64_t)item_i * a.heads + head] = exp2d(log_total);
+    if (lane == 0 && at.p0 == 0) a.decay_out[(int64_t)at.item * a.heads + at.head] = exp2d(log_total);
   }
   if constexpr (VALUES && REV) {
     dd = sum_groups(sum16(dd));
-    if (lane == 0) a.dd_part[(int64_t)item_i * a.heads * a.col_tiles + part] = dd;
+    if (lane == 0) a.dd_part[(int64_t)at.item * a.heads * a.col_tiles + at.part] = dd;
   }
 }
 
-template <class T, int NB, bool REV, bool VALUES>
+template <class T, int NB, int PT, bool REV, bool VALUES>
 void launch(const SweepArgs& a, int items, hipStream_t s) {
-  constexpr size_t bytes = sizeof(ValueLds<T, NB, REV, VALUES>);
+  constexpr size_t bytes = sizeof(ValueLds<T, NB, PT, VALUES>);
   static_assert(bytes <= 160 * 1024);
-  auto* kernel = &k_value_sweep<T, NB, REV, VALUES>;
+  auto* kernel = is_full(a, NB) ? &k_value_sweep<T, NB, PT, REV, VALUES, true>
+                                : &k_value_sweep<T, NB, PT, REV, VALUES, false>;
   hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
             "scan sweep");
   kernel<<<workgroups(a, items), 64 * WAVES, bytes, s>>>(a);
@@ -296,9 +284,10 @@ void dispatch(uint32_t dtype, const SweepArgs& a, int items, bool rev, hipStream
   auto by_size = [&](auto zero, auto reverse) {
     using T = decltype(zero);
     constexpr bool R = decltype(reverse)::value;
-    if (a.states <= 32) launch<T, 1, R, VALUES>(a, items, s);
-    else if (a.states <= 64) launch<T, 2, R, VALUES>(a, items, s);
-    else launch<T, 4, R, VALUES>(a, items, s);
+    constexpr int PT = VALUE_COLS / 16;
+    if (a.states <= 32) launch<T, 1, PT, R, VALUES>(a, items, s);
+    else if (a.states <= 64) launch<T, 2, PT, R, VALUES>(a, items, s);
+    else launch<T, 4, PT, R, VALUES>(a, items, s);
   };
   auto by_type = [&](auto reverse) {
     if (dtype == BF16) by_size(bf16{}, reverse);
