@@ -46,43 +46,49 @@ _LOGPROB = struct.Struct("=2I3q2Q")
 _LOGPROB_OUT = struct.Struct("=6Q")
 
 
-class _Device:
-    """Makes a tensor's device current where it is not, for one call."""
-
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
-        self.other = None
-
-    def __enter__(self):
-        if self.index != torch.cuda.current_device():
-            self.other = torch.cuda.device(self.index)
-            self.other.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.other is not None:
-            self.other.__exit__(*exc)
-
-
-def _need(ok, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
-def _gpu(name: str, t, dtypes, shape, like: torch.Tensor) -> None:
-    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    _need(t.device == like.device, f"{name} is on {t.device}, not {like.device}")
-    _need(t.dtype in dtypes, f"{name} must be of type {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
-    _need(tuple(t.shape) == tuple(shape), f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-
-
-def _first(name: str, t, dims) -> None:
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a tensor on the GPU")
-    _need(t.dtype in _DTYPES, f"{name} must be float32 or bfloat16, not {t.dtype}")
-    _need(t.dim() in dims, f"{name} must have {' or '.join(str(d) for d in dims)} axes, not {t.dim()}")
-
-
 _F32 = (torch.float32,)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _run(entry, like: torch.Tensor, *args) -> None:
+    """An entry point on the tensor's device and torch's current stream there."""
+    index = like.get_device()
+    if index == _current_device():
+        code = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = entry(*args, _raw_stream(index))
+    if code:
+        _lib.check(code)
+
+
+# The checks pass in a comparison each; what they say is put together when they fail.
+def _gpu(name: str, t, dtypes, shape, like: torch.Tensor) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == shape and t.device == like.device:
+        return
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not {like.device}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be of type {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
+    raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _first(name: str, t, dims: int) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a tensor on the GPU")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be float32 or bfloat16, not {t.dtype}")
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} axes, not {t.dim()}")
+
+
+def _axes(name: str, t, dims: int, what: str) -> None:
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError(f"{name} must {what}")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -94,102 +100,124 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _strides(t: torch.Tensor, packed: bool, inner: int) -> tuple:
-    """(address, sequence, token and head strides); `inner` axes follow the token."""
+def _strides(t: torch.Tensor, packed: bool) -> tuple:
+    """(address, sequence, token and head strides) of [sequence, token, head, ..]."""
     s = t.stride()
-    at = 0 if packed else 1
-    return t.data_ptr(), 0 if packed else s[0], s[at], s[at + 1] if inner else 0
+    return (t.data_ptr(), 0, s[0], s[1]) if packed else (t.data_ptr(), s[0], s[1], s[2])
 
 
-def _workspace(entry: str, device, *args) -> tuple:
+def _strides2(t: torch.Tensor, packed: bool) -> tuple:
+    """The same of [sequence, token, channel]."""
+    s = t.stride()
+    return (t.data_ptr(), 0, s[0], 0) if packed else (t.data_ptr(), s[0], s[1], 0)
+
+
+def _workspace(entry, like: torch.Tensor, *args) -> tuple:
     size = ctypes.c_size_t()
-    _lib.call(entry, *args, ctypes.byref(size))
-    return torch.empty(size.value, dtype=torch.uint8, device=device), size.value
+    code = entry(*args, ctypes.byref(size))
+    if code:
+        _lib.check(code)
+    return torch.empty(size.value, dtype=torch.uint8, device=like.device), size.value
 
 
 def _offsets(cu_seqlens, like: torch.Tensor) -> None:
-    _need(isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2,
-          "cu_seqlens must be a vector of one offset more than there are sequences")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+        raise ValueError("cu_seqlens must be a vector of one offset more than there are sequences")
     _gpu("cu_seqlens", cu_seqlens, (torch.int32,), cu_seqlens.shape, like)
-    _need(cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous")
+    if not cu_seqlens.is_contiguous():
+        raise ValueError("cu_seqlens must be contiguous")
+
+
+def _wants_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                return True
+    return False
 
 
 # ----------------------------------------------------------------- selective scan
-class _ScanArgs:
-    """Checked arguments of a scan and their packed form.  Holds what the packed form points to."""
-
-    def __init__(self, x, write, log_decay, B, C, D, initial_state, cu_seqlens):
-        packed = cu_seqlens is not None
-        _first("x", x, (3,) if packed else (4,))
-        lead, (H, P) = x.shape[:-2], x.shape[-2:]
-        _need(isinstance(B, torch.Tensor) and B.dim() == x.dim(), f"B must have {x.dim()} axes")
-        G, N = B.shape[-2:]
-        _need(H >= 1 and P >= 1 and G >= 1 and N >= 1 and H % G == 0,
-              f"{H} heads do not divide into {G} groups")
-        _need(N <= MAX_STATES, f"{N} states: at most {MAX_STATES}")
-        _gpu("B", B, (x.dtype,), (*lead, G, N), x)
-        _gpu("C", C, (x.dtype,), (*lead, G, N), x)
-        _gpu("write", write, _F32, (*lead, H), x)
-        _gpu("log_decay", log_decay, _F32, (*lead, H), x)
-        if packed:
-            _offsets(cu_seqlens, x)
-        self.seqs = cu_seqlens.numel() - 1 if packed else lead[0]
-        self.tokens = lead[-1]
-        _need(self.seqs >= 1, "no sequences")
-        self.state_shape = (self.seqs, H, P, N)
-        if D is not None:
-            _gpu("D", D, _F32, (H,), x)
-            D = D.contiguous()
-        if initial_state is not None:
-            _gpu("initial_state", initial_state, _F32, self.state_shape, x)
-            initial_state = initial_state.contiguous()
-        x, B, C = _rows(x), _rows(B), _rows(C)
-        self.held = x, write, log_decay, B, C, D, initial_state, cu_seqlens
-        self.packed = _SCAN.pack(
-            _DTYPES[x.dtype], self.seqs, H, P, N, G, self.tokens, _ptr(cu_seqlens),
-            *_strides(x, packed, 1), *_strides(B, packed, 1), *_strides(C, packed, 1),
-            *_strides(write, packed, 1), *_strides(log_decay, packed, 1), _ptr(D), _ptr(initial_state))
+def _heads(H: int, P: int, G: int, N: int) -> None:
+    if min(H, P, G, N) < 1 or H % G:
+        raise ValueError(f"{H} heads do not divide into {G} groups")
+    if N > MAX_STATES:
+        raise ValueError(f"{N} states: at most {MAX_STATES}")
 
 
-def _scan_forward(args: _ScanArgs, return_state: bool):
-    x = args.held[0]
-    with _Device(x) as stream:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        state = torch.empty(args.state_shape, dtype=torch.float32, device=x.device) if return_state else None
-        space, size = _workspace("fhe_ssm_scan_workspace", x.device, args.packed, 0)
-        _lib.call("fhe_ssm_scan", args.packed, _ptr(y), _ptr(state), _ptr(space), size, stream)
+def _check_scan(x, write, log_decay, B, C, D, initial_state, cu_seqlens) -> None:
+    packed = cu_seqlens is not None
+    dims = 3 if packed else 4
+    _first("x", x, dims)
+    _axes("B", B, dims, f"have {dims} axes")
+    lead, (H, P), (G, N) = x.shape[:-2], x.shape[-2:], B.shape[-2:]
+    _heads(H, P, G, N)
+    _gpu("B", B, (x.dtype,), (*lead, G, N), x)
+    _gpu("C", C, (x.dtype,), B.shape, x)
+    _gpu("write", write, _F32, (*lead, H), x)
+    _gpu("log_decay", log_decay, _F32, (*lead, H), x)
+    if packed:
+        _offsets(cu_seqlens, x)
+    if lead[0] < 1 and not packed:
+        raise ValueError("no sequences")
+    if D is not None:
+        _gpu("D", D, _F32, (H,), x)
+    if initial_state is not None:
+        seqs = cu_seqlens.numel() - 1 if packed else lead[0]
+        _gpu("initial_state", initial_state, _F32, (seqs, H, P, N), x)
+
+
+def _pack_scan(x, write, log_decay, B, C, D, initial_state, cu_seqlens) -> tuple:
+    """(the packed arguments, the state's shape, the tensors that they point to)."""
+    packed = cu_seqlens is not None
+    x, B, C = _rows(x), _rows(B), _rows(C)
+    D = None if D is None else D.contiguous()
+    initial_state = None if initial_state is None else initial_state.contiguous()
+    (tokens, H, P), (G, N) = x.shape[-3:], B.shape[-2:]
+    seqs = cu_seqlens.numel() - 1 if packed else x.shape[0]
+    args = _SCAN.pack(
+        _DTYPES[x.dtype], seqs, H, P, N, G, tokens, _ptr(cu_seqlens), *_strides(x, packed), *_strides(B, packed),
+        *_strides(C, packed), *_strides(write, packed), *_strides(log_decay, packed), _ptr(D), _ptr(initial_state))
+    return args, (seqs, H, P, N), (x, B, C, D, initial_state)
+
+
+def _scan_forward(tensors, return_state: bool):
+    x = tensors[0]
+    args, state_shape, held = _pack_scan(*tensors)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    state = torch.empty(state_shape, dtype=torch.float32, device=x.device) if return_state else None
+    space, size = _workspace(_lib.lib.fhe_ssm_scan_workspace, x, args, 0)
+    _run(_lib.lib.fhe_ssm_scan, x, args, _ptr(y), _ptr(state), _ptr(space), size)
     return y, state
 
 
 class _Scan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, return_state, cu_seqlens, x, write, log_decay, B, C, D, initial_state):
-        args = _ScanArgs(x, write, log_decay, B, C, D, initial_state, cu_seqlens)
-        ctx.save_for_backward(x, write, log_decay, B, C, D, initial_state, cu_seqlens)
+    def forward(ctx, return_state, *tensors):
+        ctx.save_for_backward(*tensors)
         ctx.set_materialize_grads(False)
-        return _scan_forward(args, return_state)
+        return _scan_forward(tensors, return_state)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dstate):
-        x, write, log_decay, B, C, D, initial_state, cu_seqlens = ctx.saved_tensors
-        args = _ScanArgs(x, write, log_decay, B, C, D, initial_state, cu_seqlens)
+        tensors = ctx.saved_tensors
+        x, write, log_decay, B, C, D, initial_state, cu_seqlens = tensors
+        args, _, held = _pack_scan(*tensors)
         dy = torch.zeros_like(x) if dy is None else _rows(dy)
         dstate = None if dstate is None else dstate.contiguous()
 
         def new(like, wanted=True):
-            return torch.empty(like.shape, dtype=like.dtype, device=x.device) if wanted else None
+            if like is None or not wanted:
+                return None
+            return torch.empty(like.shape, dtype=like.dtype, device=like.device)
 
-        with _Device(x) as stream:
-            dx, dw, dg, dB, dC = (new(t) for t in (x, write, log_decay, B, C))
-            dD = None if D is None else new(D, ctx.needs_input_grad[7])
-            dh = None if initial_state is None else new(initial_state, ctx.needs_input_grad[8])
-            grads = _SCAN_GRADS.pack(
-                *_strides(dy, cu_seqlens is not None, 1), _ptr(dstate), _ptr(dx), _ptr(dw), _ptr(dg), _ptr(dB),
-                _ptr(dC), _ptr(dD), _ptr(dh))
-            space, size = _workspace("fhe_ssm_scan_workspace", x.device, args.packed, 1)
-            _lib.call("fhe_ssm_scan_backward", args.packed, grads, _ptr(space), size, stream)
-        return None, None, dx, dw, dg, dB, dC, dD, dh
+        dx, dw, dg, dB, dC = new(x), new(write), new(log_decay), new(B), new(C)
+        dD, dh = new(D, ctx.needs_input_grad[6]), new(initial_state, ctx.needs_input_grad[7])
+        grads = _SCAN_GRADS.pack(*_strides(dy, cu_seqlens is not None), _ptr(dstate), _ptr(dx), _ptr(dw), _ptr(dg),
+                                 _ptr(dB), _ptr(dC), _ptr(dD), _ptr(dh))
+        space, size = _workspace(_lib.lib.fhe_ssm_scan_workspace, x, args, 1)
+        _run(_lib.lib.fhe_ssm_scan_backward, x, args, grads, _ptr(space), size)
+        return None, dx, dw, dg, dB, dC, dD, dh, None
 
 
 def ssm_scan(x, write, log_decay, B, C, D=None, *, initial_state=None, cu_seqlens=None,
@@ -202,25 +230,27 @@ def ssm_scan(x, write, log_decay, B, C, D=None, *, initial_state=None, cu_seqlen
     head_dim, states] float32 (default zeros).  Returns y, or (y, the last states) with return_state.
     Differentiable in every tensor but cu_seqlens.  Products are of 16-bit pieces with 32-bit sums for
     bfloat16 (the state and the gradients keep at least 16 bits on the way), of 32 bits for float32."""
-    tensors = (x, write, log_decay, B, C, D, initial_state)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
-        y, state = _Scan.apply(return_state, cu_seqlens, *tensors)
+    tensors = (x, write, log_decay, B, C, D, initial_state, cu_seqlens)
+    _check_scan(*tensors)
+    if _wants_grad(*tensors):
+        y, state = _Scan.apply(return_state, *tensors)
     else:
-        y, state = _scan_forward(_ScanArgs(*tensors, cu_seqlens), return_state)
+        y, state = _scan_forward(tensors, return_state)
     return (y, state) if return_state else y
 
 
-def _no_grad(name: str, tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
-
-
-def _slots(slots, requests: int, cache: int, like: torch.Tensor) -> None:
+def _slots(slots, requests: int, state: torch.Tensor, like: torch.Tensor) -> None:
+    if requests < 1:
+        raise ValueError("no requests")
+    if not state.is_contiguous():
+        raise ValueError("state must be contiguous: it is updated in place")
     if slots is None:
-        _need(requests <= cache, f"{requests} requests and {cache} rows of the state")
+        if requests > state.shape[0]:
+            raise ValueError(f"{requests} requests and {state.shape[0]} rows of the state")
         return
     _gpu("slots", slots, (torch.int32,), (requests,), like)
-    _need(slots.is_contiguous(), "slots must be contiguous")
+    if not slots.is_contiguous():
+        raise ValueError("slots must be contiguous")
 
 
 def ssm_step(state, x, write, log_decay, B, C, D=None, *, slots=None):
@@ -229,98 +259,103 @@ def ssm_step(state, x, write, log_decay, B, C, D=None, *, slots=None):
     state [cache, heads, head_dim, states] float32 and contiguous, x [requests, heads, head_dim], the
     others alike.  slots [requests] int32 names each request's row (default its own number), no row
     twice; a slot outside of the cache is padding: its y is zero and no state changes.  Returns y."""
-    _first("x", x, (3,))
-    R, H, P = x.shape
-    _need(isinstance(B, torch.Tensor) and B.dim() == 3, "B must have 3 axes")
-    G, N = B.shape[-2:]
-    _need(R >= 1, "no requests")
-    _need(H >= 1 and P >= 1 and G >= 1 and N >= 1 and H % G == 0, f"{H} heads do not divide into {G} groups")
-    _need(N <= MAX_STATES, f"{N} states: at most {MAX_STATES}")
+    _first("x", x, 3)
+    _axes("B", B, 3, "have 3 axes")
+    _axes("state", state, 4, "have 4 axes")
+    (R, H, P), (G, N) = x.shape, B.shape[-2:]
+    _heads(H, P, G, N)
     _gpu("B", B, (x.dtype,), (R, G, N), x)
-    _gpu("C", C, (x.dtype,), (R, G, N), x)
+    _gpu("C", C, (x.dtype,), B.shape, x)
     _gpu("write", write, _F32, (R, H), x)
     _gpu("log_decay", log_decay, _F32, (R, H), x)
-    _need(isinstance(state, torch.Tensor) and state.dim() == 4 and state.shape[0] >= 1, "state must have 4 axes")
     _gpu("state", state, _F32, (state.shape[0], H, P, N), x)
-    _need(state.is_contiguous(), "state must be contiguous: it is updated in place")
     if D is not None:
         _gpu("D", D, _F32, (H,), x)
         D = D.contiguous()
-    _slots(slots, R, state.shape[0], x)
-    _no_grad("ssm_step", (state, x, write, log_decay, B, C, D))
+    _slots(slots, R, state, x)
+    if _wants_grad(state, x, write, log_decay, B, C, D):
+        raise ValueError("ssm_step has no gradient: call it under torch.no_grad()")
     x, B, C = _rows(x), _rows(B), _rows(C)
-    with _Device(x) as stream:
-        y = torch.empty((R, H, P), dtype=x.dtype, device=x.device)
-        args = _STEP.pack(_DTYPES[x.dtype], R, state.shape[0], H, P, N, G, _ptr(slots), *_strides(x, True, 1),
-                          *_strides(B, True, 1), *_strides(C, True, 1), *_strides(write, True, 1),
-                          *_strides(log_decay, True, 1), _ptr(D), state.data_ptr())
-        _lib.call("fhe_ssm_step", args, y.data_ptr(), stream)
+    y = torch.empty((R, H, P), dtype=x.dtype, device=x.device)
+    args = _STEP.pack(_DTYPES[x.dtype], R, state.shape[0], H, P, N, G, _ptr(slots), *_strides(x, True),
+                      *_strides(B, True), *_strides(C, True), *_strides(write, True), *_strides(log_decay, True),
+                      _ptr(D), state.data_ptr())
+    _run(_lib.lib.fhe_ssm_step, x, args, y.data_ptr())
     return y
 
 
 # ----------------------------------------------------------------- causal convolution
-class _ConvArgs:
-    def __init__(self, x, weight, bias, initial_state, cu_seqlens, silu):
-        packed = cu_seqlens is not None
-        _first("x", x, (2,) if packed else (3,))
-        Cn = x.shape[-1]
-        _need(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight must be [channels, taps]")
-        K = weight.shape[1]
-        _need(Cn >= 1 and 2 <= K <= MAX_TAPS, f"{K} taps: 2 to {MAX_TAPS}")
-        _gpu("weight", weight, _F32, (Cn, K), x)
-        weight = weight.contiguous()
-        if bias is not None:
-            _gpu("bias", bias, _F32, (Cn,), x)
-            bias = bias.contiguous()
-        if packed:
-            _offsets(cu_seqlens, x)
-        self.seqs = cu_seqlens.numel() - 1 if packed else x.shape[0]
-        _need(self.seqs >= 1, "no sequences")
-        self.state_shape = (self.seqs, K - 1, Cn)
-        if initial_state is not None:
-            _gpu("initial_state", initial_state, (x.dtype,), self.state_shape, x)
-            initial_state = initial_state.contiguous()
-        x = _rows(x)
-        self.held = x, weight, bias, initial_state, cu_seqlens
-        self.packed = _CONV.pack(_DTYPES[x.dtype], self.seqs, Cn, K, x.shape[-2], _ptr(cu_seqlens),
-                                 *_strides(x, packed, 0), _ptr(weight), _ptr(bias), _ptr(initial_state), int(silu))
+def _check_weight(weight, bias, x: torch.Tensor) -> int:
+    _axes("weight", weight, 2, "be [channels, taps]")
+    channels, taps = x.shape[-1], weight.shape[1]
+    if channels < 1 or not 2 <= taps <= MAX_TAPS:
+        raise ValueError(f"{taps} taps: 2 to {MAX_TAPS}")
+    _gpu("weight", weight, _F32, (channels, taps), x)
+    if bias is not None:
+        _gpu("bias", bias, _F32, (channels,), x)
+    return taps
 
 
-def _conv_forward(args: _ConvArgs, return_state: bool):
-    x = args.held[0]
-    with _Device(x) as stream:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        state = torch.empty(args.state_shape, dtype=x.dtype, device=x.device) if return_state else None
-        _lib.call("fhe_causal_conv", args.packed, _ptr(y), _ptr(state), stream)
+def _check_conv(x, weight, bias, initial_state, cu_seqlens) -> None:
+    packed = cu_seqlens is not None
+    _first("x", x, 2 if packed else 3)
+    taps = _check_weight(weight, bias, x)
+    if packed:
+        _offsets(cu_seqlens, x)
+    seqs = cu_seqlens.numel() - 1 if packed else x.shape[0]
+    if seqs < 1:
+        raise ValueError("no sequences")
+    if initial_state is not None:
+        _gpu("initial_state", initial_state, (x.dtype,), (seqs, taps - 1, x.shape[-1]), x)
+
+
+def _pack_conv(x, weight, bias, initial_state, cu_seqlens, silu) -> tuple:
+    """(the packed arguments, the state's shape, the tensors that they point to)."""
+    packed = cu_seqlens is not None
+    x, weight = _rows(x), weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    initial_state = None if initial_state is None else initial_state.contiguous()
+    seqs = cu_seqlens.numel() - 1 if packed else x.shape[0]
+    channels, taps = weight.shape
+    args = _CONV.pack(_DTYPES[x.dtype], seqs, channels, taps, x.shape[-2], _ptr(cu_seqlens), *_strides2(x, packed),
+                      _ptr(weight), _ptr(bias), _ptr(initial_state), int(silu))
+    return args, (seqs, taps - 1, channels), (x, weight, bias, initial_state)
+
+
+def _conv_forward(tensors, silu: bool, return_state: bool):
+    x = tensors[0]
+    args, state_shape, held = _pack_conv(*tensors, silu)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    state = torch.empty(state_shape, dtype=x.dtype, device=x.device) if return_state else None
+    _run(_lib.lib.fhe_causal_conv, x, args, _ptr(y), _ptr(state))
     return y, state
 
 
 class _Conv(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, return_state, cu_seqlens, silu, x, weight, bias, initial_state):
-        args = _ConvArgs(x, weight, bias, initial_state, cu_seqlens, silu)
-        ctx.save_for_backward(x, weight, bias, initial_state, cu_seqlens)
+    def forward(ctx, return_state, silu, *tensors):
+        ctx.save_for_backward(*tensors)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
-        return _conv_forward(args, return_state)
+        return _conv_forward(tensors, silu, return_state)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dstate):
-        x, weight, bias, initial_state, cu_seqlens = ctx.saved_tensors
-        args = _ConvArgs(x, weight, bias, initial_state, cu_seqlens, ctx.silu)
+        tensors = ctx.saved_tensors
+        x, weight, bias, initial_state, cu_seqlens = tensors
+        args, state_shape, held = _pack_conv(*tensors, ctx.silu)
         dy = torch.zeros_like(x) if dy is None else _rows(dy)
         dstate = None if dstate is None else dstate.contiguous()
-        with _Device(x) as stream:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            dw = torch.empty(weight.shape, dtype=torch.float32, device=x.device)
-            db = None if bias is None else torch.empty(bias.shape, dtype=torch.float32, device=x.device)
-            dh = None if initial_state is None else torch.empty(args.state_shape, dtype=x.dtype, device=x.device)
-            grads = _CONV_GRADS.pack(*_strides(dy, cu_seqlens is not None, 0), _ptr(dstate), _ptr(dx), _ptr(dw),
-                                     _ptr(db), _ptr(dh))
-            space, size = _workspace("fhe_causal_conv_workspace", x.device, args.packed)
-            _lib.call("fhe_causal_conv_backward", args.packed, grads, _ptr(space), size, stream)
-        return None, None, None, dx, dw, db, dh
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty(weight.shape, dtype=torch.float32, device=x.device)
+        db = None if bias is None else torch.empty(bias.shape, dtype=torch.float32, device=x.device)
+        dh = None if initial_state is None else torch.empty(state_shape, dtype=x.dtype, device=x.device)
+        grads = _CONV_GRADS.pack(*_strides2(dy, cu_seqlens is not None), _ptr(dstate), _ptr(dx), _ptr(dw), _ptr(db),
+                                 _ptr(dh))
+        space, size = _workspace(_lib.lib.fhe_causal_conv_workspace, x, args)
+        _run(_lib.lib.fhe_causal_conv_backward, x, args, grads, _ptr(space), size)
+        return None, None, dx, dw, db, dh, None
 
 
 def causal_conv(x, weight, bias=None, *, initial_state=None, cu_seqlens=None, silu: bool = True,
@@ -331,39 +366,32 @@ def causal_conv(x, weight, bias=None, *, initial_state=None, cu_seqlens=None, si
     [sequences, taps - 1, channels] of x's type holds the inputs before each sequence's first, oldest
     first (default zeros).  silu=False leaves the sums as they are.  Returns y, or (y, each sequence's
     last taps - 1 inputs) with return_state.  Differentiable in every tensor but cu_seqlens."""
-    tensors = (x, weight, bias, initial_state)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
-        y, state = _Conv.apply(return_state, cu_seqlens, silu, *tensors)
+    tensors = (x, weight, bias, initial_state, cu_seqlens)
+    _check_conv(*tensors)
+    if _wants_grad(*tensors):
+        y, state = _Conv.apply(return_state, silu, *tensors)
     else:
-        y, state = _conv_forward(_ConvArgs(*tensors, cu_seqlens, silu), return_state)
+        y, state = _conv_forward(tensors, silu, return_state)
     return (y, state) if return_state else y
 
 
 def causal_conv_step(state, x, weight, bias=None, *, silu: bool = True, slots=None):
     """One token of each request: causal_conv on state[slots] [cache, taps - 1, channels], which moves
     on by x [requests, channels] in place.  slots as in ssm_step.  Returns y [requests, channels]."""
-    _first("x", x, (2,))
-    R, Cn = x.shape
-    _need(R >= 1, "no requests")
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight must be [channels, taps]")
-    K = weight.shape[1]
-    _need(Cn >= 1 and 2 <= K <= MAX_TAPS, f"{K} taps: 2 to {MAX_TAPS}")
-    _gpu("weight", weight, _F32, (Cn, K), x)
-    weight = weight.contiguous()
-    if bias is not None:
-        _gpu("bias", bias, _F32, (Cn,), x)
-        bias = bias.contiguous()
-    _need(isinstance(state, torch.Tensor) and state.dim() == 3 and state.shape[0] >= 1, "state must have 3 axes")
-    _gpu("state", state, (x.dtype,), (state.shape[0], K - 1, Cn), x)
-    _need(state.is_contiguous(), "state must be contiguous: it is updated in place")
-    _slots(slots, R, state.shape[0], x)
-    _no_grad("causal_conv_step", (state, x, weight, bias))
-    x = _rows(x)
-    with _Device(x) as stream:
-        y = torch.empty((R, Cn), dtype=x.dtype, device=x.device)
-        args = _CONV_STEP.pack(_DTYPES[x.dtype], R, state.shape[0], Cn, K, _ptr(slots), *_strides(x, True, 0),
-                               _ptr(weight), _ptr(bias), state.data_ptr(), int(silu))
-        _lib.call("fhe_causal_conv_step", args, y.data_ptr(), stream)
+    _first("x", x, 2)
+    _axes("state", state, 3, "have 3 axes")
+    taps = _check_weight(weight, bias, x)
+    R, channels = x.shape
+    _gpu("state", state, (x.dtype,), (state.shape[0], taps - 1, channels), x)
+    _slots(slots, R, state, x)
+    if _wants_grad(state, x, weight, bias):
+        raise ValueError("causal_conv_step has no gradient: call it under torch.no_grad()")
+    x, weight = _rows(x), weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty((R, channels), dtype=x.dtype, device=x.device)
+    args = _CONV_STEP.pack(_DTYPES[x.dtype], R, state.shape[0], channels, taps, _ptr(slots), *_strides2(x, True),
+                           _ptr(weight), _ptr(bias), state.data_ptr(), int(silu))
+    _run(_lib.lib.fhe_causal_conv_step, x, args, y.data_ptr())
     return y
 
 
@@ -384,17 +412,16 @@ def _logprob_args(logits, targets, top: int) -> bytes:
 
 def _logprob_forward(logits, targets, top: int):
     rows = logits.shape[0]
-    with _Device(logits) as stream:
-        stats = torch.empty((4, rows), dtype=torch.float32, device=logits.device)
-        best = index = None
-        if top:
-            best = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-            index = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-        args = _logprob_args(logits, targets, top)
-        at = stats.data_ptr()
-        out = _LOGPROB_OUT.pack(at, at + 4 * rows, at + 8 * rows, at + 12 * rows, _ptr(best), _ptr(index))
-        space, size = _workspace("fhe_token_logprobs_workspace", logits.device, args)
-        _lib.call("fhe_token_logprobs", args, out, _ptr(space), size, stream)
+    stats = torch.empty((4, rows), dtype=torch.float32, device=logits.device)
+    best = index = None
+    if top:
+        best = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+        index = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+    args = _logprob_args(logits, targets, top)
+    at = stats.data_ptr()
+    out = _LOGPROB_OUT.pack(at, at + 4 * rows, at + 8 * rows, at + 12 * rows, _ptr(best), _ptr(index))
+    space, size = _workspace(_lib.lib.fhe_token_logprobs_workspace, logits, args)
+    _run(_lib.lib.fhe_token_logprobs, logits, args, out, _ptr(space), size)
     return stats, best, index
 
 
@@ -414,10 +441,9 @@ class _Logprobs(torch.autograd.Function):
         logits, targets, stats = ctx.saved_tensors
         at, rows = stats.data_ptr(), logits.shape[0]  # entropy, peak, log sum
         dlogprob, dentropy = (None if d is None else d.contiguous() for d in (dlogprob, dentropy))
-        with _Device(logits) as stream:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            _lib.call("fhe_token_logprobs_backward", _logprob_args(logits, targets, 0), at + 4 * rows,
-                      at + 8 * rows, at, _ptr(dlogprob), _ptr(dentropy), _ptr(grad), stream)
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _run(_lib.lib.fhe_token_logprobs_backward, logits, _logprob_args(logits, targets, 0), at + 4 * rows,
+             at + 8 * rows, at, _ptr(dlogprob), _ptr(dentropy), _ptr(grad))
         return grad, None, None
 
 
@@ -428,26 +454,33 @@ def token_logprobs(logits, targets, *, top: int = 0) -> TokenLogprobs:
     A target below 0 is left out: log probability 0 and no gradient from it; one of vocab or more
     gives NaN.  A logit of -inf is a token that is not allowed; a row of nothing else has log
     probability -inf, entropy 0 and gradient 0.  logprob and entropy are differentiable in logits."""
-    _need(isinstance(logits, torch.Tensor) and logits.is_cuda, "logits must be a tensor on the GPU")
-    _need(logits.dtype in _DTYPES, f"logits must be float32 or bfloat16, not {logits.dtype}")
-    _need(logits.dim() >= 1 and logits.shape[-1] >= 1, "logits must have a vocabulary axis")
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise ValueError("logits must be a tensor on the GPU")
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"logits must be float32 or bfloat16, not {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits must have a vocabulary axis")
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     _gpu("targets", targets, (torch.int64,), lead, logits)
-    _need(0 <= top <= min(MAX_TOP, vocab), f"top must be 0 to {min(MAX_TOP, vocab)}")
-    flat = _rows(logits.reshape(-1, vocab))
-    if flat.shape[0] == 0:
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}")
+    flat = logits.dim() == 2
+    rows = _rows(logits if flat else logits.reshape(-1, vocab))
+    if rows.shape[0] == 0:
         empty = logits.sum(-1).float()
         return TokenLogprobs(empty, empty, *((empty.new_empty((*lead, top)),
                                               torch.empty((*lead, top), dtype=torch.int32, device=logits.device))
                                              if top else (None, None)))
-    if flat.shape[0] > 1 and flat.stride(0) < vocab:  # one row for all
-        flat = flat.contiguous()
-    targets = targets.reshape(-1).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        logprob, entropy, best, index = _Logprobs.apply(flat, targets, top)
+    if rows.shape[0] > 1 and rows.stride(0) < vocab:  # one row for all
+        rows = rows.contiguous()
+    targets = (targets if flat else targets.reshape(-1)).contiguous()
+    if _wants_grad(logits):
+        logprob, entropy, best, index = _Logprobs.apply(rows, targets, top)
     else:
-        stats, best, index = _logprob_forward(flat, targets, top)
+        stats, best, index = _logprob_forward(rows, targets, top)
         logprob, entropy = stats[0], stats[1]
+    if flat:
+        return TokenLogprobs(logprob, entropy, best, index)
     return TokenLogprobs(logprob.reshape(lead), entropy.reshape(lead),
                          None if best is None else best.reshape(*lead, top),
                          None if index is None else index.reshape(*lead, top))
