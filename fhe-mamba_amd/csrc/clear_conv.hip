@@ -2,8 +2,9 @@
 // form:  y_t = act(bias + sum_k weight_k x_{t - taps + 1 + k}).
 //
 // Bound by memory: a thread keeps the window of its channels (16 bytes of a
-// token) in registers and walks a run of tokens, so that an input is read once
-// and, at the start of a run, taps - 1 times more, which the caches answer.
+// token) in registers and walks a run of tokens, four loads ahead, so that an
+// input is read once and, at the start of a run, taps - 1 times more, which the
+// caches answer.
 // Before a sequence's first token the window holds its initial state, oldest
 // first, or zeros.
 #pragma clang fp contract(fast)
@@ -14,6 +15,13 @@
 namespace fhe::clear {
 namespace {
 
+constexpr int RUN = 16, AHEAD = 4;  // tokens of a run; loads ahead
+// A backward workgroup: BACK_RUNS runs of BACK_PIECES pieces of the channels,
+// whose weights' gradients it sums before it writes them.
+// The pieces are of at most four channels: of eight, a thread's weights, their
+// gradients, its window and its inputs' take 232 registers.
+constexpr int RUN_BACK = 16, BACK_PIECES = 32, BACK_RUNS = 8;
+
 struct ConvArgs {
   Conv c;
   void* y;
@@ -23,7 +31,7 @@ struct ConvArgs {
   const void* dfinal;
   void* dx;
   void* dinitial;
-  float* parts;    // [runs][taps + 1][channels]
+  float* parts;    // [workgroups' runs][taps + 1][channels]
   int run, runs;   // tokens of a run; runs of all tokens (packed) or of one sequence
   int pieces;      // ceil(channels / elements of a thread)
 };
@@ -56,46 +64,44 @@ struct Piece {
   float v[VEC];
 };
 
-// Elements [0, count) of a thread's channels at p; zeros past them.
+// A thread's channels as they lie in memory.
 template <class T, int VEC>
-__device__ __forceinline__ Piece<T, VEC> read(const T* p, int count) {
-  Piece<T, VEC> r;
-  if constexpr (VEC == 1) {
-    r.v[0] = (float)*p;
+struct Raw {
+  union {
+    uint32_t w __attribute__((ext_vector_type(VEC * sizeof(T) < 4 ? 1 : VEC * sizeof(T) / 4)));
+    T e[VEC];
+  };
+  __device__ __forceinline__ operator Piece<T, VEC>() const {
+    Piece<T, VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.v[i] = (float)e[i];
+    return r;
+  }
+};
+
+// Elements [0, count) of them at p; zeros past the count.
+template <class T, int VEC>
+__device__ __forceinline__ Raw<T, VEC> read(const T* p, int count) {
+  Raw<T, VEC> r;
+  if (VEC > 1 && count >= VEC) {
+    r.w = *reinterpret_cast<const decltype(r.w)*>(p);
   } else {
-    if (count >= VEC) {
-      union {
-        u32x4 w;
-        T e[VEC];
-      } u;
-      u.w = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) r.v[i] = (float)u.e[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) r.v[i] = i < count ? (float)p[i] : 0.0f;
-    }
+    for (int i = 0; i < VEC; ++i) r.e[i] = VEC == 1 || i < count ? p[i] : (T)0.0f;
   }
   return r;
 }
 template <class T, int VEC>
-__device__ __forceinline__ void write(T* p, const Piece<T, VEC>& r, int count) {
-  if constexpr (VEC == 1) {
-    *p = (T)r.v[0];
+__device__ __forceinline__ void write(T* p, const Piece<T, VEC>& v, int count) {
+  Raw<T, VEC> r;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r.e[i] = (T)v.v[i];
+  if (VEC > 1 && count >= VEC) {
+    *reinterpret_cast<decltype(r.w)*>(p) = r.w;
   } else {
-    union {
-      u32x4 w;
-      T e[VEC];
-    } u;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) u.e[i] = (T)r.v[i];
-    if (count >= VEC) {
-      *reinterpret_cast<u32x4*>(p) = u.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i < count) p[i] = u.e[i];
-    }
+    for (int i = 0; i < VEC; ++i)
+      if (VEC == 1 || i < count) p[i] = r.e[i];
   }
 }
 
@@ -128,7 +134,12 @@ __device__ __forceinline__ void add_taps(float (&v)[VEC], const float (&w)[KT][V
   }
 }
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
+// From the hardware's 2^x and reciprocal, each good to about a unit in the last
+// place: with the exact functions the arithmetic takes twice as long as the
+// memory.
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
 
 // The input at position t of a sequence (in its numbering, begin its first
 // token): its tokens, before them its initial state, before that nothing.
@@ -183,6 +194,7 @@ __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
   T* y = (T*)a.y + (c.offsets ? 0 : (int64_t)seq * c.tokens * c.channels) + c0;
 
   Piece<T, VEC> window[KT];
+  Raw<T, VEC> next[AHEAD];
   int t = t0;
   while (t < t1) {
     const Span s = c.offsets ? find_span(c, t) : Span{seq, 0, (int)c.tokens};
@@ -193,8 +205,16 @@ __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < KT - 1; ++k) window[k] = input_at<T, VEC>(c, x, s, t - (KT - 1) + k, c0, count);
-    for (; t < end; ++t) {
-      window[KT - 1] = read<T, VEC>(x + t * c.x.tok + c0, count);
+    for (int ahead = 0; t < end; ++t, --ahead) {
+      if (ahead == 0) {
+        ahead = AHEAD;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+          if (t + u < end) next[u] = read<T, VEC>(x + (t + u) * c.x.tok + c0, count);
+      }
+      window[KT - 1] = next[0];
+#pragma unroll
+      for (int u = 0; u + 1 < AHEAD; ++u) next[u] = next[u + 1];
       Piece<T, VEC> out;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) out.v[i] = b[i];
@@ -215,31 +235,11 @@ __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
 // begins in it) and so walks taps - 1 tokens further, whose d it makes again,
 // and sums the weights' gradients over its own tokens.
 template <class T, int VEC, int KT>
-__global__ __launch_bounds__(256) void k_conv_back(ConvArgs a) {
+__device__ __forceinline__ void conv_back_run(const ConvArgs& a, int64_t job, int c0, int count,
+                                              float (&dw)[KT][VEC], float (&db)[VEC]) {
   const Conv& c = a.c;
-  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int piece = (int)(at % a.pieces);
-  const int64_t job = at / a.pieces;
-  const int c0 = piece * VEC, count = min(VEC, c.channels - c0);
-  const int64_t jobs = c.offsets ? a.runs : (int64_t)a.runs * c.seqs;
   const int keep = c.taps - 1;
-  if (job >= jobs) {
-    // the initial states of empty sequences, which no run visits
-    const int64_t row = job - jobs;
-    if (!a.dinitial || row >= (int64_t)c.seqs * keep) return;
-    const int seq = (int)(row / keep);
-    int begin = 0, end = (int)c.tokens;
-    if (c.offsets) {
-      begin = min(max(c.offsets[seq], 0), (int)c.tokens);
-      end = min(c.offsets[seq + 1], (int)c.tokens);
-    }
-    if (end > begin) return;
-    Piece<T, VEC> p = {};
-    if (a.dfinal) p = read<T, VEC>((const T*)a.dfinal + row * c.channels + c0, count);
-    write<T, VEC>((T*)a.dinitial + row * c.channels + c0, p, count);
-    return;
-  }
-  float w[KT][VEC], b[VEC], dw[KT][VEC] = {}, db[VEC] = {};
+  float w[KT][VEC], b[VEC];
   read_weights<VEC, KT>(c.weight, c.bias, c0, count, c.taps, w, b);
   const int seq = c.offsets ? 0 : (int)(job / a.runs);
   const int t0 = (int)(c.offsets ? job : job % a.runs) * a.run, t1 = min(t0 + a.run, (int)c.tokens);
@@ -317,34 +317,66 @@ __global__ __launch_bounds__(256) void k_conv_back(ConvArgs a) {
     for (int k = 0; k < KT - 1; ++k) emit(last - (KT - 1) + k, grad[k]);
     t = own;
   }
-  float* part = a.parts + job * (c.taps + 1) * c.channels + c0;
-#pragma unroll
-  for (int k = 0; k < KT; ++k) {
-    const int tap = k - (KT - c.taps);
-    if (tap >= 0) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i < count) part[(int64_t)tap * c.channels + i] = dw[k][i];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    if (i < count) part[(int64_t)c.taps * c.channels + i] = db[i];
 }
 
-// Sums the runs' parts: 64 channels a workgroup, its four wavefronts a quarter
-// of the runs each.
-__global__ __launch_bounds__(256) void k_conv_sum(const float* parts, int64_t runs, int channels, int taps,
-                                                  float* dweight, float* dbias) {
-  __shared__ float sums[4][64];
+// The gradients of the initial states of empty sequences, which no run visits.
+template <class T>
+__global__ __launch_bounds__(256) void k_conv_empty(ConvArgs a) {
+  const Conv& c = a.c;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, size = (int64_t)(c.taps - 1) * c.channels;
+  const int seq = (int)(at / size);
+  if (seq >= c.seqs) return;
+  int begin = 0, end = (int)c.tokens;
+  if (c.offsets) {
+    begin = min(max(c.offsets[seq], 0), (int)c.tokens);
+    end = min(c.offsets[seq + 1], (int)c.tokens);
+  }
+  if (end <= begin) ((T*)a.dinitial)[at] = a.dfinal ? ((const T*)a.dfinal)[at] : (T)0.0f;
+}
+
+template <class T, int VEC, int KT>
+__global__ __launch_bounds__(256) void k_conv_back(ConvArgs a) {
+  const Conv& c = a.c;
+  const int lane = threadIdx.x % BACK_PIECES, line = threadIdx.x / BACK_PIECES;
+  const int c0 = (blockIdx.y * BACK_PIECES + lane) * VEC, count = min(VEC, c.channels - c0);
+  const int64_t job = (int64_t)blockIdx.x * BACK_RUNS + line;
+  const int64_t jobs = c.offsets ? a.runs : (int64_t)a.runs * c.seqs;
+  float dw[KT][VEC] = {}, db[VEC] = {};
+  if (count > 0 && job < jobs) conv_back_run<T, VEC, KT>(a, job, c0, count, dw, db);
+  // the workgroup's runs, in order
+  __shared__ float sums[BACK_RUNS][BACK_PIECES * VEC + 1];
+#pragma unroll
+  for (int k = 0; k <= KT; ++k) {
+    const int tap = k - (KT - c.taps);
+    if (tap < 0) continue;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sums[line][lane * VEC + i] = k < KT ? dw[k < KT ? k : 0][i] : db[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < BACK_PIECES * VEC; e += 256) {
+      const int ch = blockIdx.y * BACK_PIECES * VEC + e;
+      float sum = sums[0][e];
+#pragma unroll
+      for (int r = 1; r < BACK_RUNS; ++r) sum += sums[r][e];
+      if (ch < c.channels) a.parts[((int64_t)blockIdx.x * (c.taps + 1) + tap) * c.channels + ch] = sum;
+    }
+    __syncthreads();
+  }
+}
+// Sums the workgroups' parts: 64 channels a workgroup, each of its sixteen
+// wavefronts every sixteenth part.
+__global__ __launch_bounds__(1024) void k_conv_sum(const float* parts, int64_t count, int channels, int taps,
+                                                   float* dweight, float* dbias) {
+  __shared__ float sums[16][64];
   const int ch = blockIdx.x * 64 + (threadIdx.x & 63), k = blockIdx.y, wave = threadIdx.x >> 6;
   float sum = 0.0f;
-  if (ch < channels)
-    for (int64_t r = wave; r < runs; r += 4) sum += parts[(r * (taps + 1) + k) * channels + ch];
+  if (ch < channels) {
+#pragma unroll 4
+    for (int64_t r = wave; r < count; r += 16) sum += parts[(r * (taps + 1) + k) * channels + ch];
+  }
   sums[wave][threadIdx.x & 63] = sum;
   __syncthreads();
   if (wave || ch >= channels) return;
-  sum = (sums[0][ch & 63] + sums[1][ch & 63]) + (sums[2][ch & 63] + sums[3][ch & 63]);
+  for (int w = 1; w < 16; ++w) sum += sums[w][threadIdx.x & 63];
   if (k < taps) dweight[(int64_t)ch * taps + k] = sum;
   else if (dbias) dbias[ch] = sum;
 }
@@ -410,19 +442,19 @@ bool wide_rows(const Strided& t, uint32_t dtype, bool packed) {
   return aligned(t.p) && t.tok % vec == 0 && (packed || t.seq % vec == 0);
 }
 
-constexpr int RUN = 16, RUN_BACK = 32;
-
 int64_t jobs_of(const Conv& c, int run) {
   const int64_t runs = (c.tokens + run - 1) / run;
   return c.offsets ? runs : runs * c.seqs;
 }
+
+int64_t parts_of(const Conv& c) { return (jobs_of(c, RUN_BACK) + BACK_RUNS - 1) / BACK_RUNS; }
 
 uint32_t grid_of(int64_t threads) { return (uint32_t)((threads + 255) / 256); }
 
 }  // namespace
 
 size_t conv_workspace(const Conv& c) {
-  return (size_t)jobs_of(c, RUN_BACK) * (c.taps + 1) * c.channels * sizeof(float);
+  return (size_t)parts_of(c) * (c.taps + 1) * c.channels * sizeof(float);
 }
 
 void conv(const Conv& c, void* y, void* final_state, hipStream_t stream) {
@@ -457,16 +489,19 @@ void conv_backward(const Conv& c, const ConvGrads& g, void* workspace, hipStream
   const bool wide = c.channels % vec_of(c.dtype) == 0 && wide_rows(c.x, c.dtype, c.offsets) &&
                     wide_rows(g.dy, c.dtype, c.offsets) && aligned(g.dx) && aligned(c.initial) &&
                     aligned(g.dfinal) && aligned(g.dinitial);
-  const int64_t jobs = jobs_of(c, RUN_BACK);
+  const int64_t parts = parts_of(c);
   dispatch(c.dtype, wide, c.taps, [&](auto zero, auto vec, auto kt) {
     using T = decltype(zero);
-    a.pieces = (c.channels + vec() - 1) / vec();
-    const int64_t rows = jobs + (g.dinitial ? (int64_t)c.seqs * (c.taps - 1) : 0);
-    if (!rows) return;
-    k_conv_back<T, vec(), kt()><<<grid_of(rows * a.pieces), 256, 0, stream>>>(a);
+    if (parts) {
+      constexpr int VEC = vec() > 4 ? 4 : vec();
+      const dim3 grid((uint32_t)parts, (c.channels + BACK_PIECES * VEC - 1) / (BACK_PIECES * VEC));
+      k_conv_back<T, VEC, kt()><<<grid, BACK_PIECES * BACK_RUNS, 0, stream>>>(a);
+    }
+    if (g.dinitial && (c.offsets || !c.tokens))
+      k_conv_empty<T><<<grid_of((int64_t)c.seqs * (c.taps - 1) * c.channels), 256, 0, stream>>>(a);
   });
   hip_check(hipGetLastError(), "convolution gradient");
-  k_conv_sum<<<dim3((c.channels + 63) / 64, c.taps + 1), 256, 0, stream>>>(a.parts, jobs, c.channels, c.taps,
+  k_conv_sum<<<dim3((c.channels + 63) / 64, c.taps + 1), 1024, 0, stream>>>(a.parts, parts, c.channels, c.taps,
                                                                            g.dweight, g.dbias);
   hip_check(hipGetLastError(), "convolution gradient sums");
 }

@@ -20,6 +20,7 @@ namespace fhe::clear {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MAX_SPLITS = 64;  // workgroups of a row
 constexpr int THREADS = 256, TILE = 16 * THREADS;  // logits of a workgroup at a time
 
 // Sums relative to a maximum.
@@ -109,18 +110,19 @@ __device__ __forceinline__ int row_lead(const T* row) {
 __device__ __forceinline__ Stats add16(Stats a, const float* v) {
   float m = a.m;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) m = fmaxf(m, v[j]);
-  bool nan = false;
+  for (int j = 0; j < 16; ++j) m = fmaxf(m, v[j]);  // passes over NaN, which the sums carry
+  if (m == -INFINITY) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) nan |= v[j] != v[j];
-  if (nan) m = NAN;
-  if (m == -INFINITY) return a;
+    for (int j = 0; j < 16; ++j)
+      if (v[j] != v[j]) a = {NAN, NAN, NAN};
+    return a;
+  }
   Stats b{m, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     const float d = v[j] - m, e = __builtin_amdgcn_exp2f(d * LOG2E);
     b.s += e;
-    b.u += e == 0.0f ? 0.0f : e * d;
+    b.u += e * fmaxf(d, -1e3f);  // 0 where e is, and not 0 times infinity
   }
   return join(b, a);
 }
@@ -128,12 +130,12 @@ __device__ __forceinline__ Stats add16(Stats a, const float* v) {
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 // The `top` largest of this tile's keys and the `top` that `best` holds (0: an
-// empty place), in order, to `best`.  The top-th largest of the threads' own
-// maxima bounds the entry wanted from below, and only the `top` threads at or
-// over it can hold entries that large: the candidates are at most 16 top.
+// empty place), in order, to `best`.  The threads are 64 groups of four, one of
+// each wavefront; the top-th largest of the groups' maxima bounds the entry wanted
+// from below, and only the `top` groups at or over it can hold entries that
+// large: the candidates are at most 64 top, and hardly more than top.
 struct TopLds {
-  uint64_t maxima[THREADS], best[MAX_TOP], candidate[16 * MAX_TOP + MAX_TOP];
-  uint64_t bound;
+  uint64_t maxima[THREADS], best[MAX_TOP], candidate[64 * MAX_TOP + MAX_TOP];
   int count;
 };
 
@@ -146,16 +148,28 @@ __device__ void keep_best(TopLds& lds, const float* v, int64_t base, int64_t voc
     if (c >= 0 && c < vocab) mine = max64(mine, to_key(v[j], (uint32_t)c));
   }
   lds.maxima[threadIdx.x] = mine;
-  if (threadIdx.x == 0) {
-    lds.count = 0;
-    lds.bound = 0;  // fewer than `top` threads with entries: all are candidates
-  }
+  if (threadIdx.x == 0) lds.count = 0;
   __syncthreads();
+  const int lane = lane_id();
+  uint64_t group = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) group = max64(group, lds.maxima[64 * w + lane]);
   int rank = 0;
-  for (int i = 0; i < THREADS; ++i) rank += lds.maxima[i] > mine;
-  if (mine && rank == top - 1) lds.bound = mine;
-  __syncthreads();
-  const uint64_t bound = max64(lds.bound, lds.best[top - 1]);
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)group, i);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(group >> 32), i);
+    rank += ((uint64_t)hi << 32 | lo) > group;
+  }
+  // fewer than `top` groups with entries: all are candidates
+  const uint64_t found = __ballot(group && rank == top - 1);
+  uint64_t bound = lds.best[top - 1];
+  if (found) {
+    const int at = __builtin_ctzll(found);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)group, at);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(group >> 32), at);
+    bound = max64(bound, (uint64_t)hi << 32 | lo);
+  }
   if (mine && mine >= bound) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -245,8 +259,10 @@ __global__ __launch_bounds__(THREADS) void k_row_join(RowArgs a) {
   }
   if (!a.l.top) return;
   __syncthreads();
-  const uint64_t* best = a.best + row_i * a.splits * a.l.top;
+  __shared__ uint64_t best[MAX_SPLITS * MAX_TOP];
   const int count = a.splits * a.l.top;
+  for (int i = threadIdx.x; i < count; i += THREADS) best[i] = a.best[row_i * count + i];
+  __syncthreads();
   for (int i = threadIdx.x; i < count; i += THREADS) {
     const uint64_t k = best[i];
     if (!k) continue;
@@ -270,8 +286,11 @@ struct BackArgs {
 template <class T>
 __global__ __launch_bounds__(THREADS) void k_row_back(BackArgs a) {
   constexpr int VEC = Num<T>::VEC;
-  const int64_t row_i = blockIdx.x / a.splits;
-  const int split = blockIdx.x % a.splits;
+  // the last rows first: the forward call read them last, and what of them is
+  // still in the last-level cache is read from there
+  const uint32_t block = gridDim.x - 1 - blockIdx.x;
+  const int64_t row_i = block / a.splits;
+  const int split = block % a.splits;
   const T* row = (const T*)a.l.logits + row_i * a.l.row_stride;
   T* out = (T*)a.out + row_i * a.l.vocab;
   const int lead = row_lead(row);
@@ -318,7 +337,7 @@ int64_t tiles_of(const Logprob& l) { return (l.vocab + 7 + TILE - 1) / TILE; }
 // four a CU in all; the parts' best entries are joined by comparing all pairs.
 int splits_of(const Logprob& l) {
   const int64_t tiles = tiles_of(l), want = std::max<int64_t>(1, 4096 / l.rows);
-  return (int)std::min<int64_t>({tiles, want, 64});
+  return (int)std::min<int64_t>({tiles, want, MAX_SPLITS});
 }
 
 }  // namespace

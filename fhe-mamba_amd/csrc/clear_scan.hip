@@ -32,58 +32,42 @@ namespace {
 // a partition whatever they hold: clamped to the tokens and made to rise.  The
 // tokens before the first and after the last sequence are items without one;
 // entries past the last item are empty.
-__global__ __launch_bounds__(256) void k_items(const int* offsets, int seqs, int tokens, int length,
-                                               bool keep_empty, int items, Item* table, int* first) {
-  __shared__ int most[256], sum[256];
-  __shared__ int carry_most, carry_sum;
-  const int i = threadIdx.x;
-  if (i == 0) {
-    carry_most = 0;
-    carry_sum = 0;
-  }
-  __syncthreads();
+__global__ __launch_bounds__(64) void k_items(const int* offsets, int seqs, int tokens, int length,
+                                              bool keep_empty, int items, Item* table, int* first) {
+  const int lane = lane_id();
   const int start0 = min(max(offsets[0], 0), tokens);
-  for (int s0 = 0; s0 < seqs; s0 += 256) {
-    const int s = s0 + i;
-    // ends of the sequences, rising
-    most[i] = s < seqs ? min(max(offsets[s + 1], start0), tokens) : 0;
-    __syncthreads();
-    for (int d = 1; d < 256; d *= 2) {
-      const int v = i >= d ? most[i - d] : 0;
-      __syncthreads();
-      most[i] = max(most[i], v);
-      __syncthreads();
+  int last = start0, count = 0;  // of the sequences so far: where they end, their items
+  for (int s0 = 0; s0 < seqs; s0 += 64) {
+    const int s = s0 + lane;
+    int end = s < seqs ? min(max(offsets[s + 1], last), tokens) : last;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int up = __shfl_up(end, d);
+      if (lane >= d) end = max(end, up);
     }
-    const int before = max(carry_most, start0);
-    const int begin = i ? max(most[i - 1], before) : before, end = max(most[i], before);
+    int begin = __shfl_up(end, 1);
+    if (lane == 0) begin = last;
     int mine = 0;
-    if (s < seqs) mine = keep_empty ? max(1, (end - begin + length - 1) / length) : (end - begin + length - 1) / length;
-    sum[i] = mine;
-    __syncthreads();
-    for (int d = 1; d < 256; d *= 2) {
-      const int v = i >= d ? sum[i - d] : 0;
-      __syncthreads();
-      sum[i] += v;
-      __syncthreads();
+    if (s < seqs) mine = max(keep_empty ? 1 : 0, (int)(((int64_t)end - begin + length - 1) / length));
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int up = __shfl_up(sum, d);
+      if (lane >= d) sum += up;
     }
-    const int at = carry_sum + sum[i] - mine;
     if (s < seqs) {
-      first[s] = at;
+      first[s] = count + sum - mine;
       for (int k = 0; k < mine; ++k)
-        table[at + k] = {s, begin + k * length, min(length, end - begin - k * length), 1};
+        table[count + sum - mine + k] = {s, begin + k * length, min(length, end - begin - k * length), 1};
     }
-    __syncthreads();
-    if (i == 255) {
-      carry_most = end;
-      carry_sum += sum[255];
-    }
-    __syncthreads();
+    last = __shfl(end, 63);
+    count += __shfl(sum, 63);
   }
-  const int last = carry_most, count = carry_sum;
-  if (i == 0) first[seqs] = count;
+  if (lane == 0) first[seqs] = count;
   // outside of the sequences
-  const int head = (start0 + length - 1) / length, tail = (tokens - last + length - 1) / length;
-  for (int k = i; k < items - count; k += 256) {
+  const int head = (int)(((int64_t)start0 + length - 1) / length);
+  const int tail = (int)(((int64_t)tokens - last + length - 1) / length);
+  for (int k = lane; k < items - count; k += 64) {
     Item it = {-1, 0, 0, 0};
     if (k < head) it = {-1, k * length, min(length, start0 - k * length), 0};
     else if (k < head + tail)
@@ -345,7 +329,7 @@ struct Sweep {
 
   void make_items(hipStream_t stream) const {
     if (!s.offsets) return;
-    k_items<<<1, 256, 0, stream>>>(s.offsets, s.seqs, (int)s.tokens, p.length, !p.by_item, p.items,
+    k_items<<<1, 64, 0, stream>>>(s.offsets, s.seqs, (int)s.tokens, p.length, !p.by_item, p.items,
                                    at<Item>(p.table), at<int>(p.first));
     hip_check(hipGetLastError(), "scan segments");
   }
