@@ -31,7 +31,7 @@ CFLAGS = [
 ]
 SOURCES = ["moddown.hip", "ntt.hip", "convert.hip", "rescale.hip", "small_ring.hip",
            "poly_ops.hip", "keyswitch.hip", "encode.hip", "keygen.hip", "clear_scan.hip",
-           "clear_scan_value.hip", "clear_scan_query.hip", "clear_step.hip", "clear_conv.hip",
+           "clear_scan_forward.hip", "clear_scan_backward.hip", "clear_step.hip", "clear_conv.hip",
            "clear_logprob.hip", "context.cpp", "capi.cpp", "clear_capi.cpp"]
 
 

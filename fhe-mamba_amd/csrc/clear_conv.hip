@@ -125,7 +125,7 @@ __device__ __forceinline__ void read_weights(const float* weight, const float* b
 // v += the taps of a window.
 template <class T, int VEC, int KT>
 __device__ __forceinline__ void add_taps(float (&v)[VEC], const float (&w)[KT][VEC],
-                                         const Piece<T, VEC> (&window)[KT], int taps) {
+                                         const Piece<T, VEC>* window, int taps) {
 #pragma unroll
   for (int k = 0; k < KT; ++k) {
     if (k < KT - taps) continue;
@@ -193,8 +193,7 @@ __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
   const T* x = (const T*)c.x.p + (c.offsets ? 0 : seq * c.x.seq);
   T* y = (T*)a.y + (c.offsets ? 0 : (int64_t)seq * c.tokens * c.channels) + c0;
 
-  Piece<T, VEC> window[KT];
-  Raw<T, VEC> next[AHEAD];
+  Piece<T, VEC> window[KT - 1 + AHEAD];  // the inputs from KT - 1 before token t
   int t = t0;
   while (t < t1) {
     const Span s = c.offsets ? find_span(c, t) : Span{seq, 0, (int)c.tokens};
@@ -205,28 +204,29 @@ __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < KT - 1; ++k) window[k] = input_at<T, VEC>(c, x, s, t - (KT - 1) + k, c0, count);
-    for (int ahead = 0; t < end; ++t, --ahead) {
-      if (ahead == 0) {
-        ahead = AHEAD;
+    for (; t < end; t += AHEAD) {
+      Raw<T, VEC> in[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-          if (t + u < end) next[u] = read<T, VEC>(x + (t + u) * c.x.tok + c0, count);
+      for (int u = 0; u < AHEAD; ++u)
+        in[u] = read<T, VEC>(x + min(t + u, end - 1) * c.x.tok + c0, count);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) window[KT - 1 + u] = in[u];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        Piece<T, VEC> out;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out.v[i] = b[i];
+        add_taps<T, VEC, KT>(out.v, w, window + u, c.taps);
+        if (c.silu) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) out.v[i] *= sigmoid(out.v[i]);
+        }
+        if (t + u < end) write<T, VEC>(y + (int64_t)(t + u) * c.channels, out, count);
       }
-      window[KT - 1] = next[0];
 #pragma unroll
-      for (int u = 0; u + 1 < AHEAD; ++u) next[u] = next[u + 1];
-      Piece<T, VEC> out;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) out.v[i] = b[i];
-      add_taps<T, VEC, KT>(out.v, w, window, c.taps);
-      if (c.silu) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) out.v[i] *= sigmoid(out.v[i]);
-      }
-      write<T, VEC>(y + (int64_t)t * c.channels, out, count);
-#pragma unroll
-      for (int k = 0; k < KT - 1; ++k) window[k] = window[k + 1];
+      for (int k = 0; k < KT - 1; ++k) window[k] = window[k + AHEAD];
     }
+    t = end;
   }
 }
 

@@ -71,13 +71,17 @@ struct RowArgs {
   uint64_t* best;     // [rows][splits][top]
 };
 
-// Sixteen logits of a thread: columns first + 16-byte piece p of the thread,
-// with the row's misaligned start before them.  -inf outside of [0, vocab).
+// Sixteen logits of a thread in a tile that begins at column `base` (a multiple
+// of 16 bytes; it may be negative), as they lie in memory.  -inf outside of the
+// row.
 template <class T>
 struct Sixteen {
   static constexpr int VEC = Num<T>::VEC, PIECES = 16 / VEC;
-  float v[16];
-  // column of element j of a tile at column `base` (may be negative)
+  union {
+    u32x4 w[PIECES];
+    T e[16];
+  };
+  // column of element j
   static __device__ __forceinline__ int64_t column(int64_t base, int j) {
     return base + (int64_t)(j / VEC) * THREADS * VEC + threadIdx.x * VEC + j % VEC;
   }
@@ -86,18 +90,16 @@ struct Sixteen {
     for (int p = 0; p < PIECES; ++p) {
       const int64_t c = column(base, p * VEC);
       if (c >= 0 && c + VEC <= vocab) {
-        union {
-          u32x4 w;
-          T e[VEC];
-        } u;
-        u.w = *reinterpret_cast<const u32x4*>(row + c);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[p * VEC + i] = (float)u.e[i];
+        w[p] = *reinterpret_cast<const u32x4*>(row + c);
       } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[p * VEC + i] = c + i >= 0 && c + i < vocab ? (float)row[c + i] : -INFINITY;
+        for (int i = 0; i < VEC; ++i) e[p * VEC + i] = c + i >= 0 && c + i < vocab ? row[c + i] : (T)-INFINITY;
       }
     }
+  }
+  __device__ __forceinline__ void widen(float* v) const {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = (float)e[j];
   }
 };
 
@@ -206,13 +208,17 @@ __global__ __launch_bounds__(THREADS) void k_row_parts(RowArgs a) {
     __syncthreads();
   }
   Stats st{-INFINITY, 0.0f, 0.0f};
+  const int64_t start = (int64_t)split * a.tiles * TILE - lead;
+  Sixteen<T> x;
+  x.read(row, start, a.l.vocab);
   for (int t = 0; t < a.tiles; ++t) {
-    const int64_t base = ((int64_t)split * a.tiles + t) * TILE - lead;
+    const int64_t base = start + (int64_t)t * TILE;
     if (base >= a.l.vocab) break;
-    Sixteen<T> x;
-    x.read(row, base, a.l.vocab);
-    st = add16(st, x.v);
-    if constexpr (TOP) keep_best<T>(lds, x.v, base, a.l.vocab, a.l.top);
+    float v[16];
+    x.widen(v);
+    if (t + 1 < a.tiles) x.read(row, base + TILE, a.l.vocab);  // in flight meanwhile
+    st = add16(st, v);
+    if constexpr (TOP) keep_best<T>(lds, v, base, a.l.vocab, a.l.top);
   }
   st = wave_join(st);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = st;
@@ -304,6 +310,8 @@ __global__ __launch_bounds__(THREADS) void k_row_back(BackArgs a) {
   const bool none = peak == -INFINITY;
   Sixteen<T> x;
   x.read(row, base, a.l.vocab);
+  float v[16];
+  x.widen(v);
 #pragma unroll
   for (int p = 0; p < Sixteen<T>::PIECES; ++p) {
     const int64_t c = Sixteen<T>::column(base, p * VEC);
@@ -313,7 +321,7 @@ __global__ __launch_bounds__(THREADS) void k_row_back(BackArgs a) {
     } u;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const float lp = (x.v[p * VEC + i] - peak) - log_sum, e = none ? 0.0f : __builtin_amdgcn_exp2f(lp * LOG2E);
+      const float lp = (v[p * VEC + i] - peak) - log_sum, e = none ? 0.0f : __builtin_amdgcn_exp2f(lp * LOG2E);
       float d = c + i == t ? ga : 0.0f;
       d -= ga * e;
       if (e != 0.0f) d -= gb * e * (lp + entropy);

@@ -80,40 +80,47 @@ __global__ __launch_bounds__(64) void k_items(const int* offsets, int seqs, int 
 // In: the state that each item adds.  Out: the state before it (behind it in
 // reverse), and the sequence's last.  A thread an element; eight items are read
 // at a time, since only the sums depend on each other.
-__global__ __launch_bounds__(256) void k_join(float* states, const float* decay, const int* first,
-                                              int segments, int size, int per_head, int heads, bool rev,
-                                              const float* initial, float* last) {
+struct Join {
+  float* states;
+  const float* initial;
+  float* last;
+};
+
+__global__ __launch_bounds__(256) void k_join(Join forward, Join reverse, const float* decay, const int* first,
+                                              int segments, int size, int per_head, int heads) {
   const int e = blockIdx.x * 256 + threadIdx.x, seq = blockIdx.y;
   if (e >= size) return;
+  const bool rev = blockIdx.z;
+  const Join j = rev ? reverse : forward;
   const int head = e / per_head;
   const int from = first ? first[seq] : seq * segments;
   const int count = first ? first[seq + 1] - from : segments;
-  float run = initial ? initial[(int64_t)seq * size + e] : 0.0f;
+  float run = j.initial ? j.initial[(int64_t)seq * size + e] : 0.0f;
   for (int i0 = 0; i0 < count; i0 += 8) {
     float add[8], keep[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int i = min(i0 + u, count - 1), item = from + (rev ? count - 1 - i : i);
-      add[u] = states[(int64_t)item * size + e];
+      add[u] = j.states[(int64_t)item * size + e];
       keep[u] = decay[(int64_t)item * heads + head];
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u)
       if (i0 + u < count) {
         const int item = from + (rev ? count - 1 - i0 - u : i0 + u);
-        states[(int64_t)item * size + e] = run;
+        j.states[(int64_t)item * size + e] = run;
         run = run * keep[u] + add[u];
       }
   }
-  if (last) last[(int64_t)seq * size + e] = run;
+  if (j.last) j.last[(int64_t)seq * size + e] = run;
 }
 
 // ---- the ends of the gradients ----
+// Four elements of a query gradient from its workgroups' parts.
 template <class T>
-__global__ __launch_bounds__(256) void k_sum_parts(const float* parts, int count, int64_t size, T* out) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+__device__ __forceinline__ void sum_parts(const float* parts, int count, int64_t size, T* out, int64_t i) {
   if (i >= size) return;
-  if (i + 4 <= size && size % 4 == 0) {
+  if (size % 4 == 0) {
     f32x4 sum = *reinterpret_cast<const f32x4*>(parts + i);
     for (int p = 1; p < count; ++p) sum += *reinterpret_cast<const f32x4*>(parts + p * size + i);
 #pragma unroll
@@ -136,23 +143,33 @@ __device__ __forceinline__ double block_sum(double v, double* scratch) {
   return scratch[0] + scratch[1] + scratch[2] + scratch[3];
 }
 
+// What is left when the sweeps are done: workgroups [0, 2 sums) sum the parts of
+// dC and then of dB, the next the gates' gradients of an item and head each, the
+// last the gradient of D a head each.
+struct Finish {
+  int64_t size;  // of dB and dC
+  int parts, items, entering_tiles;
+  uint32_t sums;  // workgroups of one of the two
+  const float *parts_c, *parts_b;
+  void *dc, *db;
+  const int* first;
+  const float *entering, *leaving, *adjoint, *states, *last;
+  float *dwrite, *ddecay, *dd;
+};
+
 // Gradients of write and log_decay of one item and head: the first summed over
 // the head's channels, the second from the segment's end backwards.
-__global__ __launch_bounds__(256) void k_gate_grads(SweepArgs a, const int* first, const float* entering,
-                                                    int entering_tiles, const float* leaving, const float* adjoint,
-                                                    const float* states, const float* last, float* dwrite,
-                                                    float* ddecay) {
-  __shared__ double scratch[4];
-  const int item_i = blockIdx.x, head = blockIdx.y;
+__device__ __forceinline__ void gate_grads(const SweepArgs& a, const Finish& f, int item_i, int head,
+                                           double* scratch) {
   const Item it = find_item(a, item_i);
   if (it.count <= 0) return;
   const int64_t token0 = item_token(a, it);
   const int64_t size = (int64_t)a.head_dim * a.states, all = size * a.heads;
   double carry = 0.0;
-  if (adjoint && it.live) {
-    const float* A = adjoint + (a.by_item ? item_i : it.seq) * all + head * size;
-    const bool more = a.by_item && (a.table ? item_i + 1 < first[it.seq + 1] : (item_i + 1) % a.segments != 0);
-    const float* h = (more ? states + (item_i + 1) * all : last + it.seq * all) + head * size;
+  if (f.adjoint && it.live) {
+    const float* A = f.adjoint + (a.by_item ? item_i : it.seq) * all + head * size;
+    const bool more = a.by_item && (a.table ? item_i + 1 < f.first[it.seq + 1] : (item_i + 1) % a.segments != 0);
+    const float* h = (more ? f.states + (item_i + 1) * all : f.last + it.seq * all) + head * size;
     for (int64_t e = threadIdx.x; e < size; e += 256) carry += (double)A[e] * h[e];
     carry = block_sum(carry, scratch);
   }
@@ -164,12 +181,12 @@ __global__ __launch_bounds__(256) void k_gate_grads(SweepArgs a, const int* firs
       float dw = 0.0f;
       for (int p = 0; p < a.col_tiles; ++p) {
         const int64_t at = ((int64_t)head * a.col_tiles + p) * a.all_tokens + token0 + t;
-        v += (double)leaving[at];
+        v += (double)f.leaving[at];
         dw += a.dwrite_part[at];
       }
-      for (int p = 0; p < entering_tiles; ++p)
-        v += (double)entering[((int64_t)head * entering_tiles + p) * a.all_tokens + token0 + t];
-      dwrite[(token0 + t) * a.heads + head] = dw;
+      for (int p = 0; p < f.entering_tiles; ++p)
+        v += (double)f.entering[((int64_t)head * f.entering_tiles + p) * a.all_tokens + token0 + t];
+      f.dwrite[(token0 + t) * a.heads + head] = dw;
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -184,22 +201,35 @@ __global__ __launch_bounds__(256) void k_gate_grads(SweepArgs a, const int* firs
       if (w < wave) before += scratch[w];
       carry += scratch[w];
     }
-    if (t >= 0) ddecay[(token0 + t) * a.heads + head] = (float)(before + v);
+    if (t >= 0) f.ddecay[(token0 + t) * a.heads + head] = (float)(before + v);
   }
 }
 
-__global__ __launch_bounds__(256) void k_skip_grad(SweepArgs a, int items, float* dd) {
-  __shared__ double scratch[4];
-  const int head = blockIdx.x;
+__device__ __forceinline__ void skip_grad(const SweepArgs& a, const Finish& f, int head, double* scratch) {
   double v = 0.0;
-  for (int i = threadIdx.x; i < items; i += 256) {
+  for (int i = threadIdx.x; i < f.items; i += 256) {
     const Item it = find_item(a, i);
     if (!it.live) continue;
-    for (int p = 0; p < a.col_tiles; ++p)
-      v += a.dd_part[((int64_t)i * a.heads + head) * a.col_tiles + p];
+    for (int p = 0; p < a.col_tiles; ++p) v += a.dd_part[((int64_t)i * a.heads + head) * a.col_tiles + p];
   }
   v = block_sum(v, scratch);
-  if (threadIdx.x == 0) dd[head] = (float)v;
+  if (threadIdx.x == 0) f.dd[head] = (float)v;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void k_finish(SweepArgs a, Finish f) {
+  __shared__ double scratch[4];
+  uint32_t block = blockIdx.x;
+  if (block < 2 * f.sums) {
+    const bool is_b = block >= f.sums;
+    const int64_t i = ((int64_t)(is_b ? block - f.sums : block) * 256 + threadIdx.x) * 4;
+    sum_parts<T>(is_b ? f.parts_b : f.parts_c, f.parts, f.size, (T*)(is_b ? f.db : f.dc), i);
+    return;
+  }
+  block -= 2 * f.sums;
+  const uint32_t gates = (uint32_t)f.items * a.heads;
+  if (block < gates) gate_grads(a, f, (int)(block / a.heads), (int)(block % a.heads), scratch);
+  else skip_grad(a, f, (int)(block - gates), scratch);
 }
 
 // ---- plan ----
@@ -218,7 +248,7 @@ struct Plan {
   int length, segments, items;
   bool by_item;
   // workspace, in bytes
-  size_t table, first, decays, states, adjoints, last, dwrite, gate_out, gate_in, dd, parts, total;
+  size_t table, first, decays, states, adjoints, last, dwrite, gate_out, gate_in, dd, parts_c, parts_b, total;
 };
 
 // Tokens of a segment: a whole sequence where the sequences alone fill half of
@@ -272,7 +302,8 @@ Plan make_plan(const Scan& s, bool backward) {
     p.gate_out = take(rows * all * 4);
     p.gate_in = take((size_t)s.heads * p.query.col_tiles * all * 4);
     p.dd = take(rows * p.items * 4);
-    p.parts = take((size_t)p.query.blocks * all * s.groups * s.states * 4);
+    p.parts_c = take((size_t)p.query.blocks * all * s.groups * s.states * 4);
+    p.parts_b = take((size_t)p.query.blocks * all * s.groups * s.states * 4);
   }
   return p;
 }
@@ -333,30 +364,26 @@ struct Sweep {
                                    at<Item>(p.table), at<int>(p.first));
     hip_check(hipGetLastError(), "scan segments");
   }
-  // The states before (in reverse, behind) each segment at `states`, and each
-  // sequence's last at `last`.
-  void carry(const Strided& key, const Strided& value, bool rev, size_t states, const float* initial,
-             float* last, hipStream_t stream) const {
+  // The states before each segment, and each sequence's last; with `reverse` also
+  // the adjoint's behind each.
+  SweepArgs state_args(const Strided& key, const Strided& value, size_t states) const {
     SweepArgs b = with(p.value, key, key, value, value);
     b.wide_out = true;
     b.state_out = at<float>(states);
     b.decay_out = at<float>(p.decays);
-    launch_state_sweep(s.dtype, b, p.items, rev, stream);
-    const int size = s.heads * s.head_dim * s.states;
-    k_join<<<dim3((size + 255) / 256, s.seqs), 256, 0, stream>>>(
-        at<float>(states), at<float>(p.decays), first(), p.segments, size, s.head_dim * s.states, s.heads,
-        rev, initial, last);
-    hip_check(hipGetLastError(), "scan state join");
+    return b;
   }
-  void sum_parts(void* out, hipStream_t stream) const {
-    const int64_t size = s.all_tokens() * s.groups * s.states;
-    if (!size) return;
-    const uint32_t grid = (uint32_t)((size + 1023) / 1024);
-    if (s.dtype == BF16)
-      k_sum_parts<<<grid, 256, 0, stream>>>(at<float>(p.parts), p.query.blocks, size, (bf16*)out);
-    else
-      k_sum_parts<<<grid, 256, 0, stream>>>(at<float>(p.parts), p.query.blocks, size, (float*)out);
-    hip_check(hipGetLastError(), "scan gradient sums");
+  void carry(float* last, const ScanGrads* g, hipStream_t stream) const {
+    const SweepArgs f = state_args(s.b, s.x, p.states);
+    SweepArgs r{};
+    if (g) r = state_args(s.c, g->dy, p.adjoints);
+    launch_states(s.dtype, f, g ? &r : nullptr, p.items, stream);
+    const int size = s.heads * s.head_dim * s.states;
+    const Join forward{at<float>(p.states), s.initial, last};
+    const Join reverse = g ? Join{at<float>(p.adjoints), g->dfinal, g->dinitial} : Join{};
+    k_join<<<dim3((size + 255) / 256, s.seqs, g ? 2 : 1), 256, 0, stream>>>(
+        forward, reverse, at<float>(p.decays), first(), p.segments, size, s.head_dim * s.states, s.heads);
+    hip_check(hipGetLastError(), "scan state join");
   }
 };
 
@@ -368,63 +395,71 @@ void scan(const Scan& s, void* y, float* final_state, void* workspace, hipStream
   const Plan p = make_plan(s, false);
   const Sweep sweep(s, p, (char*)workspace);
   sweep.make_items(stream);
-  if (p.by_item) sweep.carry(s.b, s.x, false, p.states, s.initial, final_state, stream);
+  if (p.by_item) sweep.carry(final_state, nullptr, stream);
   SweepArgs a = sweep.with(p.value, s.b, s.c, s.x, s.x);
   a.wide_out = s.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
   a.d = s.d;
   a.state_in = p.by_item ? sweep.at<float>(p.states) : s.initial;
   a.state_out = p.by_item ? nullptr : final_state;
   a.out = y;
-  launch_value_sweep(s.dtype, a, p.items, false, stream);
+  launch_forward(s.dtype, a, p.items, stream);
 }
 
 void scan_backward(const Scan& s, const ScanGrads& g, void* workspace, hipStream_t stream) {
   const Plan p = make_plan(s, true);
   const Sweep sweep(s, p, (char*)workspace);
-  float* last = g.dfinal ? sweep.at<float>(p.last) : nullptr;
   sweep.make_items(stream);
-  if (p.by_item) {
-    sweep.carry(s.b, s.x, false, p.states, s.initial, sweep.at<float>(p.last), stream);
-    sweep.carry(s.c, g.dy, true, p.adjoints, g.dfinal, g.dinitial, stream);
-  }
+  if (p.by_item) sweep.carry(sweep.at<float>(p.last), &g, stream);
   const float* states = p.by_item ? sweep.at<float>(p.states) : s.initial;
   const float* adjoints = p.by_item ? sweep.at<float>(p.adjoints) : g.dfinal;
 
-  SweepArgs a = sweep.with(p.value, s.c, s.b, g.dy, s.x);
-  a.wide_out = s.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(g.dx) % 16 == 0;
-  a.d = s.d;
-  a.state_in = adjoints;
-  a.state_out = p.by_item ? nullptr : g.dinitial;
-  a.out = g.dx;
-  a.dwrite_part = sweep.at<float>(p.dwrite);
-  a.gate_part = sweep.at<float>(p.gate_out);
-  a.dd_part = sweep.at<float>(p.dd);
-  launch_value_sweep(s.dtype, a, p.items, true, stream);
+  SweepArgs x = sweep.with(p.value, s.c, s.b, g.dy, s.x);
+  x.wide_out = s.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(g.dx) % 16 == 0;
+  x.d = s.d;
+  x.state_in = adjoints;
+  x.state_out = p.by_item ? nullptr : g.dinitial;
+  x.out = g.dx;
+  x.dwrite_part = sweep.at<float>(p.dwrite);
+  x.gate_part = sweep.at<float>(p.gate_out);
+  x.dd_part = sweep.at<float>(p.dd);
 
   SweepArgs c = sweep.with(p.query, s.b, s.c, s.x, g.dy);
   c.state_in = states;
-  c.state_out = p.by_item ? nullptr : last;
-  c.out = sweep.at<float>(p.parts);
+  c.state_out = p.by_item || !g.dfinal ? nullptr : sweep.at<float>(p.last);
+  c.out = sweep.at<float>(p.parts_c);
   c.wide_out = s.states % 4 == 0;
   c.gate_part = sweep.at<float>(p.gate_in);
-  launch_query_sweep(s.dtype, c, p.items, false, stream);
-  sweep.sum_parts(g.dc, stream);
 
   SweepArgs b = sweep.with(p.query, s.c, s.b, g.dy, s.x);
   b.state_in = adjoints;
-  b.out = sweep.at<float>(p.parts);
+  b.out = sweep.at<float>(p.parts_b);
   b.wide_out = s.states % 4 == 0;
-  launch_query_sweep(s.dtype, b, p.items, true, stream);
-  sweep.sum_parts(g.db, stream);
+  launch_backward(s.dtype, c, b, x, p.items, stream);
 
-  k_gate_grads<<<dim3(p.items, s.heads), 256, 0, stream>>>(
-      a, sweep.first(), sweep.at<float>(p.gate_in), p.query.col_tiles, sweep.at<float>(p.gate_out), adjoints, states,
-      sweep.at<float>(p.last), g.dwrite, g.ddecay);
-  hip_check(hipGetLastError(), "scan gate gradients");
-  if (g.dd) {
-    k_skip_grad<<<s.heads, 256, 0, stream>>>(a, p.items, g.dd);
-    hip_check(hipGetLastError(), "scan skip gradient");
-  }
+  Finish f{};
+  f.size = s.all_tokens() * s.groups * s.states;
+  f.parts = p.query.blocks;
+  f.items = p.items;
+  f.entering_tiles = p.query.col_tiles;
+  f.sums = (uint32_t)((f.size + 1023) / 1024);
+  f.parts_c = (const float*)c.out;
+  f.parts_b = (const float*)b.out;
+  f.dc = g.dc;
+  f.db = g.db;
+  f.first = sweep.first();
+  f.entering = c.gate_part;
+  f.leaving = x.gate_part;
+  f.adjoint = adjoints;
+  f.states = states;
+  f.last = sweep.at<float>(p.last);
+  f.dwrite = g.dwrite;
+  f.ddecay = g.ddecay;
+  f.dd = g.dd;
+  const int64_t grid = 2 * (int64_t)f.sums + (int64_t)p.items * s.heads + (g.dd ? s.heads : 0);
+  if (grid > INT32_MAX) throw ArgError("too many tokens and heads for one call");
+  if (s.dtype == BF16) k_finish<bf16><<<(uint32_t)grid, 256, 0, stream>>>(x, f);
+  else k_finish<float><<<(uint32_t)grid, 256, 0, stream>>>(x, f);
+  hip_check(hipGetLastError(), "scan gradients");
 }
 
 }  // namespace fhe::clear

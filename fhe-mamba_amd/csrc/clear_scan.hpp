@@ -233,6 +233,12 @@ __device__ __forceinline__ float sum_groups(float v) {
   return v + __shfl_xor(v, 32);
 }
 
+// Workgroups are dealt to the eight dies in turn: each die takes a run of
+// consecutive numbers, so that those which share keys and queries share an L2.
+__device__ __forceinline__ uint32_t deal(uint32_t b, uint32_t n) {
+  return b < n / 8 * 8 ? b % 8 * (n / 8) + b / 8 : b;
+}
+
 // What every sweep derives from its workgroup and wavefront.
 struct Place {
   Item it;
@@ -242,11 +248,8 @@ struct Place {
   int64_t state_at;   // of its head in the states
   int64_t part;       // its row in per-wavefront results
 
-  // Workgroups are dealt to the eight dies in turn: each die takes a run of
-  // consecutive ones, so that those which share keys and queries share an L2.
-  __device__ __forceinline__ explicit Place(const SweepArgs& a) {
-    const uint32_t n = gridDim.x, b = blockIdx.x;
-    const uint32_t id = b < n / 8 * 8 ? b % 8 * (n / 8) + b / 8 : b;
+  // `id`: the workgroup's number among its sweep's
+  __device__ __forceinline__ Place(const SweepArgs& a, uint32_t id) {
     item = (int)(id / (uint32_t)(a.groups * a.blocks));
     block = (int)(id % (uint32_t)(a.groups * a.blocks));
     it = find_item(a, item);
@@ -280,10 +283,27 @@ inline uint32_t workgroups(const SweepArgs& a, int items) {
   return (uint32_t)n;
 }
 
-// Launches of the sweeps, by type and state size (clear_scan_value.hip,
-// clear_scan_query.hip).
-void launch_value_sweep(uint32_t dtype, const SweepArgs& a, int items, bool rev, hipStream_t s);
-void launch_state_sweep(uint32_t dtype, const SweepArgs& a, int items, bool rev, hipStream_t s);
-void launch_query_sweep(uint32_t dtype, const SweepArgs& a, int items, bool rev, hipStream_t s);
+constexpr size_t LDS_BYTES = 160 * 1024;
+inline void allow_lds(const void* kernel, size_t bytes) {
+  hip_check(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "LDS of a sweep");
+}
+
+// f(an element, the 32-state blocks that hold the states)
+template <class F>
+void by_shape(uint32_t dtype, int states, F&& f) {
+  auto by_size = [&](auto zero) {
+    if (states <= 32) f(zero, std::integral_constant<int, 1>{});
+    else if (states <= 64) f(zero, std::integral_constant<int, 2>{});
+    else f(zero, std::integral_constant<int, 4>{});
+  };
+  if (dtype == BF16) by_size(bf16{});
+  else by_size(float{});
+}
+
+// clear_scan_forward.hip and clear_scan_backward.hip
+void launch_forward(uint32_t dtype, const SweepArgs& a, int items, hipStream_t s);
+void launch_states(uint32_t dtype, const SweepArgs& a, const SweepArgs* reverse, int items, hipStream_t s);
+void launch_backward(uint32_t dtype, const SweepArgs& c, const SweepArgs& b, const SweepArgs& x, int items,
+                     hipStream_t s);
 
 }  // namespace fhe::clear

@@ -1,8 +1,10 @@
 // Sweeps that give the gradients of the scan's queries: forward those of C, and
 // in reverse, where keys and queries change places, those of B.
-#pragma clang fp contract(fast)
+#pragma once
+
 #include "clear_scan.hpp"
 
+#pragma clang fp contract(fast)
 namespace fhe::clear {
 namespace {
 
@@ -21,7 +23,7 @@ struct QueryLds {
 // State tiles (rows 4 q + r the channel, column l the state) from and to
 // [head_dim][states].
 template <int NB, int PT>
-__device__ __forceinline__ void state_io(f32x4 (&h)[PT][2 * NB], const float* from, float* to, int p0,
+__device__ __forceinline__ void channel_state_io(f32x4 (&h)[PT][2 * NB], const float* from, float* to, int p0,
                                          int head_dim, int states) {
   const int q = lane_id() >> 4, l = lane_id() & 15;
 #pragma unroll
@@ -46,16 +48,15 @@ __device__ __forceinline__ void state_io(f32x4 (&h)[PT][2 * NB], const float* fr
 // group; forward also the part of the gates' gradient that the state before the
 // chunk has in it.
 template <class T, int NB, int PT, bool REV, bool FULL>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_query_sweep(SweepArgs a) {
+__device__ __forceinline__ void query_sweep(const SweepArgs& a, char* lds_raw, uint32_t id) {
   using N = Num<T>;
   using Frag = typename N::Frag;
   using Lds = QueryLds<T, NB, PT>;
   using Key = typename Lds::Key;
   using Value = typename Lds::Value;
-  extern __shared__ __align__(16) char lds_raw[];
   Lds& lds = *reinterpret_cast<Lds*>(lds_raw);
 
-  const Place at(a);
+  const Place at(a, id);
   const Item it = at.it;
   if (it.count <= 0 && it.seq < 0) return;
   const int lane = lane_id(), q = lane >> 4, l = lane & 15;
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_query_sweep(SweepArgs a) {
 
   f32x4 h[PT][2 * NB] = {};
   if (a.state_in && at.active && it.live)
-    state_io<NB, PT>(h, a.state_in + at.state_at, nullptr, at.p0, a.head_dim, a.states);
+    channel_state_io<NB, PT>(h, a.state_in + at.state_at, nullptr, at.p0, a.head_dim, a.states);
 
   T* vt = lds.value[at.wave];
   Gates& t = lds.gates[at.wave];
@@ -203,42 +204,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_query_sweep(SweepArgs a) {
     }
   }
   if (a.state_out && at.active && it.live)
-    state_io<NB, PT>(h, nullptr, a.state_out + at.state_at, at.p0, a.head_dim, a.states);
-}
-
-template <class T, int NB, int PT, bool REV>
-void launch(const SweepArgs& a, int items, hipStream_t s) {
-  constexpr size_t bytes = sizeof(QueryLds<T, NB, PT>);
-  static_assert(bytes <= 160 * 1024);
-  auto* kernel = is_full(a, NB) ? &k_query_sweep<T, NB, PT, REV, true> : &k_query_sweep<T, NB, PT, REV, false>;
-  hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
-            "scan gradient sweep");
-  kernel<<<workgroups(a, items), 64 * WAVES, bytes, s>>>(a);
-  hip_check(hipGetLastError(), "scan gradient sweep");
-}
-
-template <bool REV>
-void dispatch(uint32_t dtype, const SweepArgs& a, int items, hipStream_t s) {
-  auto by_size = [&](auto zero, auto cols) {
-    using T = decltype(zero);
-    constexpr int PT = decltype(cols)::value / 16;
-    if (a.states <= 32) launch<T, 1, PT, REV>(a, items, s);
-    else if (a.states <= 64) launch<T, 2, PT, REV>(a, items, s);
-    else launch<T, 4, PT, REV>(a, items, s);
-  };
-  auto by_cols = [&](auto zero) {
-    if (a.cols == 32) by_size(zero, std::integral_constant<int, 32>{});
-    else by_size(zero, std::integral_constant<int, 64>{});
-  };
-  if (dtype == BF16) by_cols(bf16{});
-  else by_cols(float{});
+    channel_state_io<NB, PT>(h, nullptr, a.state_out + at.state_at, at.p0, a.head_dim, a.states);
 }
 
 }  // namespace
-
-void launch_query_sweep(uint32_t dtype, const SweepArgs& a, int items, bool rev, hipStream_t s) {
-  if (rev) dispatch<true>(dtype, a, items, s);
-  else dispatch<false>(dtype, a, items, s);
-}
-
 }  // namespace fhe::clear

@@ -1,8 +1,10 @@
 // Sweeps over the chunks of a segment with the state in registers: the scan's
 // results, and the state that a segment leaves.
-#pragma clang fp contract(fast)
+#pragma once
+
 #include "clear_scan.hpp"
 
+#pragma clang fp contract(fast)
 namespace fhe::clear {
 namespace {
 
@@ -70,16 +72,15 @@ __device__ __forceinline__ void state_io(f32x4 (&h)[2 * NB][PT], const float* fr
 // y (or, in reverse, the gradient of x) of a segment, 16 PT channels of one head
 // a wavefront, four wavefronts of one group on shared keys and queries.
 template <class T, int NB, int PT, bool REV, bool VALUES, bool FULL>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_value_sweep(SweepArgs a) {
+__device__ __forceinline__ void value_sweep(const SweepArgs& a, char* lds_raw, uint32_t id) {
   using N = Num<T>;
   using Frag = typename N::Frag;
   using Lds = ValueLds<T, NB, PT, VALUES>;
   using Key = typename Lds::Key;
   using Value = typename Lds::Value;
-  extern __shared__ __align__(16) char lds_raw[];
   Lds& lds = *reinterpret_cast<Lds*>(lds_raw);
 
-  const Place at(a);
+  const Place at(a, id);
   const Item it = at.it;
   if (it.count <= 0 && it.seq < 0) return;
   const int lane = lane_id(), q = lane >> 4, l = lane & 15;
@@ -267,43 +268,5 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_value_sweep(SweepArgs a) {
   }
 }
 
-template <class T, int NB, int PT, bool REV, bool VALUES>
-void launch(const SweepArgs& a, int items, hipStream_t s) {
-  constexpr size_t bytes = sizeof(ValueLds<T, NB, PT, VALUES>);
-  static_assert(bytes <= 160 * 1024);
-  auto* kernel = is_full(a, NB) ? &k_value_sweep<T, NB, PT, REV, VALUES, true>
-                                : &k_value_sweep<T, NB, PT, REV, VALUES, false>;
-  hip_check(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
-            "scan sweep");
-  kernel<<<workgroups(a, items), 64 * WAVES, bytes, s>>>(a);
-  hip_check(hipGetLastError(), "scan sweep");
-}
-
-template <bool VALUES>
-void dispatch(uint32_t dtype, const SweepArgs& a, int items, bool rev, hipStream_t s) {
-  auto by_size = [&](auto zero, auto reverse) {
-    using T = decltype(zero);
-    constexpr bool R = decltype(reverse)::value;
-    constexpr int PT = VALUE_COLS / 16;
-    if (a.states <= 32) launch<T, 1, PT, R, VALUES>(a, items, s);
-    else if (a.states <= 64) launch<T, 2, PT, R, VALUES>(a, items, s);
-    else launch<T, 4, PT, R, VALUES>(a, items, s);
-  };
-  auto by_type = [&](auto reverse) {
-    if (dtype == BF16) by_size(bf16{}, reverse);
-    else by_size(float{}, reverse);
-  };
-  if (rev) by_type(std::true_type{});
-  else by_type(std::false_type{});
-}
-
 }  // namespace
-
-void launch_value_sweep(uint32_t dtype, const SweepArgs& a, int items, bool rev, hipStream_t s) {
-  dispatch<true>(dtype, a, items, rev, s);
-}
-void launch_state_sweep(uint32_t dtype, const SweepArgs& a, int items, bool rev, hipStream_t s) {
-  dispatch<false>(dtype, a, items, rev, s);
-}
-
 }  // namespace fhe::clear
