@@ -16,7 +16,7 @@
 // dB and dC.  With M_ts the part of the loss in source s and target t,
 // dg_r is the sum of M over t >= r > s: what crosses the segment's end,
 // <A, h> there, plus the sums over t >= r of what enters at t less what leaves.
-// Terms with s = t are in neither, and the sums restart in every segment.
+// Terms with s = t are in neither, and the sums restart every few hundred tokens.
 #pragma clang fp contract(fast)
 #include "clear_scan.hpp"
 
@@ -86,33 +86,36 @@ struct Join {
   float* last;
 };
 
+template <int VEC>
 __global__ __launch_bounds__(256) void k_join(Join forward, Join reverse, const float* decay, const int* first,
                                               int segments, int size, int per_head, int heads) {
-  const int e = blockIdx.x * 256 + threadIdx.x, seq = blockIdx.y;
+  typedef float Vec __attribute__((ext_vector_type(VEC)));
+  const int e = (blockIdx.x * 256 + threadIdx.x) * VEC, seq = blockIdx.y;
   if (e >= size) return;
   const bool rev = blockIdx.z;
   const Join j = rev ? reverse : forward;
   const int head = e / per_head;
   const int from = first ? first[seq] : seq * segments;
   const int count = first ? first[seq + 1] - from : segments;
-  float run = j.initial ? j.initial[(int64_t)seq * size + e] : 0.0f;
+  auto at = [&](float* p, int64_t row) { return reinterpret_cast<Vec*>(p + row * size + e); };
+  Vec run = j.initial ? *reinterpret_cast<const Vec*>(j.initial + (int64_t)seq * size + e) : Vec(0.0f);
   for (int i0 = 0; i0 < count; i0 += 8) {
-    float add[8], keep[8];
+    Vec add[8];
+    float keep[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int i = min(i0 + u, count - 1), item = from + (rev ? count - 1 - i : i);
-      add[u] = j.states[(int64_t)item * size + e];
+      add[u] = *at(j.states, item);
       keep[u] = decay[(int64_t)item * heads + head];
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u)
       if (i0 + u < count) {
-        const int item = from + (rev ? count - 1 - i0 - u : i0 + u);
-        j.states[(int64_t)item * size + e] = run;
+        *at(j.states, from + (rev ? count - 1 - i0 - u : i0 + u)) = run;
         run = run * keep[u] + add[u];
       }
   }
-  if (j.last) j.last[(int64_t)seq * size + e] = run;
+  if (j.last) *at(j.last, seq) = run;
 }
 
 // ---- the ends of the gradients ----
@@ -134,21 +137,20 @@ __device__ __forceinline__ void sum_parts(const float* parts, int count, int64_t
   }
 }
 
-__device__ __forceinline__ double block_sum(double v, double* scratch) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
+  return v;
 }
 
-// What is left when the sweeps are done: workgroups [0, 2 sums) sum the parts of
-// dC and then of dB, the next the gates' gradients of an item and head each, the
-// last the gradient of D a head each.
+constexpr int FINISH_THREADS = 256, FINISH_HEADS = FINISH_THREADS / 64, FINISH_STEPS = 4;
+
+// What is left when the sweeps are done: the first workgroups, which take longest,
+// make the gates' gradients of an item and four heads each, the next the gradient
+// of D of four heads each, then `sums` sum the parts of dC and as many those of dB.
 struct Finish {
   int64_t size;  // of dB and dC
-  int parts, items, entering_tiles;
+  int parts, items, entering_tiles, group;
   uint32_t sums;  // workgroups of one of the two
   const float *parts_c, *parts_b;
   void *dc, *db;
@@ -157,79 +159,119 @@ struct Finish {
   float *dwrite, *ddecay, *dd;
 };
 
-// Gradients of write and log_decay of one item and head: the first summed over
-// the head's channels, the second from the segment's end backwards.
-__device__ __forceinline__ void gate_grads(const SweepArgs& a, const Finish& f, int item_i, int head,
-                                           double* scratch) {
+// Gradients of write and log_decay of four heads, a wavefront each, and of up
+// to `group` items of one sequence, by the workgroup of the last of them: the first
+// summed over the head's channels, the second from the items' end backwards.  What
+// crosses that end takes both states' bandwidth, so short items share one end; the
+// sums of a few hundred tokens lose nothing against it.  The results of 64 tokens
+// go through LDS, so that a token's heads are written together.
+__device__ __forceinline__ void gate_grads(const SweepArgs& a, const Finish& f, int item_i, int head0,
+                                           float (&tile)[2][64 * FINISH_STEPS][FINISH_HEADS + 1]) {
   const Item it = find_item(a, item_i);
   if (it.count <= 0) return;
-  const int64_t token0 = item_token(a, it);
+  int count = it.count;  // tokens of the group
+  bool last_item = true;
+  if (a.by_item && it.live) {
+    const int at = a.table ? item_i - f.first[it.seq] : item_i % a.segments;
+    const int items = a.table ? f.first[it.seq + 1] - f.first[it.seq] : a.segments;
+    last_item = at == items - 1;
+    if (!last_item && at % f.group != f.group - 1) return;
+    count += at % f.group * a.length;
+  }
+  const int lane = lane_id(), wave = threadIdx.x >> 6, head = min(head0 + wave, a.heads - 1);
+  const int64_t token0 = item_token(a, it) + it.count - count;
   const int64_t size = (int64_t)a.head_dim * a.states, all = size * a.heads;
   double carry = 0.0;
   if (f.adjoint && it.live) {
     const float* A = f.adjoint + (a.by_item ? item_i : it.seq) * all + head * size;
-    const bool more = a.by_item && (a.table ? item_i + 1 < f.first[it.seq + 1] : (item_i + 1) % a.segments != 0);
-    const float* h = (more ? f.states + (item_i + 1) * all : f.last + it.seq * all) + head * size;
-    for (int64_t e = threadIdx.x; e < size; e += 256) carry += (double)A[e] * h[e];
-    carry = block_sum(carry, scratch);
-  }
-  const int lane = lane_id(), wave = threadIdx.x >> 6;
-  for (int end = it.count; end > 0; end -= 256) {
-    const int t = end - 1 - (int)threadIdx.x;  // the last token first
-    double v = 0.0;
-    if (t >= 0) {
-      float dw = 0.0f;
-      for (int p = 0; p < a.col_tiles; ++p) {
-        const int64_t at = ((int64_t)head * a.col_tiles + p) * a.all_tokens + token0 + t;
-        v += (double)f.leaving[at];
-        dw += a.dwrite_part[at];
+    const float* h = (last_item ? f.last + it.seq * all : f.states + (item_i + 1) * all) + head * size;
+    if (size % 4 == 0 && reinterpret_cast<uintptr_t>(f.adjoint) % 16 == 0) {
+#pragma unroll 8
+      for (int64_t e = 4 * lane; e < size; e += 256) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(A + e), y = *reinterpret_cast<const f32x4*>(h + e);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) carry += (double)x[r] * y[r];
       }
-      for (int p = 0; p < f.entering_tiles; ++p)
-        v += (double)f.entering[((int64_t)head * f.entering_tiles + p) * a.all_tokens + token0 + t];
-      f.dwrite[(token0 + t) * a.heads + head] = dw;
+    } else {
+      for (int64_t e = lane; e < size; e += 64) carry += (double)A[e] * h[e];
+    }
+    carry = wave_sum(carry);
+  }
+  for (int end = count; end > 0; end -= 64 * FINISH_STEPS) {
+    double v[FINISH_STEPS] = {};
+    float dw[FINISH_STEPS] = {};
+    const int t0 = end - 1 - lane;  // the last token first, then those 64 before it
+    for (int p = 0; p < a.col_tiles; ++p) {
+      const int64_t at = ((int64_t)head * a.col_tiles + p) * a.all_tokens + token0 + t0;
+#pragma unroll
+      for (int u = 0; u < FINISH_STEPS; ++u)
+        if (t0 >= 64 * u) {
+          v[u] += (double)f.leaving[at - 64 * u];
+          dw[u] += a.dwrite_part[at - 64 * u];
+        }
+    }
+    for (int p = 0; p < f.entering_tiles; ++p) {
+      const int64_t at = ((int64_t)head * f.entering_tiles + p) * a.all_tokens + token0 + t0;
+#pragma unroll
+      for (int u = 0; u < FINISH_STEPS; ++u)
+        if (t0 >= 64 * u) v[u] += (double)f.entering[at - 64 * u];
     }
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double up = __shfl_up(v, d);
-      if (lane >= d) v += up;
+    for (int u = 0; u < FINISH_STEPS; ++u) v[u] = wave_scan(v[u]);  // four at a time, then what is before each
+#pragma unroll
+    for (int u = 0; u < FINISH_STEPS; ++u) {
+      tile[0][64 * u + lane][wave] = dw[u];
+      tile[1][64 * u + lane][wave] = (float)(v[u] + carry);
+      carry += read_lane(v[u], 63);
     }
     __syncthreads();
-    if (lane == 63) scratch[wave] = v;
-    __syncthreads();
-    double before = carry;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += scratch[w];
-      carry += scratch[w];
+    const int col = threadIdx.x % FINISH_HEADS;
+#pragma unroll
+    for (int u = 0; u < FINISH_STEPS; ++u) {
+      const int row = 64 * u + threadIdx.x / FINISH_HEADS;
+      if (row < end && head0 + col < a.heads) {
+        const int64_t at = (token0 + end - 1 - row) * a.heads + head0 + col;
+        f.dwrite[at] = tile[0][row][col];
+        f.ddecay[at] = tile[1][row][col];
+      }
     }
-    if (t >= 0) f.ddecay[(token0 + t) * a.heads + head] = (float)(before + v);
+    __syncthreads();
   }
 }
 
-__device__ __forceinline__ void skip_grad(const SweepArgs& a, const Finish& f, int head, double* scratch) {
+__device__ __forceinline__ void skip_grad(const SweepArgs& a, const Finish& f, int head0) {
+  const int head = head0 + (threadIdx.x >> 6);
+  if (head >= a.heads) return;
   double v = 0.0;
-  for (int i = threadIdx.x; i < f.items; i += 256) {
+  for (int i = lane_id(); i < f.items; i += 64) {
     const Item it = find_item(a, i);
     if (!it.live) continue;
     for (int p = 0; p < a.col_tiles; ++p) v += a.dd_part[((int64_t)i * a.heads + head) * a.col_tiles + p];
   }
-  v = block_sum(v, scratch);
-  if (threadIdx.x == 0) f.dd[head] = (float)v;
+  v = wave_sum(v);
+  if (lane_id() == 0) f.dd[head] = (float)v;
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void k_finish(SweepArgs a, Finish f) {
-  __shared__ double scratch[4];
+__global__ __launch_bounds__(FINISH_THREADS) void k_finish(SweepArgs a, Finish f) {
+  __shared__ float tile[2][64 * FINISH_STEPS][FINISH_HEADS + 1];
   uint32_t block = blockIdx.x;
-  if (block < 2 * f.sums) {
-    const bool is_b = block >= f.sums;
-    const int64_t i = ((int64_t)(is_b ? block - f.sums : block) * 256 + threadIdx.x) * 4;
-    sum_parts<T>(is_b ? f.parts_b : f.parts_c, f.parts, f.size, (T*)(is_b ? f.db : f.dc), i);
+  const uint32_t across = (a.heads + FINISH_HEADS - 1) / FINISH_HEADS, gates = (uint32_t)f.items * across;
+  if (block < gates) {
+    gate_grads(a, f, (int)(block / across), (int)(block % across) * FINISH_HEADS, tile);
     return;
   }
-  block -= 2 * f.sums;
-  const uint32_t gates = (uint32_t)f.items * a.heads;
-  if (block < gates) gate_grads(a, f, (int)(block / a.heads), (int)(block % a.heads), scratch);
-  else skip_grad(a, f, (int)(block - gates), scratch);
+  block -= gates;
+  if (f.dd) {
+    if (block < across) {
+      skip_grad(a, f, (int)block * FINISH_HEADS);
+      return;
+    }
+    block -= across;
+  }
+  const bool is_b = block >= f.sums;
+  const int64_t i = ((int64_t)(is_b ? block - f.sums : block) * FINISH_THREADS + threadIdx.x) * 4;
+  sum_parts<T>(is_b ? f.parts_b : f.parts_c, f.parts, f.size, (T*)(is_b ? f.db : f.dc), i);
 }
 
 // ---- plan ----
@@ -251,20 +293,32 @@ struct Plan {
   size_t table, first, decays, states, adjoints, last, dwrite, gate_out, gate_in, dd, parts_c, parts_b, total;
 };
 
-// Tokens of a segment: a whole sequence where the sequences alone fill half of
-// the chip's places for workgroups (two a CU), else as many chunks as leave
-// about three workgroups a CU: lengths are whole chunks and sequences ragged, and
-// with fewer the last round is half empty.  Each segment's states are written
-// and read twice, which holds the number down.  us of all launches, two / three /
-// four a CU: 30011 packed tokens of 24 heads 314 / 265 / 265, the gradients of
-// 4 x 2048 349 / 313 / 314.
-int segment_length(int64_t all, int64_t longest, int seqs, int64_t per_item, bool packed) {
-  constexpr int64_t WANT = 768, ENOUGH = 256;
-  if (!packed && seqs * per_item >= ENOUGH) return (int)std::max<int64_t>(longest, 1);
-  const int64_t items = std::max<int64_t>(1, WANT / per_item);
-  const int64_t chunks = (all + CHUNK - 1) / CHUNK;
-  const int64_t len = std::max<int64_t>(1, (chunks + items - 1) / items) * CHUNK;
-  return (int)std::min<int64_t>(len, std::max<int64_t>(longest, 1));
+// Tokens of a segment: of all numbers of chunks the one whose estimated time is
+// least.  Workgroups run in rounds of two a CU, a round as long as a segment; a
+// chunk of a round takes about 14 us in the sweeps for the states and the results
+// together, and a segment's states are written once and read and written once
+// more, at 6.6 TB/s.  A whole sequence's state stays in registers.  us of the
+// launches forward, at lengths of 4 / 6 / 8 / 12 / 16 chunks of 30011 packed tokens of
+// 24 heads of 64 x 128: 269 / 258 / 256 / 301 / 267; at 2 / 4 / 5 chunks of 4 x 2048:
+// 89 / 84 / 92, and their gradients 281 / 265 / 268.
+int segment_length(int64_t all, int64_t longest, int seqs, int64_t per_item, size_t state, bool packed) {
+  const int64_t slots = 2 * 256, most = std::max<int64_t>(1, (longest + CHUNK - 1) / CHUNK);
+  double best = 0;
+  int64_t length = most;
+  for (int64_t chunks = 1; chunks <= most; chunks += 1 + chunks / 16) {
+    // ragged sequences end inside a segment each
+    const int64_t items = packed ? (all + chunks * CHUNK - 1) / (chunks * CHUNK) + seqs
+                                 : seqs * ((most + chunks - 1) / chunks);
+    const int64_t rounds = (items * per_item + slots - 1) / slots;
+    const double us = 14.0 * rounds * chunks + items * (3.0 * state / 6.6e6);
+    if (chunks == 1 || us < best) {
+      best = us;
+      length = chunks;
+    }
+  }
+  const double whole = 10.0 * most * ((seqs * per_item + slots - 1) / slots);
+  if (whole <= best) length = most;
+  return (int)std::min<int64_t>(length * CHUNK, std::max<int64_t>(longest, 1));
 }
 
 Plan make_plan(const Scan& s, bool backward) {
@@ -276,11 +330,11 @@ Plan make_plan(const Scan& s, bool backward) {
   // 4 x 2048 tokens of 24 heads of 64, 32 channels 183
   p.query = Cut(s, s.head_dim <= 32 ? 32 : 64);
   const int64_t all = s.all_tokens();
-  p.length = segment_length(all, s.tokens, s.seqs, (int64_t)p.value.blocks * s.groups, packed);
+  const size_t state = (size_t)s.heads * s.head_dim * s.states * 4;
+  p.length = segment_length(all, s.tokens, s.seqs, (int64_t)p.value.blocks * s.groups, state, packed);
   p.segments = packed ? 0 : std::max<int>(1, (int)((s.tokens + p.length - 1) / p.length));
   p.by_item = p.length < s.tokens;
   p.items = packed ? (int)(s.tokens / p.length) + s.seqs + 2 : s.seqs * p.segments;
-  const size_t state = (size_t)s.heads * s.head_dim * s.states * 4;
   const size_t rows = (size_t)s.heads * p.value.col_tiles;
   auto take = [&](size_t bytes) {
     const size_t at = p.total;
@@ -381,7 +435,14 @@ struct Sweep {
     const int size = s.heads * s.head_dim * s.states;
     const Join forward{at<float>(p.states), s.initial, last};
     const Join reverse = g ? Join{at<float>(p.adjoints), g->dfinal, g->dinitial} : Join{};
-    k_join<<<dim3((size + 255) / 256, s.seqs, g ? 2 : 1), 256, 0, stream>>>(
+    // four elements of one head a thread where all rows are of whole fours
+    bool wide = s.head_dim * s.states % 4 == 0;
+    for (const void* q : {(const void*)forward.initial, (const void*)forward.last, (const void*)reverse.initial,
+                          (const void*)reverse.last})
+      wide = wide && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    const int vec = wide ? 4 : 1;
+    auto* kernel = wide ? &k_join<4> : &k_join<1>;
+    kernel<<<dim3((size / vec + 255) / 256, s.seqs, g ? 2 : 1), 256, 0, stream>>>(
         forward, reverse, at<float>(p.decays), first(), p.segments, size, s.head_dim * s.states, s.heads);
     hip_check(hipGetLastError(), "scan state join");
   }
@@ -441,7 +502,8 @@ void scan_backward(const Scan& s, const ScanGrads& g, void* workspace, hipStream
   f.parts = p.query.blocks;
   f.items = p.items;
   f.entering_tiles = p.query.col_tiles;
-  f.sums = (uint32_t)((f.size + 1023) / 1024);
+  f.sums = (uint32_t)((f.size + 4 * FINISH_THREADS - 1) / (4 * FINISH_THREADS));
+  f.group = std::max(1, 256 / p.length);
   f.parts_c = (const float*)c.out;
   f.parts_b = (const float*)b.out;
   f.dc = g.dc;
@@ -455,10 +517,11 @@ void scan_backward(const Scan& s, const ScanGrads& g, void* workspace, hipStream
   f.dwrite = g.dwrite;
   f.ddecay = g.ddecay;
   f.dd = g.dd;
-  const int64_t grid = 2 * (int64_t)f.sums + (int64_t)p.items * s.heads + (g.dd ? s.heads : 0);
+  const int64_t across = (s.heads + FINISH_HEADS - 1) / FINISH_HEADS;
+  const int64_t grid = 2 * (int64_t)f.sums + p.items * across + (g.dd ? across : 0);
   if (grid > INT32_MAX) throw ArgError("too many tokens and heads for one call");
-  if (s.dtype == BF16) k_finish<bf16><<<(uint32_t)grid, 256, 0, stream>>>(x, f);
-  else k_finish<float><<<(uint32_t)grid, 256, 0, stream>>>(x, f);
+  if (s.dtype == BF16) k_finish<bf16><<<(uint32_t)grid, FINISH_THREADS, 0, stream>>>(x, f);
+  else k_finish<float><<<(uint32_t)grid, FINISH_THREADS, 0, stream>>>(x, f);
   hip_check(hipGetLastError(), "scan gradients");
 }
 

@@ -52,6 +52,8 @@ __device__ __forceinline__ void query_sweep(const SweepArgs& a, char* lds_raw, u
   using N = Num<T>;
   using Frag = typename N::Frag;
   using Lds = QueryLds<T, NB, PT>;
+  // forward the state's part ends in the gates' gradients too
+  constexpr int STATE = REV ? N::FAIR : N::FULL, PAIRS = N::FAIR;
   using Key = typename Lds::Key;
   using Value = typename Lds::Value;
   Lds& lds = *reinterpret_cast<Lds*>(lds_raw);
@@ -114,7 +116,7 @@ __device__ __forceinline__ void query_sweep(const SweepArgs& a, char* lds_raw, u
         for (int nt = 0; nt < 2 * NB; ++nt) {
 #pragma unroll
           for (int k = 0; k < PT / 2; ++k)
-            got[nt] = mma<T, N::FAIR>(split<T, N::FAIR>(join(h[2 * k][nt], h[2 * k + 1][nt])), of[k], got[nt]);
+            got[nt] = mma<T, STATE>(split<T, STATE>(join(h[2 * k][nt], h[2 * k + 1][nt])), of[k], got[nt]);
           got[nt] *= in;
         }
         if constexpr (!REV) {
@@ -145,10 +147,10 @@ __device__ __forceinline__ void query_sweep(const SweepArgs& a, char* lds_raw, u
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           if (REV ? 2 * m + 1 < i : 2 * m > i) continue;
-          const auto s = split<T, N::FAIR>(join(pairs[2 * m], pairs[2 * m + 1]));
+          const auto s = split<T, PAIRS>(join(pairs[2 * m], pairs[2 * m + 1]));
 #pragma unroll
           for (int nt = 0; nt < 2 * NB; ++nt)
-            got[nt] = mma<T, N::FAIR>(Key::cols(lds.key, 32 * m, 16 * nt), s, got[nt]);
+            got[nt] = mma<T, PAIRS>(Key::cols(lds.key, 32 * m, 16 * nt), s, got[nt]);
         }
         if constexpr (REV) {
           const float w = t.w[tok];
@@ -188,17 +190,17 @@ __device__ __forceinline__ void query_sweep(const SweepArgs& a, char* lds_raw, u
 #pragma unroll
       for (int p2 = 0; p2 < PT; p2 += 2) {
         step_end();
-        Split<T, N::FINE> s[2];
+        Split<T, N::FULL> s[2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const Frag v = Value::cols(vt, 32 * m, 16 * (p2 + p));
-          s[p] = split<T, N::FINE>(widen(v) * f);
+          s[p] = split<T, N::FULL>(widen(v) * f);
         }
 #pragma unroll
         for (int nt = 0; nt < 2 * NB; ++nt) {
           const auto k = Key::cols(lds.key, 32 * m, 16 * nt);
 #pragma unroll
-          for (int p = 0; p < 2; ++p) h[p2 + p][nt] = mma<T, N::FINE>(s[p], k, h[p2 + p][nt]);
+          for (int p = 0; p < 2; ++p) h[p2 + p][nt] = mma<T, N::FULL>(s[p], k, h[p2 + p][nt]);
         }
       }
     }

@@ -34,15 +34,15 @@ __device__ __forceinline__ void add_chunk(f32x4 (&h)[2 * NB][PT], const T* key, 
   for (int m = 0; m < 2; ++m) {
     if (32 * m >= n) break;
     const f32x8 f = to_state<REV>(t, m);
-    Split<T, N::FINE> s[PT];
+    Split<T, N::FULL> s[PT];
 #pragma unroll
     for (int p = 0; p < PT; ++p)
-      s[p] = split<T, N::FINE>(widen(Tile<T, 16 * PT>::cols(value, 32 * m, 16 * p)) * f);
+      s[p] = split<T, N::FULL>(widen(Tile<T, 16 * PT>::cols(value, 32 * m, 16 * p)) * f);
 #pragma unroll
     for (int nt = 0; nt < 2 * NB; ++nt) {
       const auto k = Tile<T, 32 * NB>::cols(key, 32 * m, 16 * nt);
 #pragma unroll
-      for (int p = 0; p < PT; ++p) h[nt][p] = mma<T, N::FINE>(k, s[p], h[nt][p]);
+      for (int p = 0; p < PT; ++p) h[nt][p] = mma<T, N::FULL>(k, s[p], h[nt][p]);
     }
   }
 }
@@ -76,6 +76,8 @@ __device__ __forceinline__ void value_sweep(const SweepArgs& a, char* lds_raw, u
   using N = Num<T>;
   using Frag = typename N::Frag;
   using Lds = ValueLds<T, NB, PT, VALUES>;
+  // in reverse the results end in the gates' gradients too
+  constexpr int PIECES = REV ? N::FULL : N::FAIR;
   using Key = typename Lds::Key;
   using Value = typename Lds::Value;
   Lds& lds = *reinterpret_cast<Lds*>(lds_raw);
@@ -138,14 +140,14 @@ __device__ __forceinline__ void value_sweep(const SweepArgs& a, char* lds_raw, u
       f32x4 y[TILES][PT] = {};
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
-        Split<T, N::FAIR> state[PT];
+        Split<T, PIECES> state[PT];
 #pragma unroll
-        for (int p = 0; p < PT; ++p) state[p] = split<T, N::FAIR>(join(h[2 * k][p], h[2 * k + 1][p]));
+        for (int p = 0; p < PT; ++p) state[p] = split<T, PIECES>(join(h[2 * k][p], h[2 * k + 1][p]));
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
           const Frag qf = Key::rows(lds.query, 16 * i, 32 * k);
 #pragma unroll
-          for (int p = 0; p < PT; ++p) y[i][p] = mma<T, N::FAIR>(state[p], qf, y[i][p]);
+          for (int p = 0; p < PT; ++p) y[i][p] = mma<T, PIECES>(state[p], qf, y[i][p]);
         }
       }
       f32x4 row_sum[REV ? TILES : 1] = {};
@@ -199,10 +201,10 @@ __device__ __forceinline__ void value_sweep(const SweepArgs& a, char* lds_raw, u
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           if (REV ? 2 * m + 1 < i : 2 * m > i) continue;
-          const auto s = split<T, N::FAIR>(join(pairs[2 * m], pairs[2 * m + 1]));
+          const auto s = split<T, PIECES>(join(pairs[2 * m], pairs[2 * m + 1]));
 #pragma unroll
           for (int p = 0; p < PT; ++p)
-            y[i][p] = mma<T, N::FAIR>(Value::cols(vt, 32 * m, 16 * p), s, y[i][p]);
+            y[i][p] = mma<T, PIECES>(Value::cols(vt, 32 * m, 16 * p), s, y[i][p]);
         }
         Frag vf[PT / 2];
 #pragma unroll
