@@ -1,10 +1,11 @@
 // The causal convolution of each channel, its gradients and its single-token
 // form:  y_t = act(bias + sum_k weight_k x_{t - taps + 1 + k}).
 //
-// Bound by memory: a thread keeps the window of its channels (16 bytes of a
-// token) in registers and walks a run of tokens, four loads ahead, so that an
-// input is read once and, at the start of a run, taps - 1 times more, which the
-// caches answer.
+// Bound by memory: a thread keeps the window of its channels in registers and
+// walks a run of tokens, loads ahead, so that an input is read once and, at the
+// start of a run, taps - 1 times more, which the caches answer.  Two channels a
+// thread: a wavefront's loads are whole lines either way, and more wavefronts
+// cover more of a load's wait than wider ones.
 // Before a sequence's first token the window holds its initial state, oldest
 // first, or zeros.
 #pragma clang fp contract(fast)
@@ -15,12 +16,18 @@
 namespace fhe::clear {
 namespace {
 
-constexpr int RUN = 16, AHEAD = 4;  // tokens of a run; loads ahead
+// Tokens of a run, loads ahead and channels of a thread.  17409 tokens of 1792
+// channels in 16 bits: 47.6 us (the copy's rate) with these; with 8 channels and
+// 4 loads ahead 67, with 4 and 8 50, with 2 and runs of 32 or 64 45 and 48.
+// 8192 tokens: 16.6 us, with runs of 32 or 64 18.3 and 22.  A single token of
+// 1792 channels: 3.7 us, with 8 channels a thread 5.6.
+constexpr int RUN = 16, AHEAD = 8, NARROW = 2;
 // A backward workgroup: BACK_RUNS runs of BACK_PIECES pieces of the channels,
-// whose weights' gradients it sums before it writes them.
-// The pieces are of at most four channels: of eight, a thread's weights, their
-// gradients, its window and its inputs' take 232 registers.
-constexpr int RUN_BACK = 16, BACK_PIECES = 32, BACK_RUNS = 8;
+// whose weights' gradients it sums before it writes them.  8192 tokens of 1792
+// channels in 16 bits: 33 us; runs of 8 or 32 37 and 40; pieces of 2 channels 41;
+// four loads ahead 42, for a thread's weights, their gradients, its window and
+// its inputs' fill its registers.
+constexpr int RUN_BACK = 16, BACK_PIECES = 32, BACK_RUNS = 8, WIDE = 4;
 
 struct ConvArgs {
   Conv c;
@@ -112,8 +119,20 @@ template <int VEC, int KT>
 __device__ __forceinline__ void read_weights(const float* weight, const float* bias, int c0, int count,
                                              int taps, float (&w)[KT][VEC], float (&b)[VEC]) {
 #pragma unroll
+  for (int i = 0; i < VEC; ++i) b[i] = bias && i < count ? bias[c0 + i] : 0.0f;
+  if (KT == 4 && taps == 4 && reinterpret_cast<uintptr_t>(weight) % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float4 v = i < count ? reinterpret_cast<const float4*>(weight)[c0 + i] : float4{};
+      w[0][i] = v.x;
+      w[1][i] = v.y;
+      w[2][i] = v.z;
+      w[3][i] = v.w;
+    }
+    return;
+  }
+#pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    b[i] = bias && i < count ? bias[c0 + i] : 0.0f;
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
       const int at = k - (KT - taps);
@@ -419,8 +438,9 @@ __global__ __launch_bounds__(256) void k_conv_step(ConvStep c, T* y, int pieces)
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// f(type, elements of a thread, places of the window) for a launch.  16-byte
-// pieces need the channels to be a multiple of them and every row aligned.
+// f(type, most elements of a thread, places of the window) for a launch.  Pieces
+// of more than one need the channels to be a multiple of 16 bytes and every row
+// aligned.
 template <class F>
 void dispatch(uint32_t dtype, bool wide, int taps, F&& f) {
   auto by_taps = [&](auto zero, auto vec) {
@@ -468,10 +488,11 @@ void conv(const Conv& c, void* y, void* final_state, hipStream_t stream) {
                     aligned(final_state) && aligned(c.initial);
   dispatch(c.dtype, wide, c.taps, [&](auto zero, auto vec, auto kt) {
     using T = decltype(zero);
-    a.pieces = (c.channels + vec() - 1) / vec();
+    constexpr int VEC = vec() > NARROW ? NARROW : vec();
+    a.pieces = (c.channels + VEC - 1) / VEC;
     const int64_t rows = jobs_of(c, RUN) + (final_state ? (int64_t)c.seqs * (c.taps - 1) : 0);
     if (!rows) return;
-    k_conv<T, vec(), kt()><<<grid_of(rows * a.pieces), 256, 0, stream>>>(a);
+    k_conv<T, VEC, kt()><<<grid_of(rows * a.pieces), 256, 0, stream>>>(a);
   });
   hip_check(hipGetLastError(), "convolution");
 }
@@ -493,7 +514,7 @@ void conv_backward(const Conv& c, const ConvGrads& g, void* workspace, hipStream
   dispatch(c.dtype, wide, c.taps, [&](auto zero, auto vec, auto kt) {
     using T = decltype(zero);
     if (parts) {
-      constexpr int VEC = vec() > 4 ? 4 : vec();
+      constexpr int VEC = vec() > WIDE ? WIDE : vec();
       const dim3 grid((uint32_t)parts, (c.channels + BACK_PIECES * VEC - 1) / (BACK_PIECES * VEC));
       k_conv_back<T, VEC, kt()><<<grid, BACK_PIECES * BACK_RUNS, 0, stream>>>(a);
     }
@@ -511,8 +532,9 @@ void conv_step(const ConvStep& c, void* y, hipStream_t stream) {
                     aligned(y) && aligned(c.state);
   dispatch(c.dtype, wide, c.taps, [&](auto zero, auto vec, auto kt) {
     using T = decltype(zero);
-    const int pieces = (c.channels + vec() - 1) / vec();
-    k_conv_step<T, vec(), kt()><<<grid_of((int64_t)c.requests * pieces), 256, 0, stream>>>(c, (T*)y, pieces);
+    constexpr int VEC = vec() > NARROW ? NARROW : vec();
+    const int pieces = (c.channels + VEC - 1) / VEC;
+    k_conv_step<T, VEC, kt()><<<grid_of((int64_t)c.requests * pieces), 256, 0, stream>>>(c, (T*)y, pieces);
   });
   hip_check(hipGetLastError(), "convolution step");
 }
