@@ -16,7 +16,7 @@
 namespace fhe::clear {
 namespace {
 
-// Tokens of a run, loads ahead and channels of a thread.  17409 tokens of 1792
+// Tokens of a run, loads ahead and channels of a thread.  30011 tokens of 1792
 // channels in 16 bits: 47.6 us (the copy's rate) with these; with 8 channels and
 // 4 loads ahead 67, with 4 and 8 50, with 2 and runs of 32 or 64 45 and 48.
 // 8192 tokens: 16.6 us, with runs of 32 or 64 18.3 and 22.  A single token of

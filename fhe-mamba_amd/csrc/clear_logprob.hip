@@ -6,8 +6,7 @@
 //   d l_i = a (1[i = t] - p_i) - b p_i (log p_i + H)   for gradients a, b
 //
 // One pass over the logits: each workgroup of a row keeps m, s and u of its
-// part and its part's best entries; a second kernel joins the parts.  Bound by
-// memory.  Entries of -inf are tokens that are not allowed: p = 0, and they add
+// part; a second kernel joins the parts.  Bound by memory.  Entries of -inf are tokens that are not allowed: p = 0, and they add
 // nothing anywhere.
 #pragma clang fp contract(fast)
 #include <algorithm>
@@ -50,25 +49,13 @@ __device__ __forceinline__ Stats wave_join(Stats a) {
   return a;
 }
 
-// An entry as a number that orders by value, then by the lower index.
-__device__ __forceinline__ uint64_t to_key(float v, uint32_t index) {
-  uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);  // -0 is 0
-  b = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (uint64_t)b << 32 | (0xffffffffu - index);
-}
-__device__ __forceinline__ float key_value(uint64_t k) {
-  uint32_t b = (uint32_t)(k >> 32);
-  b = b & 0x80000000u ? b & 0x7fffffffu : ~b;
-  return __builtin_bit_cast(float, b);
-}
-__device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xffffffffu - (uint32_t)k; }
-
 struct RowArgs {
   Logprob l;
   LogprobOut o;
   int splits, tiles;  // workgroups a row; tiles of each
+  int64_t all_tiles;  // of a row
   Stats* stats;       // [rows][splits]
-  uint64_t* best;     // [rows][splits][top]
+  uint64_t* keys;     // [rows][all_tiles][SETS]
 };
 
 // Sixteen logits of a thread in a tile that begins at column `base` (a multiple
@@ -131,24 +118,86 @@ __device__ __forceinline__ Stats add16(Stats a, const float* v) {
 
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// The `top` largest of this tile's keys and the `top` that `best` holds (0: an
-// empty place), in order, to `best`.  The threads are 64 groups of four, one of
-// each wavefront; the top-th largest of the groups' maxima bounds the entry wanted
-// from below, and only the `top` groups at or over it can hold entries that
-// large: the candidates are at most 64 top, and hardly more than top.
+// An entry's value as a number that orders as it, above 0; equal for the zeros.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+// Ordered by value, then by the lower index.
+__device__ __forceinline__ uint64_t to_key(uint32_t order, uint32_t index) {
+  return (uint64_t)order << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xffffffffu - (uint32_t)k; }
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad_swap(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+
+// The likeliest entries are found in two steps.  The 64 entries that four
+// neighbouring threads hold of a tile are a set, and the first kernel writes the
+// largest key of each.  An entry among the `top` largest lies in one of the `top`
+// sets with the largest keys: were it in another, each of these had a larger
+// entry.  The second kernel picks those sets and reads only their entries again.
+// Keeping the `top` best in the first kernel instead, tile by tile, takes it from
+// 13.6 to 28 us for 20 of 250 rows of 50280.
+constexpr int SET = 64, SETS = TILE / SET;  // entries of a set, sets of a tile
+
+// The largest key of the set of this thread, 0 if all of it lies outside of the row.
+template <class T>
+__device__ __forceinline__ uint64_t set_key(const float* v, int64_t base, int64_t vocab) {
+  uint32_t order[16], most = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) order[j] = order_of(v[j]);
+  if (base < 0 || base + TILE > vocab) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int64_t c = Sixteen<T>::column(base, j);
+      if (c < 0 || c >= vocab) order[j] = 0;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) most = max(most, order[j]);
+  most = max(most, quad_swap<0xb1>(most));  // of lanes 1, 0, 3, 2
+  most = max(most, quad_swap<0x4e>(most));  // 2, 3, 0, 1
+  if (!most) return 0;
+  uint32_t first = 0xffffffffu;
+#pragma unroll
+  for (int j = 15; j >= 0; --j)
+    if (order[j] == most) first = (uint32_t)Sixteen<T>::column(base, j);
+  first = min(first, quad_swap<0xb1>(first));
+  first = min(first, quad_swap<0x4e>(first));
+  return to_key(most, first);
+}
+
+// Column of entry e of the set that holds column c.
+template <class T>
+__device__ __forceinline__ int64_t set_column(int64_t c, int lead, int e) {
+  constexpr int RUN = 4 * Num<T>::VEC;  // a set's entries in a row
+  const int64_t at = c + lead, tile = at / TILE * TILE;
+  const int run = (int)(at - tile) / RUN % SETS;
+  return tile - lead + (e / RUN * SETS + run) * RUN + e % RUN;
+}
+
+constexpr int HELD = 8;  // keys of a thread
 struct TopLds {
-  uint64_t maxima[THREADS], best[MAX_TOP], candidate[64 * MAX_TOP + MAX_TOP];
+  uint64_t maxima[THREADS], best[MAX_TOP], candidate[4 * HELD * MAX_TOP + MAX_TOP];
   int count;
 };
 
-template <class T>
-__device__ void keep_best(TopLds& lds, const float* v, int64_t base, int64_t vocab, int top) {
+// The `top` largest of the threads' keys and of the `top` that `best` holds (0:
+// none), in order, to `best`.  No two of them are equal.  The threads are 64
+// groups of four, one of each wavefront; the top-th largest of the groups' maxima
+// bounds the keys wanted from below, and only the `top` groups at or over it can
+// hold keys that large: the candidates are at most 32 top, and hardly more than top.
+__device__ void keep_best(TopLds& lds, const uint64_t (&key)[HELD], int top) {
   uint64_t mine = 0;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int64_t c = Sixteen<T>::column(base, j);
-    if (c >= 0 && c < vocab) mine = max64(mine, to_key(v[j], (uint32_t)c));
-  }
+  for (int j = 0; j < HELD; ++j) mine = max64(mine, key[j]);
   lds.maxima[threadIdx.x] = mine;
   if (threadIdx.x == 0) lds.count = 0;
   __syncthreads();
@@ -163,7 +212,7 @@ __device__ void keep_best(TopLds& lds, const float* v, int64_t base, int64_t voc
     const uint32_t hi = __builtin_amdgcn_readlane((int)(group >> 32), i);
     rank += ((uint64_t)hi << 32 | lo) > group;
   }
-  // fewer than `top` groups with entries: all are candidates
+  // fewer than `top` groups with keys: all are candidates
   const uint64_t found = __ballot(group && rank == top - 1);
   uint64_t bound = lds.best[top - 1];
   if (found) {
@@ -174,12 +223,8 @@ __device__ void keep_best(TopLds& lds, const float* v, int64_t base, int64_t voc
   }
   if (mine && mine >= bound) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int64_t c = Sixteen<T>::column(base, j);
-      if (c < 0 || c >= vocab) continue;
-      const uint64_t k = to_key(v[j], (uint32_t)c);
-      if (k >= bound) lds.candidate[atomicAdd(&lds.count, 1)] = k;
-    }
+    for (int j = 0; j < HELD; ++j)
+      if (key[j] && key[j] >= bound) lds.candidate[atomicAdd(&lds.count, 1)] = key[j];
   }
   if ((int)threadIdx.x < top && lds.best[threadIdx.x])
     lds.candidate[atomicAdd(&lds.count, 1)] = lds.best[threadIdx.x];
@@ -189,6 +234,7 @@ __device__ void keep_best(TopLds& lds, const float* v, int64_t base, int64_t voc
   for (int i = threadIdx.x; i < count; i += THREADS) {
     const uint64_t k = lds.candidate[i];
     int r = 0;
+#pragma unroll 8
     for (int j = 0; j < count; ++j) r += lds.candidate[j] > k;
     if (r < top) lds.best[r] = k;
   }
@@ -198,15 +244,10 @@ __device__ void keep_best(TopLds& lds, const float* v, int64_t base, int64_t voc
 template <class T, bool TOP>
 __global__ __launch_bounds__(THREADS) void k_row_parts(RowArgs a) {
   __shared__ Stats waves[THREADS / 64];
-  __shared__ TopLds lds;
   const int64_t row_i = blockIdx.x / a.splits;
   const int split = blockIdx.x % a.splits;
   const T* row = (const T*)a.l.logits + row_i * a.l.row_stride;
   const int lead = row_lead(row);
-  if constexpr (TOP) {
-    if (threadIdx.x < MAX_TOP) lds.best[threadIdx.x] = 0;
-    __syncthreads();
-  }
   Stats st{-INFINITY, 0.0f, 0.0f};
   const int64_t start = (int64_t)split * a.tiles * TILE - lead;
   Sixteen<T> x;
@@ -218,7 +259,11 @@ __global__ __launch_bounds__(THREADS) void k_row_parts(RowArgs a) {
     x.widen(v);
     if (t + 1 < a.tiles) x.read(row, base + TILE, a.l.vocab);  // in flight meanwhile
     st = add16(st, v);
-    if constexpr (TOP) keep_best<T>(lds, v, base, a.l.vocab, a.l.top);
+    if constexpr (TOP) {
+      const uint64_t key = set_key<T>(v, base, a.l.vocab);
+      const int64_t tile = row_i * a.all_tiles + (int64_t)split * a.tiles + t;
+      if (threadIdx.x % 4 == 0) a.keys[tile * SETS + threadIdx.x / 4] = key;
+    }
   }
   st = wave_join(st);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = st;
@@ -228,14 +273,10 @@ __global__ __launch_bounds__(THREADS) void k_row_parts(RowArgs a) {
     for (int w = 1; w < THREADS / 64; ++w) st = join(st, waves[w]);
     a.stats[row_i * a.splits + split] = st;
   }
-  if constexpr (TOP) {
-    if ((int)threadIdx.x < a.l.top)
-      a.best[(row_i * a.splits + split) * a.l.top + threadIdx.x] = lds.best[threadIdx.x];
-  }
 }
 
 // A workgroup a row.
-template <class T>
+template <class T, bool TOP>
 __global__ __launch_bounds__(THREADS) void k_row_join(RowArgs a) {
   __shared__ Stats waves[THREADS / 64];
   __shared__ float peak, log_sum;
@@ -263,21 +304,44 @@ __global__ __launch_bounds__(THREADS) void k_row_join(RowArgs a) {
     }
     a.o.logprob[row_i] = lp;
   }
-  if (!a.l.top) return;
-  __syncthreads();
-  __shared__ uint64_t best[MAX_SPLITS * MAX_TOP];
-  const int count = a.splits * a.l.top;
-  for (int i = threadIdx.x; i < count; i += THREADS) best[i] = a.best[row_i * count + i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < count; i += THREADS) {
-    const uint64_t k = best[i];
-    if (!k) continue;
-    int r = 0;
-    for (int j = 0; j < count; ++j) r += best[j] > k;
-    if (r < a.l.top) {
+  if constexpr (TOP) {
+    const int top = a.l.top;
+    const T* row = (const T*)a.l.logits + row_i * a.l.row_stride;
+    const int lead = row_lead(row);
+    const int64_t count = (a.l.vocab + lead + TILE - 1) / TILE * SETS;  // at most all_tiles SETS
+    const uint64_t* keys = a.keys + row_i * a.all_tiles * SETS;
+    __shared__ TopLds lds;
+    __shared__ uint64_t sets[MAX_TOP];
+    if (threadIdx.x < MAX_TOP) lds.best[threadIdx.x] = 0;
+    __syncthreads();
+    uint64_t key[HELD];
+    for (int64_t first = 0; first < count; first += THREADS * HELD) {
+#pragma unroll
+      for (int j = 0; j < HELD; ++j) {
+        const int64_t at = first + j * THREADS + threadIdx.x;
+        key[j] = at < count ? keys[at] : 0;
+      }
+      keep_best(lds, key, top);
+    }
+    if (threadIdx.x < MAX_TOP) {
+      sets[threadIdx.x] = (int)threadIdx.x < top ? lds.best[threadIdx.x] : 0;
+      lds.best[threadIdx.x] = 0;
+    }
+    __syncthreads();
+    static_assert(MAX_TOP * SET <= THREADS * HELD);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      const int at = j * THREADS + threadIdx.x;
+      const uint64_t set = sets[at / SET];
+      const int64_t c = set_column<T>(key_index(set), lead, at % SET);
+      key[j] = set && c >= 0 && c < a.l.vocab ? to_key(order_of((float)row[c]), (uint32_t)c) : 0;
+    }
+    keep_best(lds, key, top);
+    if ((int)threadIdx.x < top) {
+      const uint64_t k = lds.best[threadIdx.x];
       const float v = key_value(k);
-      a.o.top_logprob[row_i * a.l.top + r] = v == -INFINITY ? -INFINITY : (v - peak) - log_sum;
-      a.o.top_index[row_i * a.l.top + r] = (int)key_index(k);
+      a.o.top_logprob[row_i * top + threadIdx.x] = v == -INFINITY ? -INFINITY : (v - peak) - log_sum;
+      a.o.top_index[row_i * top + threadIdx.x] = k ? (int)key_index(k) : 0;  // a row of NaN may have none
     }
   }
 }
@@ -341,8 +405,8 @@ __global__ __launch_bounds__(THREADS) void k_row_back(BackArgs a) {
 // first tile's end.
 int64_t tiles_of(const Logprob& l) { return (l.vocab + 7 + TILE - 1) / TILE; }
 
-// Workgroups of a row: one a tile while that is at most 64 of a row or about
-// four a CU in all; the parts' best entries are joined by comparing all pairs.
+// Workgroups of a row: one a tile, but at most 64, and more than one only up to
+// sixteen a CU in all.
 int splits_of(const Logprob& l) {
   const int64_t tiles = tiles_of(l), want = std::max<int64_t>(1, 4096 / l.rows);
   return (int)std::min<int64_t>({tiles, want, MAX_SPLITS});
@@ -351,21 +415,23 @@ int splits_of(const Logprob& l) {
 }  // namespace
 
 size_t logprob_workspace(const Logprob& l) {
-  return (size_t)l.rows * splits_of(l) * (sizeof(Stats) + 8 * (size_t)l.top) + 256;
+  const size_t keys = l.top ? (size_t)tiles_of(l) * SETS * sizeof(uint64_t) : 0;
+  return (size_t)l.rows * (keys + splits_of(l) * sizeof(Stats));
 }
 
 void logprob(const Logprob& l, const LogprobOut& o, void* workspace, hipStream_t stream) {
-  RowArgs a{l, o, splits_of(l), 0, nullptr, nullptr};
-  a.tiles = (int)((tiles_of(l) + a.splits - 1) / a.splits);
-  a.best = (uint64_t*)workspace;
-  a.stats = (Stats*)(a.best + (size_t)l.rows * a.splits * l.top);
+  RowArgs a{l, o, splits_of(l), 0, tiles_of(l), nullptr, nullptr};
+  a.tiles = (int)((a.all_tiles + a.splits - 1) / a.splits);
+  a.keys = (uint64_t*)workspace;
+  a.stats = (Stats*)(a.keys + (l.top ? (size_t)l.rows * a.all_tiles * SETS : 0));
   auto run = [&](auto zero) {
     using T = decltype(zero);
     const uint32_t grid = (uint32_t)(l.rows * a.splits);
     if (l.top) k_row_parts<T, true><<<grid, THREADS, 0, stream>>>(a);
     else k_row_parts<T, false><<<grid, THREADS, 0, stream>>>(a);
     hip_check(hipGetLastError(), "log probabilities");
-    k_row_join<T><<<(uint32_t)l.rows, THREADS, 0, stream>>>(a);
+    if (l.top) k_row_join<T, true><<<(uint32_t)l.rows, THREADS, 0, stream>>>(a);
+    else k_row_join<T, false><<<(uint32_t)l.rows, THREADS, 0, stream>>>(a);
     hip_check(hipGetLastError(), "log probabilities join");
   };
   if (l.dtype == BF16) run(bf16{});
