@@ -17,6 +17,16 @@
 // dg_r is the sum of M over t >= r > s: what crosses the segment's end,
 // <A, h> there, plus the sums over t >= r of what enters at t less what leaves.
 // Terms with s = t are in neither, and the sums restart every few hundred tokens.
+//
+// 24 heads of 64 x 128 in 16 bits: a prompt of 1000 tokens takes 13.6 us for the
+// segments' states, 11.8 for carrying them and 12.6 for the results; 30011 packed
+// tokens 62 + 22 + 147; 4 x 2048
+// tokens 26 + 9 + 48, and their gradients 34 + 16 + 188 and 22 for the last sums.
+// The sweeps read and write a fifth of what memory would pass in that time and are
+// bound by a wavefront's own work: of its cycles the vector instructions (splits
+// into 16-bit pieces, decays, pairs) take two fifths, the matrix products a quarter,
+// waits for LDS and loads the most of the rest, with the two wavefronts a SIMD that
+// the states' registers leave.
 #pragma clang fp contract(fast)
 #include "clear_scan.hpp"
 

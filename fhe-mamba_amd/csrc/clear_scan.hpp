@@ -176,8 +176,9 @@ __device__ __forceinline__ f32x8 to_state(const Gates& t, int m) {
 }
 
 // Tokens [0, n) of `width` contiguous elements on their way into the rows of an LDS
-// tile of 64 rows and SPAN columns: zeros past the width and the count.  THREADS threads; loading and storing are apart so that a
-// chunk's loads are all in flight at once.
+// tile of 64 rows and SPAN columns: zeros past the width and the count.  THREADS
+// threads; loading and storing are apart so that a chunk's loads are all in flight
+// at once.
 //
 // FULL: every row has SPAN elements and is wide, and there is a row 0.
 template <class T, int SPAN, int THREADS, bool FULL>
