@@ -8,9 +8,9 @@
 // One pass over the logits: each workgroup of a row keeps m, s and u of its
 // part; a second kernel joins the parts.  Bound by memory where there are many
 // rows: 4095 of 50280 in 16 bits take 103 + 7 us forward (4.0 TB/s, a plain sum's
-// rate) and 150 for the gradient (5.5 TB/s, part of it from the last-level cache).  A row alone takes 13 us, the waits of
-// two launches.  Entries of -inf are tokens that are not allowed: p = 0, and they
-// add nothing anywhere.
+// rate) and 150 for the gradient (5.5 TB/s, part of it from the last-level
+// cache).  A row alone takes 13 us, the waits of two launches.  Entries of -inf are
+// tokens that are not allowed: p = 0, and they add nothing anywhere.
 #pragma clang fp contract(fast)
 #include <algorithm>
 

