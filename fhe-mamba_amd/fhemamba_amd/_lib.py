@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import atexit
 import ctypes
+import importlib.util
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -112,6 +113,20 @@ SIGNATURES = {
 }
 
 
+def _one_hip_runtime():
+    """The HIP runtime that PyTorch brings, loaded before the library asks for one, or None.
+
+    A process can use one HIP runtime only: of two the second finds no GPU, or takes the streams and
+    memory of the first for its own.  PyTorch's wheels bring theirs under the library's soname and
+    would load it beside the system's; loaded first it serves both, whichever is imported first."""
+    spec = importlib.util.find_spec("torch")
+    for folder in (spec.submodule_search_locations or ()) if spec else ():
+        path = os.path.join(folder, "lib", "libamdhip64.so")
+        if os.path.exists(path):
+            return ctypes.CDLL(path)
+    return None
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -127,6 +142,7 @@ def _load():
     return lib
 
 
+_hip = _one_hip_runtime()
 lib = _load()
 
 # Finalizers stop calling into the library once interpreter shutdown begins
@@ -161,7 +177,7 @@ def device_free_bytes(device: int | None = None) -> int | None:
     hipMemGetInfo from the HIP runtime the library links, with that device
     current for the call), or None when it cannot be read."""
     try:
-        hip = ctypes.CDLL("libamdhip64.so")
+        hip = _hip or ctypes.CDLL("libamdhip64.so")
         free, total = ctypes.c_size_t(0), ctypes.c_size_t(0)
         prev = ctypes.c_int(0)
         if device is not None:
