@@ -170,3 +170,24 @@ def test_refusals():
                      ("contiguous", (state.transpose(0, 1).contiguous().transpose(0, 1), x[:, 0], w))]:
         with pytest.raises(ValueError, match=match):
             clear.causal_conv_step(*a)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("shift", [0, 1, 4])
+def test_weights_that_begin_anywhere(shift, dtype):
+    """Four taps are read as one piece where the weights are aligned to it, and singly where not."""
+    from fhemamba_amd import clear
+
+    d = make(9, 50, 48, 4, dtype, 1)
+    flat = torch.zeros(48 * 4 + 8, device="cuda")
+    weight = flat[shift:shift + 48 * 4].view(48, 4)
+    weight.copy_(d["weight"])
+    y, last = clear.causal_conv(d["x"].cuda()[None], weight, d["bias"].cuda(), initial_state=d["initial"].cuda(),
+                                return_state=True)
+    y0, last0 = R.conv(d["x"].double(), d["weight"].double(), d["bias"].double(), d["initial"].double(),
+                       R.spans([50]))
+    assert R.rel(y[0], y0) <= R.bound(y)
+    assert torch.equal(last.cpu().double(), last0)
+    state = d["initial"].cuda()
+    step = clear.causal_conv_step(state, d["x"].cuda()[:1], weight, d["bias"].cuda())
+    assert R.rel(step, y0[:1]) <= R.bound(step)

@@ -208,3 +208,40 @@ def test_refusals():
                          ("top", (logits, targets), {"top": -1})]:
         with pytest.raises(ValueError, match=match):
             clear.token_logprobs(*a, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("order", ["random", "rising", "falling", "equal", "few"])
+def test_most_of_a_long_row(order, dtype):
+    """32 of 300001, in every order of the sets of entries that they are picked from, at an odd row stride."""
+    from fhemamba_amd import clear
+
+    vocab, rows = 300001, 2
+    logits, _ = make(5, rows, vocab, dtype, False)
+    if order in ("rising", "falling"):
+        logits = torch.sort(logits, dim=1, descending=order == "falling").values
+    elif order == "equal":
+        logits[:] = 0.5
+    elif order == "few":  # fewer allowed tokens than places: the rest are masked ones, lowest first
+        keep = logits[:, 77777::100000].clone()
+        logits[:] = -math.inf
+        logits[:, 77777::100000] = keep
+    wide = torch.full((rows, vocab + 3), 9.0, dtype=dtype)
+    wide[:, 2:vocab + 2] = logits
+    print(f"[logprob] long {order} {dtype}", flush=True)
+    got = clear.token_logprobs(wide.cuda()[:, 2:vocab + 2], torch.zeros(rows, dtype=torch.int64, device="cuda"), top=32)
+    check_top(got, logits, 32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_tokens_of_a_row_of_nan_are_in_it(dtype):
+    """What they are is not defined, but an index never leaves its row."""
+    from fhemamba_amd import clear
+
+    logits, targets = make(6, 3, 5000, dtype, False)
+    logits[0, 7] = math.nan
+    logits[1] = math.nan
+    logits[2] = torch.full((5000,), -1, dtype=torch.int16 if dtype == BF else torch.int32).view(dtype)  # NaN of all ones
+    got = clear.token_logprobs(logits.cuda(), targets.cuda(), top=32)
+    assert bool(((got.top_index >= 0) & (got.top_index < 5000)).all())
+    assert bool(torch.isnan(got.top_logprob).all())
