@@ -117,7 +117,7 @@ def _workspace(entry, like: torch.Tensor, *args) -> tuple:
     code = entry(*args, ctypes.byref(size))
     if code:
         _lib.check(code)
-    return torch.empty(size.value, dtype=torch.uint8, device=like.device), size.value
+    return like.new_empty(size.value, dtype=torch.uint8), size.value
 
 
 def _offsets(cu_seqlens, like: torch.Tensor) -> None:
@@ -131,7 +131,7 @@ def _offsets(cu_seqlens, like: torch.Tensor) -> None:
 def _wants_grad(*tensors) -> bool:
     if torch.is_grad_enabled():
         for t in tensors:
-            if isinstance(t, torch.Tensor) and t.requires_grad:
+            if t is not None and t.requires_grad:
                 return True
     return False
 
@@ -183,8 +183,8 @@ def _pack_scan(x, write, log_decay, B, C, D, initial_state, cu_seqlens) -> tuple
 def _scan_forward(tensors, return_state: bool):
     x = tensors[0]
     args, state_shape, held = _pack_scan(*tensors)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    state = torch.empty(state_shape, dtype=torch.float32, device=x.device) if return_state else None
+    y = x.new_empty(x.shape)
+    state = x.new_empty(state_shape, dtype=torch.float32) if return_state else None
     space, size = _workspace(_lib.lib.fhe_ssm_scan_workspace, x, args, 0)
     _run(_lib.lib.fhe_ssm_scan, x, args, _ptr(y), _ptr(state), _ptr(space), size)
     return y, state
@@ -209,7 +209,7 @@ class _Scan(torch.autograd.Function):
         def new(like, wanted=True):
             if like is None or not wanted:
                 return None
-            return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+            return like.new_empty(like.shape)
 
         dx, dw, dg, dB, dC = new(x), new(write), new(log_decay), new(B), new(C)
         dD, dh = new(D, ctx.needs_input_grad[6]), new(initial_state, ctx.needs_input_grad[7])
@@ -276,7 +276,7 @@ def ssm_step(state, x, write, log_decay, B, C, D=None, *, slots=None):
     if _wants_grad(state, x, write, log_decay, B, C, D):
         raise ValueError("ssm_step has no gradient: call it under torch.no_grad()")
     x, B, C = _rows(x), _rows(B), _rows(C)
-    y = torch.empty((R, H, P), dtype=x.dtype, device=x.device)
+    y = x.new_empty((R, H, P))
     args = _STEP.pack(_DTYPES[x.dtype], R, state.shape[0], H, P, N, G, _ptr(slots), *_strides(x, True),
                       *_strides(B, True), *_strides(C, True), *_strides(write, True), *_strides(log_decay, True),
                       _ptr(D), state.data_ptr())
@@ -325,8 +325,8 @@ def _pack_conv(x, weight, bias, initial_state, cu_seqlens, silu) -> tuple:
 def _conv_forward(tensors, silu: bool, return_state: bool):
     x = tensors[0]
     args, state_shape, held = _pack_conv(*tensors, silu)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    state = torch.empty(state_shape, dtype=x.dtype, device=x.device) if return_state else None
+    y = x.new_empty(x.shape)
+    state = x.new_empty(state_shape) if return_state else None
     _run(_lib.lib.fhe_causal_conv, x, args, _ptr(y), _ptr(state))
     return y, state
 
@@ -347,10 +347,10 @@ class _Conv(torch.autograd.Function):
         args, state_shape, held = _pack_conv(*tensors, ctx.silu)
         dy = torch.zeros_like(x) if dy is None else _rows(dy)
         dstate = None if dstate is None else dstate.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty(weight.shape, dtype=torch.float32, device=x.device)
-        db = None if bias is None else torch.empty(bias.shape, dtype=torch.float32, device=x.device)
-        dh = None if initial_state is None else torch.empty(state_shape, dtype=x.dtype, device=x.device)
+        dx = x.new_empty(x.shape)
+        dw = weight.new_empty(weight.shape)
+        db = None if bias is None else bias.new_empty(bias.shape)
+        dh = None if initial_state is None else x.new_empty(state_shape)
         grads = _CONV_GRADS.pack(*_strides2(dy, cu_seqlens is not None), _ptr(dstate), _ptr(dx), _ptr(dw), _ptr(db),
                                  _ptr(dh))
         space, size = _workspace(_lib.lib.fhe_causal_conv_workspace, x, args)
@@ -388,7 +388,7 @@ def causal_conv_step(state, x, weight, bias=None, *, silu: bool = True, slots=No
         raise ValueError("causal_conv_step has no gradient: call it under torch.no_grad()")
     x, weight = _rows(x), weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    y = torch.empty((R, channels), dtype=x.dtype, device=x.device)
+    y = x.new_empty((R, channels))
     args = _CONV_STEP.pack(_DTYPES[x.dtype], R, state.shape[0], channels, taps, _ptr(slots), *_strides2(x, True),
                            _ptr(weight), _ptr(bias), state.data_ptr(), int(silu))
     _run(_lib.lib.fhe_causal_conv_step, x, args, y.data_ptr())
@@ -412,11 +412,11 @@ def _logprob_args(logits, targets, top: int) -> bytes:
 
 def _logprob_forward(logits, targets, top: int):
     rows = logits.shape[0]
-    stats = torch.empty((4, rows), dtype=torch.float32, device=logits.device)
+    stats = logits.new_empty((4, rows), dtype=torch.float32)
     best = index = None
     if top:
-        best = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-        index = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+        best = logits.new_empty((rows, top), dtype=torch.float32)
+        index = logits.new_empty((rows, top), dtype=torch.int32)
     args = _logprob_args(logits, targets, top)
     at = stats.data_ptr()
     out = _LOGPROB_OUT.pack(at, at + 4 * rows, at + 8 * rows, at + 12 * rows, _ptr(best), _ptr(index))
@@ -441,7 +441,7 @@ class _Logprobs(torch.autograd.Function):
         logits, targets, stats = ctx.saved_tensors
         at, rows = stats.data_ptr(), logits.shape[0]  # entropy, peak, log sum
         dlogprob, dentropy = (None if d is None else d.contiguous() for d in (dlogprob, dentropy))
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = logits.new_empty(logits.shape)
         _run(_lib.lib.fhe_token_logprobs_backward, logits, _logprob_args(logits, targets, 0), at + 4 * rows,
              at + 8 * rows, at, _ptr(dlogprob), _ptr(dentropy), _ptr(grad))
         return grad, None, None
