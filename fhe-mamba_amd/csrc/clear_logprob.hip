@@ -31,12 +31,13 @@ struct Stats {
 };
 
 __device__ __forceinline__ Stats join(Stats a, Stats b) {
-  if (b.m > a.m) {
+  if (b.m > a.m || b.m != b.m) {
     const Stats t = a;
     a = b;
     b = t;
   }
-  // a holds the larger maximum (or one of them is NaN, which the sums carry on)
+  // a holds the larger maximum, or NaN if either is: that of entries of which all
+  // others are masked, so that a maximum of -inf says that there is no entry
   const float gap = b.m - a.m;
   if (b.m == -INFINITY && b.s == 0.0f) return a;
   const float f = __builtin_amdgcn_exp2f(gap * LOG2E);
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(THREADS) void k_row_join(RowArgs a) {
     if ((int)threadIdx.x < top) {
       const uint64_t k = lds.best[threadIdx.x];
       const float v = key_value(k);
-      a.o.top_logprob[row_i * top + threadIdx.x] = v == -INFINITY ? -INFINITY : (v - peak) - log_sum;
+      a.o.top_logprob[row_i * top + threadIdx.x] = (v == -INFINITY ? v : v - peak) - log_sum;
       a.o.top_index[row_i * top + threadIdx.x] = k ? (int)key_index(k) : 0;  // a row of NaN may have none
     }
   }

@@ -453,7 +453,7 @@ def token_logprobs(logits, targets, *, top: int = 0) -> TokenLogprobs:
 
     A target below 0 is left out: log probability 0 and no gradient from it; one of vocab or more
     gives NaN.  A logit of -inf is a token that is not allowed; a row of nothing else has log
-    probability -inf, entropy 0 and gradient 0.  logprob and entropy are differentiable in logits."""
+    probability -inf, entropy 0 and gradient 0.  A NaN makes its row NaN.  logprob and entropy are differentiable in logits."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError("logits must be a tensor on the GPU")
     if logits.dtype not in _DTYPES:

@@ -467,9 +467,9 @@ int fhe_causal_conv_step(const fhe_conv_step_args *args, void *y,
  * the logarithm of the sum of exponentials relative to that, and the `top` <=
  * FHE_MAX_TOP likeliest tokens with their log probabilities, the lower index
  * first among equals.  A logit of -infinity is a token that is not allowed; a
- * row of nothing else has log probability -infinity and entropy 0.  targets
- * (NULL: none) below 0 are left out (log probability 0); one of vocab or more
- * gives NaN. */
+ * row of nothing else has log probability -infinity and entropy 0.  A NaN makes
+ * its row's results NaN.  targets (NULL: none) below 0 are left out (log
+ * probability 0); one of vocab or more gives NaN. */
 typedef struct {
   uint32_t dtype, top;
   int64_t rows, vocab, row_stride;
