@@ -45,8 +45,9 @@ _CONV_STEP = struct.Struct("=5I4xQ" + _STRIDED + "3Qi4x")
 _LOGPROB = struct.Struct("=2I3q2Q")
 _LOGPROB_OUT = struct.Struct("=6Q")
 
-
 _F32 = (torch.float32,)
+# of a tensor that a kernel wrote in place: a backward pass that saved it raises, as after torch's own
+_changed = torch.autograd.graph.increment_version
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -258,7 +259,8 @@ def ssm_step(state, x, write, log_decay, B, C, D=None, *, slots=None):
 
     state [cache, heads, head_dim, states] float32 and contiguous, x [requests, heads, head_dim], the
     others alike.  slots [requests] int32 names each request's row (default its own number), no row
-    twice; a slot outside of the cache is padding: its y is zero and no state changes.  Returns y."""
+    twice; a slot outside of the cache is padding: its y is zero and no state changes.  Returns y.
+    A backward pass that needs the state as it was before raises, as after torch's in-place operations."""
     _first("x", x, 3)
     _axes("B", B, 3, "have 3 axes")
     _axes("state", state, 4, "have 4 axes")
@@ -281,6 +283,7 @@ def ssm_step(state, x, write, log_decay, B, C, D=None, *, slots=None):
                       *_strides(B, True), *_strides(C, True), *_strides(write, True), *_strides(log_decay, True),
                       _ptr(D), state.data_ptr())
     _run(_lib.lib.fhe_ssm_step, x, args, y.data_ptr())
+    _changed(state)
     return y
 
 
@@ -392,6 +395,7 @@ def causal_conv_step(state, x, weight, bias=None, *, silu: bool = True, slots=No
     args = _CONV_STEP.pack(_DTYPES[x.dtype], R, state.shape[0], channels, taps, _ptr(slots), *_strides2(x, True),
                            _ptr(weight), _ptr(bias), state.data_ptr(), int(silu))
     _run(_lib.lib.fhe_causal_conv_step, x, args, y.data_ptr())
+    _changed(state)
     return y
 
 
