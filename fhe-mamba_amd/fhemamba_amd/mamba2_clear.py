@@ -160,13 +160,15 @@ class ClearMamba2:
         return clear.token_logprobs(self.logits(hidden), targets, top=top)
 
     def loss(self, ids, *, cu_seqlens=None):
-        """Mean negative log probability of each token's successor; ids [sequences, tokens], or packed."""
+        """Mean negative log probability of each token's successor; ids [sequences, tokens], or packed, where
+        tokens outside of every sequence take no part."""
         hidden, _ = self.forward(self.embedding[ids], cu_seqlens=cu_seqlens)
         targets = torch.cat([ids[..., 1:], torch.full_like(ids[..., :1], -1)], dim=-1)
-        if cu_seqlens is not None:  # no sequence's last token has a successor (nor has what an empty one points to)
-            ends = cu_seqlens[1:].long()
-            last = torch.where(ends > cu_seqlens[:-1], ends - 1, ids.shape[0] - 1)
-            targets = targets.index_fill(0, last, -1)
+        if cu_seqlens is not None:  # neither a sequence's last token nor one outside of all has a successor
+            begins, ends = cu_seqlens[:-1].long(), cu_seqlens[1:].long()
+            at = torch.arange(ids.shape[0], device=ids.device)
+            own = torch.searchsorted(ends, at, right=True).clamp(max=ends.shape[0] - 1)  # the first that ends behind it
+            targets = torch.where((at >= begins[own]) & (at + 1 < ends[own]), targets, -1)
         scored = self.score(hidden, targets).logprob
         return -scored.sum() / (targets >= 0).sum().clamp(min=1)
 
