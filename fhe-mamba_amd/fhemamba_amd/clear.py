@@ -21,6 +21,7 @@ GPU: tokens cu_seqlens[i] .. cu_seqlens[i + 1] are sequence i, which may be empt
 every sequence give zeros.  Nothing crosses from one sequence into another.  A number that is not
 finite makes what depends on it not finite, and may do the same to other tokens of the 64 around it
 in its own sequence.  The gradients' sums have a fixed order: equal inputs give equal bits.
+Gradients are of reverse mode and first order.
 """
 from __future__ import annotations
 
@@ -48,6 +49,7 @@ _LOGPROB_OUT = struct.Struct("=6Q")
 _F32 = (torch.float32,)
 # of a tensor that a kernel wrote in place: a backward pass that saved it raises, as after torch's own
 _changed = torch.autograd.graph.increment_version
+_forward_ad = torch.autograd.forward_ad
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -130,6 +132,10 @@ def _offsets(cu_seqlens, like: torch.Tensor) -> None:
 
 
 def _wants_grad(*tensors) -> bool:
+    if getattr(_forward_ad, "_current_level", 0) >= 0:  # within a level of forward-mode derivatives
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("forward-mode derivatives are not available: a tensor has a tangent")
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
