@@ -115,12 +115,13 @@ def _strides2(t: torch.Tensor, packed: bool) -> tuple:
     return (t.data_ptr(), 0, s[0], 0) if packed else (t.data_ptr(), s[0], s[1], 0)
 
 
-def _workspace(entry, like: torch.Tensor, *args) -> tuple:
+def _workspace(entry, like: torch.Tensor, *args, more: int = 0) -> tuple:
+    """(bytes that the entry point asks for and `more` behind them, how many it asks for)."""
     size = ctypes.c_size_t()
     code = entry(*args, ctypes.byref(size))
     if code:
         _lib.check(code)
-    return like.new_empty(size.value, dtype=torch.uint8), size.value
+    return like.new_empty(size.value + more, dtype=torch.uint8), size.value
 
 
 def _offsets(cu_seqlens, like: torch.Tensor) -> None:
@@ -420,40 +421,45 @@ def _logprob_args(logits, targets, top: int) -> bytes:
                          logits.data_ptr(), _ptr(targets))
 
 
-def _logprob_forward(logits, targets, top: int):
+def _logprob_forward(logits, targets, top: int, keep: bool):
+    """(log probability, entropy, best, index, each a tensor of its own, and with `keep` the peaks and the logs
+    of the sums for the backward pass)."""
     rows = logits.shape[0]
-    stats = logits.new_empty((4, rows), dtype=torch.float32)
-    best = index = None
+    logprob = logits.new_empty(rows, dtype=torch.float32)
+    entropy = logits.new_empty(rows, dtype=torch.float32)
+    best = index = stats = None
     if top:
         best = logits.new_empty((rows, top), dtype=torch.float32)
         index = logits.new_empty((rows, top), dtype=torch.int32)
     args = _logprob_args(logits, targets, top)
-    at = stats.data_ptr()
-    out = _LOGPROB_OUT.pack(at, at + 4 * rows, at + 8 * rows, at + 12 * rows, _ptr(best), _ptr(index))
-    space, size = _workspace(_lib.lib.fhe_token_logprobs_workspace, logits, args)
-    _run(_lib.lib.fhe_token_logprobs, logits, args, out, _ptr(space), size)
-    return stats, best, index
+    space, size = _workspace(_lib.lib.fhe_token_logprobs_workspace, logits, args, more=0 if keep else 8 * rows)
+    if keep:
+        stats = logits.new_empty((2, rows), dtype=torch.float32)
+    at = stats.data_ptr() if keep else space.data_ptr() + size  # a workspace is whole words
+    out = _LOGPROB_OUT.pack(logprob.data_ptr(), entropy.data_ptr(), at, at + 4 * rows, _ptr(best), _ptr(index))
+    _run(_lib.lib.fhe_token_logprobs, logits, args, out, space.data_ptr(), size)
+    return logprob, entropy, best, index, stats
 
 
 class _Logprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top):
-        stats, best, index = _logprob_forward(logits, targets, top)
-        ctx.save_for_backward(logits, targets, stats[1:])
+        logprob, entropy, best, index, stats = _logprob_forward(logits, targets, top, True)
+        ctx.save_for_backward(logits, targets, entropy, stats)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(best, index)
-        return stats[0], stats[1], best, index
+        return logprob, entropy, best, index
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dlogprob, dentropy, *_):
-        logits, targets, stats = ctx.saved_tensors
-        at, rows = stats.data_ptr(), logits.shape[0]  # entropy, peak, log sum
+        logits, targets, entropy, stats = ctx.saved_tensors
+        peak, rows = stats.data_ptr(), logits.shape[0]
         dlogprob, dentropy = (None if d is None else d.contiguous() for d in (dlogprob, dentropy))
         grad = logits.new_empty(logits.shape)
-        _run(_lib.lib.fhe_token_logprobs_backward, logits, _logprob_args(logits, targets, 0), at + 4 * rows,
-             at + 8 * rows, at, _ptr(dlogprob), _ptr(dentropy), _ptr(grad))
+        _run(_lib.lib.fhe_token_logprobs_backward, logits, _logprob_args(logits, targets, 0), peak, peak + 4 * rows,
+             entropy.data_ptr(), _ptr(dlogprob), _ptr(dentropy), _ptr(grad))
         return grad, None, None
 
 
@@ -463,7 +469,8 @@ def token_logprobs(logits, targets, *, top: int = 0) -> TokenLogprobs:
 
     A target below 0 is left out: log probability 0 and no gradient from it; one of vocab or more
     gives NaN.  A logit of -inf is a token that is not allowed; a row of nothing else has log
-    probability -inf, entropy 0 and gradient 0.  A NaN makes its row NaN.  logprob and entropy are differentiable in logits."""
+    probability -inf, entropy 0 and gradient 0.  A NaN makes its row NaN.  logprob and entropy are
+    differentiable in logits; the backward pass needs the entropy as it was."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError("logits must be a tensor on the GPU")
     if logits.dtype not in _DTYPES:
@@ -478,17 +485,18 @@ def token_logprobs(logits, targets, *, top: int = 0) -> TokenLogprobs:
     rows = _rows(logits if flat else logits.reshape(-1, vocab))
     if rows.shape[0] == 0:
         empty = logits.sum(-1).float()
-        return TokenLogprobs(empty, empty, *((empty.new_empty((*lead, top)),
-                                              torch.empty((*lead, top), dtype=torch.int32, device=logits.device))
-                                             if top else (None, None)))
+        best = index = None
+        if top:
+            best = empty.new_empty((*lead, top))
+            index = torch.empty((*lead, top), dtype=torch.int32, device=logits.device)
+        return TokenLogprobs(empty, empty.clone(), best, index)
     if rows.shape[0] > 1 and rows.stride(0) < vocab:  # one row for all
         rows = rows.contiguous()
     targets = (targets if flat else targets.reshape(-1)).contiguous()
     if _wants_grad(logits):
         logprob, entropy, best, index = _Logprobs.apply(rows, targets, top)
     else:
-        stats, best, index = _logprob_forward(rows, targets, top)
-        logprob, entropy = stats[0], stats[1]
+        logprob, entropy, best, index, _ = _logprob_forward(rows, targets, top, False)
     if flat:
         return TokenLogprobs(logprob, entropy, best, index)
     return TokenLogprobs(logprob.reshape(lead), entropy.reshape(lead),
