@@ -118,12 +118,19 @@ def _one_hip_runtime():
 
     A process can use one HIP runtime only: of two the second finds no GPU, or takes the streams and
     memory of the first for its own.  PyTorch's wheels bring theirs under the library's soname and
-    would load it beside the system's; loaded first it serves both, whichever is imported first."""
-    spec = importlib.util.find_spec("torch")
+    would load it beside the system's; loaded first it serves both, whichever is imported first.  Where
+    there is no PyTorch, only a stand-in for it, or a runtime that does not load, the system's serves."""
+    try:
+        spec = importlib.util.find_spec("torch")
+    except (ImportError, ValueError):  # a module without a specification in its place
+        return None
     for folder in (spec.submodule_search_locations or ()) if spec else ():
         path = os.path.join(folder, "lib", "libamdhip64.so")
         if os.path.exists(path):
-            return ctypes.CDLL(path)
+            try:
+                return ctypes.CDLL(path)
+            except OSError:  # PyTorch itself cannot load it either
+                return None
     return None
 
 
