@@ -14,9 +14,12 @@
 // same recurrence in reversed time with B and C, x and dy in each other's
 // place, so the same sweeps give V_t = A_t B_t (dx = w V + D dy, dw = x . V),
 // dB and dC.  With M_ts the part of the loss in source s and target t,
-// dg_r is the sum of M over t >= r > s: what crosses the segment's end,
-// <A, h> there, plus the sums over t >= r of what enters at t less what leaves.
-// Terms with s = t are in neither, and the sums restart every few hundred tokens.
+// dg_r is the sum of M over t >= r > s.  At a place where both states are known it is
+// <A, h>, and from one token to the next it changes by what enters less what leaves;
+// terms with s = t are in neither.  Those are rounded to 32 bits and may be far
+// larger than what is left of them, so the running sums start again every 256 tokens
+// (WINDOW) at the latest, whatever the segments' length, and a token takes the sum
+// from that end of the window from where less was added up.
 //
 // 24 heads of 64 x 128 in 16 bits: a prompt of 1000 tokens takes 13.6 us for the
 // segments' states, 11.8 for carrying them and 12.6 for the results; 30011 packed
@@ -147,10 +150,51 @@ __device__ __forceinline__ void sum_parts(const float* parts, int count, int64_t
   }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
+// What crosses the marks, and the ends of sequences that are not cut: the products of
+// the adjoint and the state that the sweeps left there.  A wavefront a head, four
+// heads a workgroup; it takes both states' bandwidth.
+struct Marks {
+  const float *adjoints, *states;  // the marks
+  const float *dfinal, *last;      // null where sequences are cut or nothing enters at their end
+};
+__global__ __launch_bounds__(256) void k_cross(SweepArgs a, Marks m) {
+  const int across = (a.heads + 3) / 4;
+  const int edge = 1 + (int)(blockIdx.x / across) % a.windows, item_i = (int)(blockIdx.x / across) / a.windows;
+  const int head = (int)(blockIdx.x % across) * 4 + (threadIdx.x >> 6), lane = lane_id();
+  const Item it = find_item(a, item_i);
+  if (!it.live || head >= a.heads) return;
+  const int64_t size = (int64_t)a.head_dim * a.states, all = size * a.heads;
+  const float *A, *h;
+  if (edge < a.windows) {
+    if (edge * WINDOW >= it.count) return;
+    const int64_t mark = mark_of(item_token(a, it), edge * WINDOW);
+    A = m.adjoints + mark * all;
+    h = m.states + mark * all;
+  } else {
+    if (!m.dfinal) return;
+    A = m.dfinal + it.seq * all;
+    h = m.last + it.seq * all;
+  }
+  A += head * size;
+  h += head * size;
+  double sum = 0.0;
+  float squares = 0.0f;
+  auto add = [&](float x, float y) {
+    sum += (double)x * y;
+    squares += x * y * (x * y);
+  };
+  if (size % 4 == 0 && reinterpret_cast<uintptr_t>(A) % 16 == 0) {
+#pragma unroll 8
+    for (int64_t e = 4 * lane; e < size; e += 256) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(A + e), y = *reinterpret_cast<const f32x4*>(h + e);
 #pragma unroll
-  for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
-  return v;
+      for (int r = 0; r < 4; ++r) add(x[r], y[r]);
+    }
+  } else {
+    for (int64_t e = lane; e < size; e += 64) add(A[e], h[e]);
+  }
+  const Crossing c{wave_sum(sum), wave_sum((double)squares)};
+  for (int p = lane; p < a.col_tiles; p += 64) a.crossing(item_i, edge, head)[p] = p ? Crossing{0.0, 0.0} : c;
 }
 
 constexpr int FINISH_THREADS = 256, FINISH_HEADS = FINISH_THREADS / 64, FINISH_STEPS = 4;
@@ -161,91 +205,118 @@ constexpr int FINISH_THREADS = 256, FINISH_HEADS = FINISH_THREADS / 64, FINISH_S
 struct Finish {
   int64_t size;  // of dB and dC
   int parts, items, entering_tiles, group;
+  bool ends;      // whether something crosses a sequence's end
   uint32_t sums;  // workgroups of one of the two
   const float *parts_c, *parts_b;
   void *dc, *db;
-  const int* first;
-  const float *entering, *leaving, *adjoint, *states, *last;
+  const float *entering, *leaving;
   float *dwrite, *ddecay, *dd;
 };
 
-// Gradients of write and log_decay of four heads, a wavefront each, and of up
-// to `group` items of one sequence, by the workgroup of the last of them: the first
-// summed over the head's channels, the second from the items' end backwards.  What
-// crosses that end takes both states' bandwidth, so short items share one end; the
-// sums of a few hundred tokens lose nothing against it.  The results of 64 tokens
-// go through LDS, so that a token's heads are written together.
-__device__ __forceinline__ void gate_grads(const SweepArgs& a, const Finish& f, int item_i, int head0,
+// A value of each lane, in the lanes' reverse order.
+__device__ __forceinline__ double turned(double v) { return __shfl(v, 63 - lane_id()); }
+
+// Gradients of write and log_decay of four heads, a wavefront each, and of a
+// window of up to WINDOW tokens: the first summed over the head's channels, the
+// second the running sums from the window's end backwards and from its beginning.  A
+// window lies in an item that is longer, or it is up to `group` items of one sequence,
+// done by the workgroup of the last of them.  What crosses its ends is known.  The
+// results of 64 tokens go through LDS, so that a token's heads are written together.
+__device__ __forceinline__ void gate_grads(const SweepArgs& a, const Finish& f, int item_i, int window, int head0,
                                            float (&tile)[2][64 * FINISH_STEPS][FINISH_HEADS + 1]) {
+  static_assert(64 * FINISH_STEPS == WINDOW);
   const Item it = find_item(a, item_i);
-  if (it.count <= 0) return;
-  int count = it.count;  // tokens of the group
-  bool last_item = true;
+  const int from = window * WINDOW;
+  if (it.count <= from) return;
+  const bool inside = it.count - from > WINDOW;  // its end is a mark
+  const int end = inside ? from + WINDOW : it.count;  // in the item
+  int count = end - from, before = 0;  // `before` items of the window come before this one
+  bool is_first = true;
   if (a.by_item && it.live) {
-    const int at = a.table ? item_i - f.first[it.seq] : item_i % a.segments;
-    const int items = a.table ? f.first[it.seq + 1] - f.first[it.seq] : a.segments;
-    last_item = at == items - 1;
-    if (!last_item && at % f.group != f.group - 1) return;
-    count += at % f.group * a.length;
+    const int number = a.number(item_i, it.seq);
+    before = number % f.group;
+    is_first = number == before;
+    if (number != a.items_of(it.seq) - 1 && before != f.group - 1) return;
+    count += before * a.length;
   }
   const int lane = lane_id(), wave = threadIdx.x >> 6, head = min(head0 + wave, a.heads - 1);
-  const int64_t token0 = item_token(a, it) + it.count - count;
-  const int64_t size = (int64_t)a.head_dim * a.states, all = size * a.heads;
-  double carry = 0.0;
-  if (f.adjoint && it.live) {
-    const float* A = f.adjoint + (a.by_item ? item_i : it.seq) * all + head * size;
-    const float* h = (last_item ? f.last + it.seq * all : f.states + (item_i + 1) * all) + head * size;
-    if (size % 4 == 0 && reinterpret_cast<uintptr_t>(f.adjoint) % 16 == 0) {
-#pragma unroll 8
-      for (int64_t e = 4 * lane; e < size; e += 256) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(A + e), y = *reinterpret_cast<const f32x4*>(h + e);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) carry += (double)x[r] * y[r];
-      }
-    } else {
-      for (int64_t e = lane; e < size; e += 64) carry += (double)A[e] * h[e];
-    }
-    carry = wave_sum(carry);
-  }
-  for (int end = count; end > 0; end -= 64 * FINISH_STEPS) {
-    double v[FINISH_STEPS] = {};
-    float dw[FINISH_STEPS] = {};
-    const int t0 = end - 1 - lane;  // the last token first, then those 64 before it
+  const int64_t token0 = item_token(a, it) + end - count;
+  // what crosses before the window's first token and behind its last, and its size
+  struct Sum {
+    double v, size;
+  } ahead{0.0, 0.0}, behind{0.0, 0.0};
+  auto crossing = [&](int item, int edge) {
+    Crossing c{0.0, 0.0};
     for (int p = 0; p < a.col_tiles; ++p) {
-      const int64_t at = ((int64_t)head * a.col_tiles + p) * a.all_tokens + token0 + t0;
-#pragma unroll
-      for (int u = 0; u < FINISH_STEPS; ++u)
-        if (t0 >= 64 * u) {
-          v[u] += (double)f.leaving[at - 64 * u];
-          dw[u] += a.dwrite_part[at - 64 * u];
-        }
+      const Crossing x = a.crossing(item, edge, head)[p];
+      c.sum += x.sum;
+      c.squares += x.squares;
     }
-    for (int p = 0; p < f.entering_tiles; ++p) {
-      const int64_t at = ((int64_t)head * f.entering_tiles + p) * a.all_tokens + token0 + t0;
+    return Sum{c.sum, sqrt(c.squares)};
+  };
+  if (it.live) {
+    if (inside) behind = crossing(item_i, window + 1);
+    else if (f.ends) behind = crossing(item_i, a.windows);
+    if (from) ahead = crossing(item_i, window);
+    else if (!is_first) ahead = crossing(item_i - before - 1, a.windows);
+    else if (a.initial) ahead = crossing(item_i - before, 0);
+  }
+  // what enters at a token less what leaves, and both sizes together
+  double v[FINISH_STEPS] = {}, m[FINISH_STEPS] = {};
+  float dw[FINISH_STEPS] = {};
+  const int t0 = count - 1 - lane;  // the last token first, then those 64 before it
+  for (int p = 0; p < a.col_tiles; ++p) {
+    const int64_t at = ((int64_t)head * a.col_tiles + p) * a.all_tokens + token0 + t0;
 #pragma unroll
-      for (int u = 0; u < FINISH_STEPS; ++u)
-        if (t0 >= 64 * u) v[u] += (double)f.entering[at - 64 * u];
-    }
-#pragma unroll
-    for (int u = 0; u < FINISH_STEPS; ++u) v[u] = wave_scan(v[u]);  // four at a time, then what is before each
-#pragma unroll
-    for (int u = 0; u < FINISH_STEPS; ++u) {
-      tile[0][64 * u + lane][wave] = dw[u];
-      tile[1][64 * u + lane][wave] = (float)(v[u] + carry);
-      carry += read_lane(v[u], 63);
-    }
-    __syncthreads();
-    const int col = threadIdx.x % FINISH_HEADS;
-#pragma unroll
-    for (int u = 0; u < FINISH_STEPS; ++u) {
-      const int row = 64 * u + threadIdx.x / FINISH_HEADS;
-      if (row < end && head0 + col < a.heads) {
-        const int64_t at = (token0 + end - 1 - row) * a.heads + head0 + col;
-        f.dwrite[at] = tile[0][row][col];
-        f.ddecay[at] = tile[1][row][col];
+    for (int u = 0; u < FINISH_STEPS; ++u)
+      if (t0 >= 64 * u) {
+        const float g = f.leaving[at - 64 * u];
+        v[u] += (double)g;
+        m[u] += (double)fabsf(g);
+        dw[u] += a.dwrite_part[at - 64 * u];
       }
+  }
+  for (int p = 0; p < f.entering_tiles; ++p) {
+    const int64_t at = ((int64_t)head * f.entering_tiles + p) * a.all_tokens + token0 + t0;
+#pragma unroll
+    for (int u = 0; u < FINISH_STEPS; ++u)
+      if (t0 >= 64 * u) {
+        const float g = f.entering[at - 64 * u];
+        v[u] += (double)g;
+        m[u] += (double)fabsf(g);
+      }
+  }
+  // from the window's beginning: without the token itself, since what crosses there is
+  // the gradient at the first one
+  double fv[FINISH_STEPS], fm[FINISH_STEPS];
+#pragma unroll
+  for (int u = FINISH_STEPS - 1; u >= 0; --u) {
+    const double mine = turned(v[u]), its = turned(m[u]);
+    const double sum = wave_scan(mine), sizes = wave_scan(its);
+    fv[u] = turned(ahead.v - (sum - mine));
+    fm[u] = turned(ahead.size + (sizes - its));
+    ahead.v -= read_lane(sum, 63);
+    ahead.size += read_lane(sizes, 63);
+  }
+#pragma unroll
+  for (int u = 0; u < FINISH_STEPS; ++u) {
+    const double sum = behind.v + wave_scan(v[u]), sizes = behind.size + wave_scan(m[u]);
+    tile[0][64 * u + lane][wave] = dw[u];
+    // where one of the two is not finite, the other
+    tile[1][64 * u + lane][wave] = (float)(sizes <= fm[u] || fm[u] != fm[u] ? sum : fv[u]);
+    behind.v = read_lane(sum, 63);
+    behind.size = read_lane(sizes, 63);
+  }
+  __syncthreads();
+  const int col = threadIdx.x % FINISH_HEADS;
+#pragma unroll
+  for (int u = 0; u < FINISH_STEPS; ++u) {
+    const int row = 64 * u + threadIdx.x / FINISH_HEADS;
+    if (row < count && head0 + col < a.heads) {
+      const int64_t at = (token0 + count - 1 - row) * a.heads + head0 + col;
+      f.dwrite[at] = tile[0][row][col];
+      f.ddecay[at] = tile[1][row][col];
     }
-    __syncthreads();
   }
 }
 
@@ -263,12 +334,13 @@ __device__ __forceinline__ void skip_grad(const SweepArgs& a, const Finish& f, i
 }
 
 template <class T>
-__global__ __launch_bounds__(FINISH_THREADS) void k_finish(SweepArgs a, Finish f) {
+__global__ __launch_bounds__(FINISH_THREADS, 8) void k_finish(SweepArgs a, Finish f) {
   __shared__ float tile[2][64 * FINISH_STEPS][FINISH_HEADS + 1];
   uint32_t block = blockIdx.x;
-  const uint32_t across = (a.heads + FINISH_HEADS - 1) / FINISH_HEADS, gates = (uint32_t)f.items * across;
+  const uint32_t across = (a.heads + FINISH_HEADS - 1) / FINISH_HEADS, gates = (uint32_t)f.items * a.windows * across;
   if (block < gates) {
-    gate_grads(a, f, (int)(block / across), (int)(block % across) * FINISH_HEADS, tile);
+    const uint32_t window = block / across;
+    gate_grads(a, f, (int)(window / a.windows), (int)(window % a.windows), (int)(block % across) * FINISH_HEADS, tile);
     return;
   }
   block -= gates;
@@ -298,9 +370,11 @@ struct Cut {
 struct Plan {
   Cut value, query;
   int length, segments, items;
+  int windows;  // of an item
   bool by_item;
   // workspace, in bytes
-  size_t table, first, decays, states, adjoints, last, dwrite, gate_out, gate_in, dd, parts_c, parts_b, total;
+  size_t table, first, decays, states, adjoints, last, dwrite, gate_out, gate_in, dd, parts_c, parts_b, crossings,
+      mark_states, mark_adjoints, total;
 };
 
 // Tokens of a segment: of all numbers of chunks the one whose estimated time is
@@ -345,6 +419,7 @@ Plan make_plan(const Scan& s, bool backward) {
   p.segments = packed ? 0 : std::max<int>(1, (int)((s.tokens + p.length - 1) / p.length));
   p.by_item = p.length < s.tokens;
   p.items = packed ? (int)(s.tokens / p.length) + s.seqs + 2 : s.seqs * p.segments;
+  p.windows = (p.length + WINDOW - 1) / WINDOW;
   const size_t rows = (size_t)s.heads * p.value.col_tiles;
   auto take = [&](size_t bytes) {
     const size_t at = p.total;
@@ -368,6 +443,11 @@ Plan make_plan(const Scan& s, bool backward) {
     p.dd = take(rows * p.items * 4);
     p.parts_c = take((size_t)p.query.blocks * all * s.groups * s.states * 4);
     p.parts_b = take((size_t)p.query.blocks * all * s.groups * s.states * 4);
+    p.crossings = take(rows * p.items * (p.windows + 1) * sizeof(Crossing));
+    if (p.windows > 1) {
+      p.mark_states = take((all / WINDOW + 1) * state);
+      p.mark_adjoints = take((all / WINDOW + 1) * state);
+    }
   }
   return p;
 }
@@ -493,6 +573,13 @@ void scan_backward(const Scan& s, const ScanGrads& g, void* workspace, hipStream
   x.dwrite_part = sweep.at<float>(p.dwrite);
   x.gate_part = sweep.at<float>(p.gate_out);
   x.dd_part = sweep.at<float>(p.dd);
+  x.windows = p.windows;
+  x.first = sweep.first();
+  x.end_states = states;
+  x.last_states = sweep.at<float>(p.last);
+  x.initial = s.initial;
+  x.crossings = sweep.at<Crossing>(p.crossings);
+  if (p.windows > 1) x.marks = sweep.at<float>(p.mark_adjoints);
 
   SweepArgs c = sweep.with(p.query, s.b, s.c, s.x, g.dy);
   c.state_in = states;
@@ -500,36 +587,41 @@ void scan_backward(const Scan& s, const ScanGrads& g, void* workspace, hipStream
   c.out = sweep.at<float>(p.parts_c);
   c.wide_out = s.states % 4 == 0;
   c.gate_part = sweep.at<float>(p.gate_in);
+  if (p.windows > 1) c.marks = sweep.at<float>(p.mark_states);
 
   SweepArgs b = sweep.with(p.query, s.c, s.b, g.dy, s.x);
   b.state_in = adjoints;
   b.out = sweep.at<float>(p.parts_b);
   b.wide_out = s.states % 4 == 0;
+  const int64_t across = (s.heads + FINISH_HEADS - 1) / FINISH_HEADS, windows = (int64_t)p.items * p.windows;
+  const int64_t sums = (s.all_tokens() * s.groups * s.states + 4 * FINISH_THREADS - 1) / (4 * FINISH_THREADS);
+  const int64_t grid = 2 * sums + windows * across + (g.dd ? across : 0);
+  if (grid > INT32_MAX) throw ArgError("too many tokens and heads for one call");
   launch_backward(s.dtype, c, b, x, p.items, stream);
+  const bool ends = !p.by_item && g.dfinal;
+  if (x.marks || ends) {
+    k_cross<<<(uint32_t)(windows * across), 256, 0, stream>>>(
+        x, Marks{x.marks, c.marks, ends ? g.dfinal : nullptr, sweep.at<float>(p.last)});
+    hip_check(hipGetLastError(), "scan crossings");
+  }
 
   Finish f{};
   f.size = s.all_tokens() * s.groups * s.states;
   f.parts = p.query.blocks;
   f.items = p.items;
   f.entering_tiles = p.query.col_tiles;
-  f.sums = (uint32_t)((f.size + 4 * FINISH_THREADS - 1) / (4 * FINISH_THREADS));
-  f.group = std::max(1, 256 / p.length);
+  f.ends = p.by_item || g.dfinal;
+  f.sums = (uint32_t)sums;
+  f.group = std::max(1, WINDOW / p.length);
   f.parts_c = (const float*)c.out;
   f.parts_b = (const float*)b.out;
   f.dc = g.dc;
   f.db = g.db;
-  f.first = sweep.first();
   f.entering = c.gate_part;
   f.leaving = x.gate_part;
-  f.adjoint = adjoints;
-  f.states = states;
-  f.last = sweep.at<float>(p.last);
   f.dwrite = g.dwrite;
   f.ddecay = g.ddecay;
   f.dd = g.dd;
-  const int64_t across = (s.heads + FINISH_HEADS - 1) / FINISH_HEADS;
-  const int64_t grid = 2 * (int64_t)f.sums + p.items * across + (g.dd ? across : 0);
-  if (grid > INT32_MAX) throw ArgError("too many tokens and heads for one call");
   if (s.dtype == BF16) k_finish<bf16><<<(uint32_t)grid, FINISH_THREADS, 0, stream>>>(x, f);
   else k_finish<float><<<(uint32_t)grid, FINISH_THREADS, 0, stream>>>(x, f);
   hip_check(hipGetLastError(), "scan gradients");

@@ -11,6 +11,16 @@ namespace fhe::clear {
 constexpr int CHUNK = 64, TILES = CHUNK / 16;  // tokens of a chunk, its tiles
 constexpr int WAVES = 4;                       // wavefronts of a workgroup
 constexpr int VALUE_COLS = 32;                 // head channels of a value sweep's wavefront
+// Tokens over which the gates' gradients are one running sum, at most.  Of longer
+// segments the gradient sweeps keep the states at every WINDOW tokens: their marks.
+constexpr int WINDOW = 256;
+
+// What crosses a place between two tokens of a head: the sum of the products of the
+// adjoint and the state there, and that of their squares, by whose root the sum's
+// rounding errors go.
+struct Crossing {
+  double sum, squares;
+};
 
 // Consecutive tokens of one sequence.  `live` is 0 for tokens outside of every
 // sequence, whose results are zeros; such an item has no sequence.
@@ -35,6 +45,22 @@ struct SweepArgs {
   bool by_item;           // states are indexed by item, not by sequence
   void* out;
   float *dwrite_part, *gate_part, *dd_part, *decay_out;
+  float* marks;           // the gradients: states at multiples of WINDOW tokens inside of items, or null
+  // the reverse sweep of x: the states at segments' ends, where those are cut, and what
+  // crosses there
+  int windows;            // of a segment
+  const int* first;       // each sequence's first item where packed
+  const float *end_states, *last_states, *initial;
+  Crossing* crossings;    // [item][its beginning, its marks, its end][head][wavefronts a head]
+
+  // an item's number among its sequence's, and how many those are
+  __device__ __forceinline__ int number(int item, int seq) const {
+    return table ? item - first[seq] : item % segments;
+  }
+  __device__ __forceinline__ int items_of(int seq) const { return table ? first[seq + 1] - first[seq] : segments; }
+  __device__ __forceinline__ Crossing* crossing(int item, int edge, int head) const {
+    return crossings + (((int64_t)item * (windows + 1) + edge) * heads + head) * col_tiles;
+  }
 };
 
 __device__ __forceinline__ Item find_item(const SweepArgs& a, int i) {
@@ -51,6 +77,10 @@ __device__ __forceinline__ int64_t item_at(const SweepArgs& a, const Strided& t,
 __device__ __forceinline__ int64_t item_token(const SweepArgs& a, const Item& it) {
   return (a.table ? 0 : it.seq * a.tokens) + it.start;
 }
+
+// The number of the mark at token `at` of an item, a multiple of WINDOW inside of it.  By
+// the tokens before it: two marks are WINDOW tokens apart or more, so no number comes twice.
+__device__ __forceinline__ int64_t mark_of(int64_t token0, int at) { return (token0 + at) / WINDOW; }
 
 // 2^d, of a 64-bit difference of sums of logarithms: such differences lose
 // nothing to the length of the sums.
@@ -228,6 +258,11 @@ __device__ __forceinline__ float sum16(float v) {
 #undef FHE_ROW_ROR
   return v;
 }
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
+  return v;
+}
 // Sum over the four lane groups, in each lane.
 __device__ __forceinline__ float sum_groups(float v) {
   v += __shfl_xor(v, 16);
@@ -267,13 +302,18 @@ struct Place {
     state_at = ((int64_t)(a.by_item ? item : it.seq) * a.heads + head) * a.head_dim * a.states;
     part = (int64_t)head * a.col_tiles + p0 / a.cols;
   }
+  // of its head in the marks
+  __device__ __forceinline__ int64_t mark_at(const SweepArgs& a, int token) const {
+    return (mark_of(token0, token) * a.heads + head) * a.head_dim * a.states;
+  }
 };
 
 // Whether a sweep's rows are all of whole 16-byte pieces and fill its tiles.
 inline bool is_full(const SweepArgs& a, int nb) {
   for (const Strided& t : {a.key, a.query, a.value, a.other})
     if (t.tok >= (1 << 24)) return false;
-  if (reinterpret_cast<uintptr_t>(a.state_in) % 16 || reinterpret_cast<uintptr_t>(a.state_out) % 16) return false;
+  for (const float* p : {a.state_in, (const float*)a.state_out, a.initial})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
   return a.head_dim % a.cols == 0 && a.states == 32 * nb && a.wide_key && a.wide_query && a.wide_value &&
          a.wide_other && a.wide_out;
 }

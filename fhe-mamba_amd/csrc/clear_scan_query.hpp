@@ -24,8 +24,8 @@ struct QueryLds {
 // [head_dim][states].
 template <int NB, int PT>
 __device__ __forceinline__ void channel_state_io(f32x4 (&h)[PT][2 * NB], const float* from, float* to, int p0,
-                                         int head_dim, int states) {
-  const int q = lane_id() >> 4, l = lane_id() & 15;
+                                         int head_dim, int states, int lane) {
+  const int q = lane >> 4, l = lane & 15;
 #pragma unroll
   for (int p = 0; p < PT; ++p)
 #pragma unroll
@@ -75,7 +75,7 @@ __device__ __forceinline__ void query_sweep(const SweepArgs& a, char* lds_raw, u
 
   f32x4 h[PT][2 * NB] = {};
   if (a.state_in && at.active && it.live)
-    channel_state_io<NB, PT>(h, a.state_in + at.state_at, nullptr, at.p0, a.head_dim, a.states);
+    channel_state_io<NB, PT>(h, a.state_in + at.state_at, nullptr, at.p0, a.head_dim, a.states, lane);
 
   T* vt = lds.value[at.wave];
   Gates& t = lds.gates[at.wave];
@@ -204,9 +204,16 @@ __device__ __forceinline__ void query_sweep(const SweepArgs& a, char* lds_raw, u
         }
       }
     }
+    // the state behind the chunk, where the gates' gradients start again
+    if constexpr (!REV) {
+      const int end = first + CHUNK;
+      if (a.marks && end % WINDOW == 0 && end < it.count && it.live)
+        channel_state_io<NB, PT>(h, nullptr, a.marks + at.mark_at(a, end), at.p0, a.head_dim, a.states,
+                                 lane_here());
+    }
   }
   if (a.state_out && at.active && it.live)
-    channel_state_io<NB, PT>(h, nullptr, a.state_out + at.state_at, at.p0, a.head_dim, a.states);
+    channel_state_io<NB, PT>(h, nullptr, a.state_out + at.state_at, at.p0, a.head_dim, a.states, lane);
 }
 
 }  // namespace

@@ -52,8 +52,8 @@ __device__ __forceinline__ void add_chunk(f32x4 (&h)[2 * NB][PT], const T* key, 
 // [head_dim][states].
 template <int NB, int PT, bool FULL>
 __device__ __forceinline__ void state_io(f32x4 (&h)[2 * NB][PT], const float* from, float* to, int p0,
-                                         int head_dim, int states) {
-  const int q = lane_id() >> 4, l = lane_id() & 15;
+                                         int head_dim, int states, int lane) {
+  const int q = lane >> 4, l = lane & 15;
   const bool wide = FULL || (states % 4 == 0 && reinterpret_cast<uintptr_t>(to ? to : from) % 16 == 0);
 #pragma unroll
   for (int p = 0; p < PT; ++p) {
@@ -68,6 +68,32 @@ __device__ __forceinline__ void state_io(f32x4 (&h)[2 * NB][PT], const float* fr
       else h[nt][p] = load4(from + at, left, wide);
     }
   }
+}
+
+// The products of a state's tiles and those of another at `with`.
+template <int NB, int PT, bool FULL>
+__device__ __forceinline__ Crossing state_dot(const f32x4 (&h)[2 * NB][PT], const float* with, int p0, int head_dim,
+                                              int states, int lane) {
+  const int q = lane >> 4, l = lane & 15;
+  const bool wide = FULL || (states % 4 == 0 && reinterpret_cast<uintptr_t>(with) % 16 == 0);
+  double sum = 0.0;
+  float squares = 0.0f;
+#pragma unroll
+  for (int p = 0; p < PT; ++p) {
+    const int row = p0 + 16 * p + l;
+    if (!FULL && row >= head_dim) continue;
+#pragma unroll
+    for (int nt = 0; nt < 2 * NB; ++nt) {
+      const int n = 16 * nt + 4 * q;
+      const f32x4 o = load4(with + (int64_t)row * states + n, FULL ? 4 : states - n, wide);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sum += (double)h[nt][p][r] * o[r];
+        squares += h[nt][p][r] * o[r] * (h[nt][p][r] * o[r]);
+      }
+    }
+  }
+  return {wave_sum(sum), wave_sum((double)squares)};
 }
 
 // In reverse a wavefront holds nearly all the registers there are, and step_end()
@@ -108,14 +134,33 @@ __device__ __forceinline__ void value_sweep(const SweepArgs& a, char* lds_raw, u
 
   f32x4 h[2 * NB][PT] = {};
   if (VALUES && a.state_in && at.active && it.live)
-    state_io<NB, PT, FULL>(h, a.state_in + at.state_at, nullptr, at.p0, a.head_dim, a.states);
+    state_io<NB, PT, FULL>(h, a.state_in + at.state_at, nullptr, at.p0, a.head_dim, a.states, lane);
 
   T* vt = lds.value[at.wave];
   Gates& t = lds.gates[at.wave];
   float dd = 0.0f;
   double log_total = 0.0;
   const int chunks = (it.count + CHUNK - 1) / CHUNK;
-  for (int c = 0; c < chunks; ++c) {
+  for (int c = 0; c < chunks || (VALUES && REV); ++c) {
+    if constexpr (VALUES && REV) {
+      // what crosses a cut segment's end and a sequence's beginning, whose states are known
+      if (at.active && it.live && (c == 0 || c == chunks)) {
+        const float* with = nullptr;
+        const int number = a.by_item ? a.number(at.item, it.seq) : 0;
+        const int64_t all = (int64_t)a.heads * a.head_dim * a.states;
+        if (c == chunks) with = number == 0 && a.initial ? a.initial + it.seq * all : nullptr;
+        else if (a.by_item && number == a.items_of(it.seq) - 1) with = a.last_states + it.seq * all;
+        else if (a.by_item) with = a.end_states + (at.item + 1) * all;
+        if (with) {
+          step_end();
+          const Crossing x = state_dot<NB, PT, FULL>(h, with + (int64_t)at.head * a.head_dim * a.states, at.p0,
+                                                     a.head_dim, a.states, lane_here());
+          if (lane == 0) a.crossing(at.item, c == chunks ? 0 : a.windows, at.head)[at.p0 / a.cols] = x;
+          step_end();
+        }
+      }
+      if (c == chunks) break;
+    }
     const int first = (REV ? chunks - 1 - c : c) * CHUNK;
     const int n = min(CHUNK, it.count - first), live = it.live ? n : 0;
     {
@@ -265,10 +310,15 @@ __device__ __forceinline__ void value_sweep(const SweepArgs& a, char* lds_raw, u
       log_total += t.ends[TILES];
     }
     add_chunk<T, NB, PT, REV>(h, lds.key, vt, t, n);
+    // the adjoint behind the tokens before the chunk, where the gates' gradients start again
+    if constexpr (VALUES && REV) {
+      if (a.marks && first % WINDOW == 0 && first > 0 && it.live)
+        state_io<NB, PT, FULL>(h, nullptr, a.marks + at.mark_at(a, first), at.p0, a.head_dim, a.states, lane_here());
+    }
   }
   if (!at.active) return;
   if (a.state_out && (a.by_item || it.live))
-    state_io<NB, PT, FULL>(h, nullptr, a.state_out + at.state_at, at.p0, a.head_dim, a.states);
+    state_io<NB, PT, FULL>(h, nullptr, a.state_out + at.state_at, at.p0, a.head_dim, a.states, lane);
   if constexpr (!VALUES) {
     if (lane == 0 && at.p0 == 0) a.decay_out[(int64_t)at.item * a.heads + at.head] = exp2d(log_total);
   }

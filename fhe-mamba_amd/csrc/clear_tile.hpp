@@ -39,6 +39,14 @@ __device__ __forceinline__ void step_end() { __builtin_amdgcn_sched_barrier(0); 
 
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 
+// The lane's number, of which the compiler knows nothing: what is computed from it
+// is computed there, and not kept in registers through a loop around it.
+__device__ __forceinline__ int lane_here() {
+  int lane = lane_id();
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 template <class T>
 struct Num;
 
