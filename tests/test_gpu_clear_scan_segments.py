@@ -24,6 +24,8 @@ PLANS = {
     "packed_odd": (LONG, True, (64, 10, 7, 2), 257, 512),
     "one_item_a_gate_group": (SHORT, True, (48, 64, 32, 1), 192, 192),
     "two_items_a_gate_group": (SHORT, True, (64, 32, 32, 1), 128, 128),
+    # a sequence or two in each item's length, as prompts of a serving batch
+    "many_short": ([(37 * i) % 101 for i in range(240)], True, (8, 32, 32, 1), 64, 128),
     "whole": ([2048] * 32, False, (64, 8, 8, 1), 0, 0),
     "whole_odd": ([777] * 60, False, (60, 10, 7, 3), 0, 0),
 }
