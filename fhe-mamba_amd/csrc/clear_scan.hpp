@@ -16,8 +16,8 @@ constexpr int VALUE_COLS = 32;                 // head channels of a value sweep
 constexpr int WINDOW = 256;
 
 // What crosses a place between two tokens of a head: the sum of the products of the
-// adjoint and the state there, and that of their squares, by whose root the sum's
-// rounding errors go.
+// adjoint and the state there, and that of their squares, by which the sum's rounding
+// errors go.
 struct Crossing {
   double sum, squares;
 };
