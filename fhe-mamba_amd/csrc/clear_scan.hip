@@ -24,15 +24,18 @@
 // 48, 40 states and 1777 tokens in 32 bits is 2.2e-7 off so, by the terms' sizes 2.8e-7,
 // always from the end 2.2e-7 and, with two texts of 3000 tokens, 3.4e-7 for 2.5e-7.
 //
-// 24 heads of 64 x 128 in 16 bits: a prompt of 1000 tokens takes 13.6 us for the
-// segments' states, 11.8 for carrying them and 12.6 for the results; 30011 packed
-// tokens 62 + 22 + 147; 4 x 2048
-// tokens 26 + 9 + 48, and their gradients 34 + 16 + 188 and 22 for the last sums.
-// The sweeps read and write a fifth of what memory would pass in that time and are
-// bound by a wavefront's own work: of its cycles the vector instructions (splits
-// into 16-bit pieces, decays, pairs) take two fifths, the matrix products a quarter,
-// waits for LDS and loads the most of the rest, with the two wavefronts a SIMD that
-// the states' registers leave.
+// 24 heads of 64 x 128 in 16 bits: a prompt of 1000 tokens takes 13.9 us for the
+// segments' states, 11.6 for carrying them and 12.5 for the results; 30011 packed
+// tokens 62 + 23 + 148; 4 x 2048 tokens 26 + 9 + 48, and their gradients 35 + 16 +
+// 192 and 15 for the last sums.  In 32 bits 1000 tokens take 16 + 11 + 33, 4 x 2048
+// tokens 52 + 9 + 190 and their gradients 79 + 16 + 513 + 18.  32 x 2048 tokens stay
+// whole: 328 us in 16 bits, their gradients 1453, 76 for the marks' products and 95 for
+// the sums.
+// The sweeps read and write a fifth of what memory would pass in that time, and no
+// unit is full either: of a CU's 252 thousand cycles in the results of 30011 tokens
+// the vector units work 119 (splits into 16-bit pieces, decays, pairs) and the matrix
+// units 79.  What is left are the waits of a wavefront's chain of products, which the
+// two wavefronts a SIMD that the states' registers leave do not cover.
 #pragma clang fp contract(fast)
 #include "clear_scan.hpp"
 
@@ -382,7 +385,11 @@ struct Plan {
 // least.  Workgroups run in rounds of two a CU, a round as long as a segment; a
 // chunk of a round takes about 14 us in the sweeps for the states and the results
 // together, and a segment's states are written once and read and written once
-// more, at 6.6 TB/s.  A whole sequence's state stays in registers.  us of the
+// more, at 6.6 TB/s.  A whole sequence's state stays in registers.  The times are
+// those of 24 heads of 64 x 128 in 16 bits and are taken for every type and size:
+// 32-bit products are slower and few states quicker, and other lengths than these may
+// be best there.  Packed sequences' lengths are not known on the host, so a batch of
+// them is planned as one, and is cut also where each would fit a segment.  us of the
 // launches forward, at lengths of 4 / 6 / 8 / 12 / 16 chunks of 30011 packed tokens of
 // 24 heads of 64 x 128: 269 / 258 / 256 / 301 / 267; at 2 / 4 / 5 chunks of 4 x 2048:
 // 89 / 84 / 92, and their gradients 281 / 265 / 268.

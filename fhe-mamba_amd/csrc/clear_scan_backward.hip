@@ -1,7 +1,7 @@
 // The three sweeps of the scan's gradients in one launch: those of C forward,
 // those of B and of x in reverse.  None needs another's results, and together
-// they leave fewer places of the chip empty than one after the other: 188 us at
-// 4 x 2048 tokens of 24 heads of 64 x 128 in 16 bits, apart 73 for x and about 140
+// they leave fewer places of the chip empty than one after the other: 192 us at
+// 4 x 2048 tokens of 24 heads of 64 x 128 in 16 bits, apart about 75 for x and 140
 // for the two others.
 #include "clear_scan_query.hpp"
 #include "clear_scan_value.hpp"

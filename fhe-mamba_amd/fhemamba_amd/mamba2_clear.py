@@ -1,8 +1,9 @@
 """A chain payload's Mamba-2 model in the clear on the GPU.
 
-The encrypted decode starts from a state; a client that holds the prompt makes that state here, with
-the whole prompt in one call, and whoever fits the polynomials or tunes the weights to them runs and
-differentiates the same model.  The layer is mamba2_payload.layer_step with exact functions
+A client that holds the prompt runs the model on it here, the whole prompt in one call, and whoever
+fits the polynomials or tunes the weights to them runs and differentiates the same model.  The states
+that it leaves start the plain decode (mamba2_payload.decode_tokens); the encrypted decode starts from
+empty ones.  The layer is mamba2_payload.layer_step with exact functions
 (src/fhemamba/reference.py:182-339): RMSNorm, in_proj, causal convolution and SiLU, the selective scan,
 the gate and its norm, out_proj, the residual; the norms and projections are torch's, the rest
 clear.py's kernels.
@@ -174,7 +175,7 @@ class ClearMamba2:
 
 
 def layer_states(states, row: int = 0) -> list:
-    """One row of the states as mamba2_payload.LayerState, the start of a plain or encrypted decode."""
+    """One row of the states as mamba2_payload.LayerState, the start of a plain decode."""
     return [LayerState(s.ssm[row].double().cpu().numpy(), list(s.conv[row].double().cpu().numpy())) for s in states]
 
 
