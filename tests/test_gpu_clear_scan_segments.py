@@ -27,6 +27,7 @@ PLANS = {
     # a sequence or two in each item's length, as prompts of a serving batch
     "many_short": ([(37 * i) % 101 for i in range(240)], True, (8, 32, 32, 1), 64, 128),
     "whole": ([2048] * 32, False, (64, 8, 8, 1), 0, 0),
+    "packed_whole": ([1300], True, (4096, 4, 4, 1), 0, 0),
     "whole_odd": ([777] * 60, False, (60, 10, 7, 3), 0, 0),
 }
 
@@ -96,3 +97,40 @@ def test_how_far_a_nan_reaches(name, dtype):
             bad[1, :, 2] = False
             assert not bool(bad.any()), (k, late)
         assert bool(torch.isnan(got["log_decay"]).any())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_long_stretches_outside_of_every_sequence(dtype):
+    """700 tokens before the first sequence and 900 behind the last, all NaN: zeros, and the sequences as without."""
+    from fhemamba_amd import clear
+
+    lengths, (H, P, N, G), before, behind = [2900, 0, 1, 3502], (36, 64, 32, 1), 700, 900
+    inside = sum(lengths)
+    total = before + inside + behind
+    found = B.segment_lengths([before, *lengths, behind], True, (H, P, N, G), dtype)
+    assert found and min(found) > 256  # segments of several windows
+    d = T.make(9, inside, H, P, N, G, dtype, seqs=4, gate=0.02)
+    gen = torch.Generator().manual_seed(1)
+    grads = T.normal(gen, inside, H, P, dtype=dtype), T.normal(gen, 4, H, P, N)
+    leaves = {}
+    for k in T.NAMES:
+        t = d[k]
+        if k != "D":
+            t = torch.full((total, *t.shape[1:]), math.nan, dtype=t.dtype)
+            t[before:before + inside] = d[k]
+        leaves[k] = t.cuda().requires_grad_(True)
+    leaves["initial"] = d["initial"].cuda().requires_grad_(True)
+    cu = before + torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32)
+    y, h = clear.ssm_scan(*(leaves[k] for k in T.NAMES), initial_state=leaves["initial"], cu_seqlens=cu.cuda(),
+                          return_state=True)
+    dy = torch.full((total, H, P), math.nan, dtype=dtype)
+    dy[before:before + inside] = grads[0]
+    got = dict(zip(leaves, torch.autograd.grad([y, h], list(leaves.values()), [dy.cuda(), grads[1].cuda()])))
+    y0, h0, want = B.scan(d, lengths, grads)
+    assert B.rel(y[before:before + inside], y0) <= R.bound(y) and B.rel(h, h0) <= R.F32
+    assert bool((y[:before] == 0).all()) and bool((y[before + inside:] == 0).all())
+    for k in got:
+        gates = R.GATES if dtype == BF and k in ("write", "log_decay") else R.bound(got[k])
+        own = k in ("D", "initial")
+        assert B.rel(got[k] if own else got[k][before:before + inside], want[k]) <= gates, k
+        assert own or bool((got[k][:before] == 0).all()) and bool((got[k][before + inside:] == 0).all()), k
