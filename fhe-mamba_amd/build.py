@@ -32,7 +32,8 @@ CFLAGS = [
 SOURCES = ["moddown.hip", "ntt.hip", "convert.hip", "rescale.hip", "small_ring.hip",
            "poly_ops.hip", "keyswitch.hip", "encode.hip", "keygen.hip", "clear_scan.hip",
            "clear_scan_forward.hip", "clear_scan_backward.hip", "clear_step.hip", "clear_conv.hip",
-           "clear_logprob.hip", "context.cpp", "capi.cpp", "clear_capi.cpp"]
+           "clear_logprob.hip", "clear_norm.hip", "clear_int8.hip", "clear_embed.hip",
+           "clear_beam.hip", "context.cpp", "capi.cpp", "clear_capi.cpp"]
 
 
 def _compile(src: str) -> tuple[str, int, str]:

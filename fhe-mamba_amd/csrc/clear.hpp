@@ -107,6 +107,103 @@ void logprob(const Logprob& l, const LogprobOut& o, void* workspace, hipStream_t
 void logprob_backward(const Logprob& l, const float* peak, const float* log_sum, const float* entropy,
                       const float* dlogprob, const float* dentropy, void* dlogits, hipStream_t stream);
 
+// Rows of contiguous elements, `row` elements apart.
+struct Rows {
+  const void* p;
+  int64_t row;
+};
+
+struct Norm {
+  uint32_t dtype, out_dtype;  // of x and the gate; of y
+  int64_t rows;
+  int channels, groups;  // of a row
+  float eps;
+  Rows x, gate;  // gate.p may be null
+  const float* weight;
+};
+struct NormGrads {
+  Rows dy;
+  void *dx, *dgate;
+  float* dweight;
+};
+size_t norm_workspace(const Norm& n);
+void norm(const Norm& n, void* y, hipStream_t stream);
+void norm_backward(const Norm& n, const NormGrads& g, void* workspace, hipStream_t stream);
+
+struct AddNorm {
+  uint32_t dtype, out_dtype;  // of hidden and the sum; of the update and y
+  int64_t rows;
+  int channels;
+  float eps;
+  Rows hidden, update;
+  const float *scale, *weight;  // scale may be null
+};
+struct AddNormGrads {
+  Rows dy, dsum;    // either may be null
+  const void* sum;  // as the forward call left it, or null
+  void *dhidden, *dupdate;
+  float *dscale, *dweight;
+};
+size_t add_norm_workspace(const AddNorm& n);
+void add_norm(const AddNorm& n, void* sum, void* y, hipStream_t stream);
+void add_norm_backward(const AddNorm& n, const AddNormGrads& g, void* workspace, hipStream_t stream);
+
+struct Quantize {
+  uint32_t dtype;
+  int64_t rows;
+  int channels;
+  Rows x;
+};
+// values [rows][channels], scale [rows]
+void quantize_rows(const Quantize& z, int8_t* values, float* scale, hipStream_t stream);
+
+struct Int8 {
+  uint32_t dtype;
+  int64_t rows;
+  int inputs, outputs;
+  Rows x;
+  const int8_t* weight;  // [outputs][inputs]
+  const float *scale, *bias;  // [outputs]; bias may be null
+};
+size_t int8_workspace(const Int8& p);
+void int8_linear(const Int8& p, void* y, void* workspace, hipStream_t stream);
+
+struct Embed {
+  uint32_t dtype;
+  int64_t tokens, vocab;
+  int channels;
+  const void* weight;
+  int64_t weight_row;
+  const int64_t* ids;
+  float scale;
+};
+size_t embed_workspace(const Embed& e);
+void embed(const Embed& e, void* y, hipStream_t stream);
+void embed_backward(const Embed& e, const Rows& dy, void* dweight, void* workspace, hipStream_t stream);
+
+struct Beam {
+  uint32_t dtype;
+  int requests, beams, width;
+  int64_t vocab, row_stride, end;
+  const void* logits;       // [requests * beams][vocab]
+  const float* scores;      // [requests][beams]
+  const uint8_t* finished;  // or null
+};
+struct BeamOut {
+  float* score;  // [requests][width]
+  int *parent, *token;
+};
+size_t beam_workspace(const Beam& b);
+void beam_select(const Beam& b, const BeamOut& o, void* workspace, hipStream_t stream);
+
+struct Moved {
+  void* state;  // [cache][row_bytes]
+  int64_t row_bytes;
+};
+// state[slot of beam j] <- state[slot of beam parent[j]] in place, for each request
+void reorder_states(const Moved* states, int count, int requests, int beams, int cache, const int* parent,
+                    const int* slots, hipStream_t stream);
+
 constexpr int MAX_STATES = 128, MAX_TAPS = 8, MAX_TOP = 32;
 
 }  // namespace fhe::clear

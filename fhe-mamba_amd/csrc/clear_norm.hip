@@ -1,0 +1,367 @@
+// Root mean square norms fused with what stands before them in a layer, and
+// their gradients:
+//   v = x, x silu(z) or h + s u;   r = (mean v^2 + eps)^(-1/2);   n = v r w
+//   g = dn w,   dv = r g - v r^3 mean(g v) (+ the gradient of h + s u itself)
+//   dx = dv silu(z),  dz = dv x silu'(z);   dh = dv,  du = s dv
+//   dw = sum over rows of dn v r,   ds = sum over rows of dv u
+// A row is held in registers by one wavefront, four or sixteen, so that each
+// input is read once, and v and r are computed again in the gradient instead of
+// being kept.  Bound by memory.  The sums over rows stay in registers over the
+// rows that a wavefront walks, and a second kernel adds what the workgroups
+// leave, in a fixed order.
+#pragma clang fp contract(fast)
+#include <algorithm>
+
+#include "clear.hpp"
+#include "clear_rows.hpp"
+#include "context.hpp"
+
+namespace fhe::clear {
+namespace {
+
+enum Mode { PLAIN, GATED, ADDED, SUMMED };  // v: a, a silu(b), a + scale b, a itself but with ADDED's gradients
+
+struct NormArgs {
+  const void *a, *b;        // x or h; z or u
+  int64_t a_row, b_row;     // elements between rows
+  const float *scale, *weight;
+  void *sum, *y;            // forward; contiguous
+  const void *dy, *dsum;    // backward
+  int64_t dy_row, dsum_row;
+  void *da, *db;            // contiguous
+  float* parts;             // [1 or 2][workgroups][all channels]: of the weight's gradient, of the scale's
+  int64_t rows;
+  int channels, all;        // of a group; of a row
+  float eps;
+};
+
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
+
+// The sums of W wavefronts' lanes; `lds` is free again after the next call's barrier.
+template <int W, int COUNT>
+__device__ __forceinline__ void row_sums(float (&s)[COUNT], float (*lds)[2][COUNT], int turn) {
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) s[i] = wave_sum(s[i]);
+  if constexpr (W > 1) {
+    const int wave = threadIdx.x >> 6;
+    if (lane_id() == 0) {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) lds[wave][turn][i] = s[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      s[i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) s[i] += lds[w][turn][i];
+    }
+  }
+}
+
+// W wavefronts a row, PER pieces of four channels a lane; FULL: they are all of
+// the row.  blockIdx.y is the group.
+template <class A, class O, int MODE, int W, int PER, bool FULL>
+__global__ __launch_bounds__(threads_of(W)) void k_norm(NormArgs p) {
+  using B = std::conditional_t<MODE == ADDED, O, A>;
+  constexpr int LANES = 64 * W, ROWS = threads_of(W) / LANES;
+  __shared__ float lds[W][2][1];
+  const int lane = threadIdx.x % LANES;
+  const int64_t first = (int64_t)blockIdx.y * p.channels;
+  const float mean = 1.0f / (float)p.channels;
+  int count[PER];
+  f32x4 w[PER], scale[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int c = (k * LANES + lane) * 4;
+    count[k] = FULL ? 4 : p.channels - c;
+    w[k] = get4(p.weight + first + c, count[k]);
+    if constexpr (MODE == ADDED) scale[k] = p.scale ? get4(p.scale + first + c, count[k]) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+  }
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < p.rows;
+       row += (int64_t)gridDim.x * ROWS) {
+    const A* a = (const A*)p.a + row * p.a_row + first;
+    const B* b = (const B*)p.b + (MODE == PLAIN ? 0 : row * p.b_row + first);
+    f32x4 v[PER], other[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int c = (k * LANES + lane) * 4;
+      v[k] = get4(a + c, count[k]);
+      if constexpr (MODE != PLAIN) other[k] = get4(b + c, count[k]);
+    }
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if constexpr (MODE == ADDED) {
+        v[k] += scale[k] * other[k];
+        put4((A*)p.sum + row * p.all + first + (k * LANES + lane) * 4, v[k], count[k]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (MODE == GATED) v[k][i] *= other[k][i] * sigmoid(other[k][i]);
+        s[0] += v[k][i] * v[k][i];
+      }
+    }
+    row_sums<W>(s, lds, turn ^= 1);
+    const float r = rsqrtf(s[0] * mean + p.eps);
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      put4((O*)p.y + row * p.all + first + (k * LANES + lane) * 4, v[k] * r * w[k], count[k]);
+  }
+}
+
+template <class A, class O, int MODE, int W, int PER, bool FULL>
+__global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
+  using B = std::conditional_t<MODE == ADDED || MODE == SUMMED, O, A>;
+  constexpr int LANES = 64 * W, ROWS = threads_of(W) / LANES;
+  __shared__ float lds[W][2][2];
+  __shared__ float totals[W == 1 ? ROWS - 1 : 1][W == 1 ? PER * 256 : 1];
+  const int lane = threadIdx.x % LANES;
+  const int64_t first = (int64_t)blockIdx.y * p.channels;
+  const float mean = 1.0f / (float)p.channels;
+  int count[PER];
+  f32x4 w[PER], scale[PER], dw[PER], ds[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int c = (k * LANES + lane) * 4;
+    count[k] = FULL ? 4 : p.channels - c;
+    w[k] = get4(p.weight + first + c, count[k]);
+    if constexpr (MODE == ADDED) scale[k] = p.scale ? get4(p.scale + first + c, count[k]) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+    dw[k] = ds[k] = f32x4{};
+  }
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < p.rows;
+       row += (int64_t)gridDim.x * ROWS) {
+    const A* a = (const A*)p.a + row * p.a_row + first;
+    const B* b = (const B*)p.b + (MODE == GATED || MODE == ADDED ? row * p.b_row + first : 0);
+    const O* dy = (const O*)p.dy + row * p.dy_row + first;
+    f32x4 v[PER], other[PER], g[PER], act[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int c = (k * LANES + lane) * 4;
+      v[k] = get4(a + c, count[k]);
+      if constexpr (MODE == GATED || MODE == ADDED) other[k] = get4(b + c, count[k]);
+      g[k] = p.dy ? get4(dy + c, count[k]) : f32x4{};
+    }
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if constexpr (MODE == ADDED) v[k] += scale[k] * other[k];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float t = v[k][i];
+        if constexpr (MODE == GATED) {
+          act[k][i] = other[k][i] * sigmoid(other[k][i]);
+          t *= act[k][i];
+        }
+        s[0] += t * t;
+        s[1] += t * g[k][i] * w[k][i];
+      }
+    }
+    row_sums<W>(s, lds, turn ^= 1);
+    const float r = rsqrtf(s[0] * mean + p.eps);
+    const float back = r * r * r * (s[1] * mean);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int c = (k * LANES + lane) * 4;
+      const int64_t at = row * p.all + first + c;
+      f32x4 t = v[k];
+      if constexpr (MODE == GATED) t *= act[k];
+      f32x4 d = r * (g[k] * w[k]) - t * back;
+      dw[k] += g[k] * (t * r);
+      if constexpr (MODE == PLAIN) {
+        put4((A*)p.da + at, d, count[k]);
+      } else if constexpr (MODE == GATED) {
+        put4((A*)p.da + at, d * act[k], count[k]);
+        f32x4 dz;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float sig = sigmoid(other[k][i]);
+          dz[i] = d[i] * v[k][i] * (sig + act[k][i] * (1.0f - sig));
+        }
+        put4((A*)p.db + at, dz, count[k]);
+      } else {
+        if (p.dsum) d += get4((const A*)p.dsum + row * p.dsum_row + first + c, count[k]);
+        if (p.da) put4((A*)p.da + at, d, count[k]);
+        if constexpr (MODE == ADDED) {
+          ds[k] += d * other[k];
+          d *= scale[k];
+        }
+        if (p.db) put4((B*)p.db + at, d, count[k]);
+      }
+    }
+  }
+  // what the workgroup's rows add up to
+  auto total = [&](f32x4(&t)[PER], float* out) {
+    out += (int64_t)blockIdx.x * p.all + first;
+    if constexpr (W == 1) {
+      const int wave = threadIdx.x >> 6;
+      __syncthreads();
+      if (wave) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) *reinterpret_cast<f32x4*>(&totals[wave - 1][(k * 64 + lane) * 4]) = t[k];
+      }
+      __syncthreads();
+      if (wave) return;
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+#pragma unroll
+        for (int o = 0; o < ROWS - 1; ++o) t[k] += *reinterpret_cast<const f32x4*>(&totals[o][(k * 64 + lane) * 4]);
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) put4(out + (k * LANES + lane) * 4, t[k], count[k]);
+  };
+  total(dw, p.parts);
+  if constexpr (MODE == ADDED) {
+    if (p.scale) total(ds, p.parts + (int64_t)gridDim.x * p.all);
+  }
+}
+
+// out[c] = the sum over workgroups of parts[.][c]; blockIdx.y: of which of the outputs.
+__global__ __launch_bounds__(1024) void k_norm_sum(const float* parts, int count, int all, float* out0, float* out1) {
+  __shared__ float lds[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
+  parts += (int64_t)blockIdx.y * count * all;
+  float s = 0.0f;
+  if (c < all)
+    for (int i = lane; i < count; i += 16) s += parts[(int64_t)i * all + c];
+  lds[lane][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (lane || c >= all) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += lds[i][threadIdx.x];
+  float* out = blockIdx.y ? out1 : out0;
+  if (out) out[c] = s;
+}
+
+template <class F>
+void by_type(uint32_t dtype, uint32_t out, F&& f) {
+  if (dtype == F32 && out == F32) f(float{}, float{});
+  else if (dtype == F32) f(float{}, bf16{});
+  else f(bf16{}, bf16{});
+}
+
+int forward_grid(int64_t rows, int channels) {
+  const int at = rows_at_once(channels);
+  return (int)std::min<int64_t>((rows + at - 1) / at, 1 << 16);
+}
+
+// Workgroups of the gradient: two a CU, or four of the smaller.
+int backward_grid(int64_t rows, int channels) {
+  const int at = rows_at_once(channels);
+  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + at - 1) / at, 1024));
+}
+
+template <int MODE>
+void forward(const NormArgs& p, uint32_t dtype, uint32_t out, int groups, hipStream_t stream) {
+  if (!p.rows) return;
+  const dim3 grid(forward_grid(p.rows, p.channels), groups);
+  by_type(dtype, out, [&](auto a, auto o) {
+    by_shape(p.channels, [&](auto w, auto per, auto full) {
+      k_norm<decltype(a), decltype(o), MODE, w(), per(), full()><<<grid, threads_of(w()), 0, stream>>>(p);
+    });
+  });
+  hip_check(hipGetLastError(), "norm");
+}
+
+template <int MODE>
+void backward(const NormArgs& p, uint32_t dtype, uint32_t out, int groups, float* dweight, float* dscale,
+              hipStream_t stream) {
+  const int count = backward_grid(p.rows, p.channels);
+  by_type(dtype, out, [&](auto a, auto o) {
+    by_shape(p.channels, [&](auto w, auto per, auto full) {
+      k_norm_back<decltype(a), decltype(o), MODE, w(), per(), full()>
+          <<<dim3(count, groups), threads_of(w()), 0, stream>>>(p);
+    });
+  });
+  hip_check(hipGetLastError(), "norm gradient");
+  k_norm_sum<<<dim3((p.all + 63) / 64, p.scale ? 2 : 1), 1024, 0, stream>>>(p.parts, count, p.all, dweight, dscale);
+  hip_check(hipGetLastError(), "norm gradient sums");
+}
+
+NormArgs args_of(const Norm& n) {
+  NormArgs p{};
+  p.a = n.x.p;
+  p.a_row = n.x.row;
+  p.b = n.gate.p;
+  p.b_row = n.gate.row;
+  p.weight = n.weight;
+  p.rows = n.rows;
+  p.all = n.channels;
+  p.channels = n.channels / n.groups;
+  p.eps = n.eps;
+  return p;
+}
+
+NormArgs args_of(const AddNorm& n) {
+  NormArgs p{};
+  p.a = n.hidden.p;
+  p.a_row = n.hidden.row;
+  p.b = n.update.p;
+  p.b_row = n.update.row;
+  p.scale = n.scale;
+  p.weight = n.weight;
+  p.rows = n.rows;
+  p.all = p.channels = n.channels;
+  p.eps = n.eps;
+  return p;
+}
+
+}  // namespace
+
+size_t norm_workspace(const Norm& n) {
+  return (size_t)backward_grid(n.rows, n.channels / n.groups) * n.channels * sizeof(float);
+}
+
+void norm(const Norm& n, void* y, hipStream_t stream) {
+  NormArgs p = args_of(n);
+  p.y = y;
+  if (n.gate.p) forward<GATED>(p, n.dtype, n.out_dtype, n.groups, stream);
+  else forward<PLAIN>(p, n.dtype, n.out_dtype, n.groups, stream);
+}
+
+void norm_backward(const Norm& n, const NormGrads& g, void* workspace, hipStream_t stream) {
+  NormArgs p = args_of(n);
+  p.dy = g.dy.p;
+  p.dy_row = g.dy.row;
+  p.da = g.dx;
+  p.db = g.dgate;
+  p.parts = (float*)workspace;
+  if (n.gate.p) backward<GATED>(p, n.dtype, n.out_dtype, n.groups, g.dweight, nullptr, stream);
+  else backward<PLAIN>(p, n.dtype, n.out_dtype, n.groups, g.dweight, nullptr, stream);
+}
+
+size_t add_norm_workspace(const AddNorm& n) {
+  return (size_t)backward_grid(n.rows, n.channels) * n.channels * sizeof(float) * (n.scale ? 2 : 1);
+}
+
+void add_norm(const AddNorm& n, void* sum, void* y, hipStream_t stream) {
+  NormArgs p = args_of(n);
+  p.sum = sum;
+  p.y = y;
+  forward<ADDED>(p, n.dtype, n.out_dtype, 1, stream);
+}
+
+void add_norm_backward(const AddNorm& n, const AddNormGrads& g, void* workspace, hipStream_t stream) {
+  NormArgs p = args_of(n);
+  p.dy = g.dy.p;
+  p.dy_row = g.dy.row;
+  p.dsum = g.dsum.p;
+  p.dsum_row = g.dsum.row;
+  p.da = g.dhidden;
+  p.db = g.dupdate;
+  p.parts = (float*)workspace;
+  // The sum as the forward call left it is one read for two, where it is whole (32
+  // bits) and the update's values are not needed for the scale's gradient.
+  if (g.sum && n.dtype == F32 && !n.scale) {
+    p.a = g.sum;
+    p.a_row = n.channels;
+    backward<SUMMED>(p, n.dtype, n.out_dtype, 1, g.dweight, nullptr, stream);
+  } else {
+    backward<ADDED>(p, n.dtype, n.out_dtype, 1, g.dweight, g.dscale, stream);
+  }
+}
+
+}  // namespace fhe::clear

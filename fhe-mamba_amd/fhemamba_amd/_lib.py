@@ -110,6 +110,21 @@ SIGNATURES = {
     "fhe_token_logprobs_workspace": [_p, _p],
     "fhe_token_logprobs": [_p, _p, _p, ctypes.c_size_t, _p],
     "fhe_token_logprobs_backward": [_p, _p, _p, _p, _p, _p, _p, _p],
+    "fhe_rms_norm": [_p, _p, _p],
+    "fhe_rms_norm_workspace": [_p, _p],
+    "fhe_rms_norm_backward": [_p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_add_norm": [_p, _p, _p, _p],
+    "fhe_add_norm_workspace": [_p, _p],
+    "fhe_add_norm_backward": [_p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_quantize_rows": [_p, _p, _p, _p],
+    "fhe_int8_linear_workspace": [_p, _p],
+    "fhe_int8_linear": [_p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_embed": [_p, _p, _p],
+    "fhe_embed_workspace": [_p, _p],
+    "fhe_embed_backward": [_p, _p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_beam_select_workspace": [_p, _p],
+    "fhe_beam_select": [_p, _p, _p, ctypes.c_size_t, _p],
+    "fhe_reorder_states": [_p, _u32, _u32, _u32, _u32, _p, _p, _p],
 }
 
 

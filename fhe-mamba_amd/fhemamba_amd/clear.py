@@ -9,6 +9,10 @@ the clear (the reference does it in PyTorch on the host, src/fhemamba/reference.
   causal_conv     the causal convolution before it, with its gradients
   causal_conv_step
   token_logprobs  log probabilities of given tokens, entropy and likeliest tokens, with gradients
+  embed           embeddings of tokens, with the table's gradient
+  rms_norm, add_norm  norms with the gate or the residual before them, with gradients
+  quantize_rows, int8_linear  projections in 8-bit integers, for serving
+  beam_select, reorder_states  a step of a beam search, and its states
 
 They take torch tensors on the GPU, run libfhecore's kernels on torch's current stream and return
 without waiting; inputs made on another stream need the usual synchronisation.  Activations are
@@ -33,7 +37,7 @@ import torch
 
 from . import _lib
 
-MAX_STATES, MAX_TAPS, MAX_TOP = 128, 8, 32
+MAX_STATES, MAX_TAPS, MAX_TOP, MAX_ROW = 128, 8, 32, 32768
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 # include/fhecore.h's structures: a strided tensor is an address and three strides
 _STRIDED = "Q3q"
@@ -45,6 +49,16 @@ _CONV_GRADS = struct.Struct("=" + _STRIDED + "5Q")
 _CONV_STEP = struct.Struct("=5I4xQ" + _STRIDED + "3Qi4x")
 _LOGPROB = struct.Struct("=2I3q2Q")
 _LOGPROB_OUT = struct.Struct("=6Q")
+_ROWS = struct.Struct("=Qq")  # an address and the elements between rows
+_NORM = struct.Struct("=3If2qQqQqQ")
+_NORM_GRADS = struct.Struct("=Qq3Q")
+_ADD_NORM = struct.Struct("=2If4x2qQqQq2Q")
+_ADD_NORM_GRADS = struct.Struct("=QqQq5Q")
+_QUANTIZE = struct.Struct("=I4x2qQq")
+_INT8 = struct.Struct("=I4x3qQq3Q")
+_EMBED = struct.Struct("=If3qQqQ")
+_BEAM = struct.Struct("=4I3q3Q")
+_BEAM_OUT = struct.Struct("=3Q")
 
 _F32 = (torch.float32,)
 # of a tensor that a kernel wrote in place: a backward pass that saved it raises, as after torch's own
@@ -502,3 +516,367 @@ def token_logprobs(logits, targets, *, top: int = 0) -> TokenLogprobs:
     return TokenLogprobs(logprob.reshape(lead), entropy.reshape(lead),
                          None if best is None else best.reshape(*lead, top),
                          None if index is None else index.reshape(*lead, top))
+
+
+# ----------------------------------------------------------------- rows of channels
+def _leading(name: str, t) -> None:
+    """A float tensor [.., channels] on the GPU."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a tensor on the GPU")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be float32 or bfloat16, not {t.dtype}")
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must have an axis of channels")
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """[rows, channels] with contiguous rows."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return _rows(t)
+
+
+def _row(t: Optional[torch.Tensor]) -> tuple:
+    return (0, 0) if t is None else (t.data_ptr(), t.stride(0))
+
+
+def _eps(eps) -> float:
+    if not 0.0 <= eps < 3.4e38:
+        raise ValueError("eps must be 0 or more and finite")
+    return eps
+
+
+def _narrower(name: str, dtype, like: torch.Tensor):
+    if dtype is None:
+        return like.dtype
+    if dtype not in (like.dtype, torch.bfloat16):
+        raise ValueError(f"{name} must be {like.dtype} or torch.bfloat16, not {dtype}")
+    return dtype
+
+
+# ----------------------------------------------------------------- norms
+def _pack_norm(x, weight, gate, groups, eps, dtype) -> tuple:
+    """(the packed arguments, the tensors that they point to)."""
+    x, weight = _flat(x), weight.contiguous()
+    gate = None if gate is None else _flat(gate)
+    args = _NORM.pack(_DTYPES[x.dtype], _DTYPES[dtype], groups, eps, x.shape[0], x.shape[1], *_row(x), *_row(gate),
+                      weight.data_ptr())
+    return args, (x, weight, gate)
+
+
+def _norm_forward(x, weight, gate, groups, eps, dtype):
+    args, held = _pack_norm(x, weight, gate, groups, eps, dtype)
+    y = x.new_empty(x.shape, dtype=dtype)
+    _run(_lib.lib.fhe_rms_norm, x, args, y.data_ptr())
+    return y
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, gate, groups, eps, dtype):
+        ctx.save_for_backward(x, weight, gate)
+        ctx.options = groups, eps, dtype
+        return _norm_forward(x, weight, gate, groups, eps, dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, gate = ctx.saved_tensors
+        args, held = _pack_norm(x, weight, gate, *ctx.options)
+        dy = _flat(dy)
+        dx, dw = x.new_empty(x.shape), weight.new_empty(weight.shape)
+        dgate = None if gate is None else gate.new_empty(gate.shape)
+        grads = _NORM_GRADS.pack(*_row(dy), dx.data_ptr(), _ptr(dgate), dw.data_ptr())
+        space, size = _workspace(_lib.lib.fhe_rms_norm_workspace, x, args)
+        _run(_lib.lib.fhe_rms_norm_backward, x, args, grads, space.data_ptr(), size)
+        return dx, dw, dgate, None, None, None
+
+
+def rms_norm(x, weight, *, gate=None, groups: int = 1, eps: float = 1e-5, dtype=None):
+    """v / sqrt(mean(v^2) + eps) * weight with v = x silu(gate), or x without a gate.
+
+    x [.., channels] and gate alike, weight [channels] float32.  The mean is over each of `groups`
+    equal parts of the channels, of at most 32768 each.  The result is of x's type or, with dtype,
+    bfloat16.  Differentiable in x, weight and gate.  Squares are summed in 32 bits: a row with values
+    over 2^63 gives zeros; one with a value that is not finite has NaN in it."""
+    _leading("x", x)
+    channels = x.shape[-1]
+    if groups < 1 or channels % groups or channels // groups > MAX_ROW or groups > 65535:
+        raise ValueError(f"{channels} channels do not divide into {groups} groups of at most {MAX_ROW}")
+    _gpu("weight", weight, _F32, (channels,), x)
+    if gate is not None:
+        _gpu("gate", gate, (x.dtype,), x.shape, x)
+    dtype, eps = _narrower("dtype", dtype, x), _eps(eps)
+    if _wants_grad(x, weight, gate):
+        return _Norm.apply(x, weight, gate, groups, eps, dtype)
+    return _norm_forward(x, weight, gate, groups, eps, dtype)
+
+
+class AddNorm(NamedTuple):
+    """normed [.., channels] of the update's type and hidden, the sum, of the first hidden's."""
+    normed: torch.Tensor
+    hidden: torch.Tensor
+
+
+def _pack_add_norm(hidden, update, weight, scale, eps, dtypes, shape) -> tuple:
+    """(the packed arguments, the tensors that they point to)."""
+    weight = weight.contiguous()
+    hidden, update = (None if t is None else _flat(t) for t in (hidden, update))
+    scale = None if scale is None else scale.contiguous()
+    channels = shape[-1]
+    rows = shape.numel() // channels
+    args = _ADD_NORM.pack(_DTYPES[dtypes[0]], _DTYPES[dtypes[1]], eps, rows, channels, *_row(hidden), *_row(update),
+                          _ptr(scale), weight.data_ptr())
+    return args, (hidden, update, weight, scale)
+
+
+def _add_norm_forward(hidden, update, weight, scale, eps):
+    args, held = _pack_add_norm(hidden, update, weight, scale, eps, (hidden.dtype, update.dtype), hidden.shape)
+    total, y = hidden.new_empty(hidden.shape), update.new_empty(hidden.shape)
+    _run(_lib.lib.fhe_add_norm, hidden, args, total.data_ptr(), y.data_ptr())
+    return y, total
+
+
+class _AddNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, update, weight, scale, eps):
+        y, total = _add_norm_forward(hidden, update, weight, scale, eps)
+        ctx.options = eps, (hidden.dtype, update.dtype), hidden.shape
+        ctx.whole = hidden.dtype == torch.float32 and scale is None  # the sum says all that the gradient needs
+        if ctx.whole:
+            ctx.save_for_backward(weight, total)
+        else:
+            ctx.save_for_backward(weight, hidden, update, scale)
+        ctx.set_materialize_grads(False)
+        return y, total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dtotal):
+        eps, dtypes, shape = ctx.options
+        total = hidden = update = scale = None
+        if ctx.whole:
+            weight, total = ctx.saved_tensors
+        else:
+            weight, hidden, update, scale = ctx.saved_tensors
+        args, held = _pack_add_norm(hidden, update, weight, scale, eps, dtypes, shape)
+        dy, dtotal = (None if t is None else _flat(t) for t in (dy, dtotal))
+        dh, du = (weight.new_empty(shape, dtype=t) for t in dtypes)
+        dw, ds = weight.new_empty(weight.shape), None if scale is None else scale.new_empty(scale.shape)
+        grads = _ADD_NORM_GRADS.pack(*_row(dy), *_row(dtotal), _ptr(total), dh.data_ptr(), du.data_ptr(), _ptr(ds),
+                                     dw.data_ptr())
+        space, size = _workspace(_lib.lib.fhe_add_norm_workspace, weight, args)
+        _run(_lib.lib.fhe_add_norm_backward, weight, args, grads, space.data_ptr(), size)
+        return dh, du, dw, ds, None
+
+
+def add_norm(hidden, update, weight, *, scale=None, eps: float = 1e-5) -> AddNorm:
+    """The residual and the next norm: h = hidden + scale update, and h / sqrt(mean(h^2) + eps) * weight.
+
+    hidden [.., channels] (at most 32768) and update alike, of hidden's type or bfloat16; scale (default
+    ones) and weight [channels] float32.  The norm is of the unrounded sum, and has the update's type.
+    Differentiable in all four; the backward pass needs the sum (32-bit hidden without a scale) or hidden
+    and update as they were.  Large and not finite values as in rms_norm."""
+    _leading("hidden", hidden)
+    channels = hidden.shape[-1]
+    if channels > MAX_ROW:
+        raise ValueError(f"{channels} channels: at most {MAX_ROW}")
+    _gpu("update", update, (hidden.dtype, torch.bfloat16), hidden.shape, hidden)
+    _gpu("weight", weight, _F32, (channels,), hidden)
+    if scale is not None:
+        _gpu("scale", scale, _F32, (channels,), hidden)
+    eps = _eps(eps)
+    if _wants_grad(hidden, update, weight, scale):
+        return AddNorm(*_AddNorm.apply(hidden, update, weight, scale, eps))
+    return AddNorm(*_add_norm_forward(hidden, update, weight, scale, eps))
+
+
+# ----------------------------------------------------------------- 8-bit products
+class Int8Rows(NamedTuple):
+    """values [.., channels] int8 and scale [..] float32: a row is its values times its scale."""
+    values: torch.Tensor
+    scale: torch.Tensor
+
+
+def quantize_rows(x) -> Int8Rows:
+    """Each row of x [.., channels] (at most 32768) as 8-bit integers: scale = max|x| / 127, values = the
+    integer nearest to x / scale, even among equals, both quotients rounded to float32 first.
+
+    A row of zeros has scale 0; one with a value that is not finite has scale NaN and values 0."""
+    _leading("x", x)
+    channels = x.shape[-1]
+    if channels > MAX_ROW:
+        raise ValueError(f"{channels} channels: at most {MAX_ROW}")
+    if _wants_grad(x):
+        raise ValueError("quantize_rows has no gradient: call it under torch.no_grad()")
+    rows = _flat(x)
+    values = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    args = _QUANTIZE.pack(_DTYPES[x.dtype], rows.shape[0], channels, *_row(rows))
+    _run(_lib.lib.fhe_quantize_rows, x, args, values.data_ptr(), scale.data_ptr())
+    return Int8Rows(values, scale)
+
+
+def int8_linear(x, weight, weight_scale, bias=None):
+    """x [.., inputs] times weight [outputs, inputs] int8 and weight_scale [outputs] float32 (as
+    quantize_rows gives them), plus bias [outputs] float32: [.., outputs] of x's type.
+
+    x's rows are rounded as quantize_rows does (at most 32768 inputs); the sums of products are exact, and
+    scaled in 32 bits.  A row with a value that is not finite gives NaN.  For serving: no gradient."""
+    _leading("x", x)
+    _axes("weight", weight, 2, "be [outputs, inputs]")
+    inputs, outputs = x.shape[-1], weight.shape[0]
+    if inputs > MAX_ROW:
+        raise ValueError(f"{inputs} inputs: at most {MAX_ROW}")
+    if outputs < 1:
+        raise ValueError("no outputs")
+    _gpu("weight", weight, (torch.int8,), (outputs, inputs), x)
+    _gpu("weight_scale", weight_scale, _F32, (outputs,), x)
+    if bias is not None:
+        _gpu("bias", bias, _F32, (outputs,), x)
+        bias = bias.contiguous()
+    if _wants_grad(x, weight_scale, bias):
+        raise ValueError("int8_linear has no gradient: call it under torch.no_grad()")
+    rows, weight, weight_scale = _flat(x), weight.contiguous(), weight_scale.contiguous()
+    y = x.new_empty((*x.shape[:-1], outputs))
+    args = _INT8.pack(_DTYPES[x.dtype], rows.shape[0], inputs, outputs, *_row(rows), weight.data_ptr(),
+                      weight_scale.data_ptr(), _ptr(bias))
+    space, size = _workspace(_lib.lib.fhe_int8_linear_workspace, x, args)
+    _run(_lib.lib.fhe_int8_linear, x, args, y.data_ptr(), space.data_ptr(), size)
+    return y
+
+
+# ----------------------------------------------------------------- embeddings
+def _pack_embed(weight: Optional[torch.Tensor], ids, scale: float, dtype, vocab: int, channels: int) -> bytes:
+    return _EMBED.pack(_DTYPES[dtype], scale, ids.numel(), vocab, channels, *_row(weight), ids.data_ptr())
+
+
+def _embed_forward(weight, ids, scale: float):
+    rows, ids = _rows(weight), ids.contiguous()
+    y = weight.new_empty((*ids.shape, weight.shape[1]))
+    _run(_lib.lib.fhe_embed, weight, _pack_embed(rows, ids, scale, weight.dtype, *weight.shape), y.data_ptr())
+    return y
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale):
+        ctx.save_for_backward(ids)
+        ctx.options = scale, weight.dtype, *weight.shape
+        return _embed_forward(weight, ids, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        ids, dy = ids.contiguous(), _flat(dy)
+        args = _pack_embed(None, ids, *ctx.options)
+        dw = dy.new_empty(ctx.options[2:])
+        space, size = _workspace(_lib.lib.fhe_embed_workspace, dy, args)
+        _run(_lib.lib.fhe_embed_backward, dy, args, _ROWS.pack(*_row(dy)), dw.data_ptr(), space.data_ptr(), size)
+        return dw, None, None
+
+
+def embed(weight, ids, *, scale: float = 1.0):
+    """scale * weight[ids]: weight [vocab, channels], ids [..] int64 -> [.., channels] of weight's type.
+
+    An id below 0 is padding: zeros, and no gradient from it; one of vocab or more gives NaN.
+    Differentiable in weight: the gradient is dense, each row the sum in 32 bits of its tokens' in
+    their order."""
+    _first("weight", weight, 2)
+    if min(weight.shape) < 1:
+        raise ValueError("weight must have a vocabulary and channels")
+    if not isinstance(ids, torch.Tensor):
+        raise ValueError("ids must be a tensor")
+    _gpu("ids", ids, (torch.int64,), ids.shape, weight)
+    if not abs(scale) < 3.4e38:
+        raise ValueError("scale must be finite")
+    if _wants_grad(weight):
+        return _Embed.apply(weight, ids, scale)
+    return _embed_forward(weight, ids, scale)
+
+
+# ----------------------------------------------------------------- beam search
+class BeamChoice(NamedTuple):
+    """score float32, parent and token int32, each [requests, width], best first."""
+    score: torch.Tensor
+    parent: torch.Tensor
+    token: torch.Tensor
+
+
+def beam_select(logits, scores, width: Optional[int] = None, *, finished=None, end: Optional[int] = None) -> BeamChoice:
+    """The `width` (default: as many as there are beams; at most 32) best continuations of each request.
+
+    logits [requests, beams, vocab] (at most 32 beams) and scores [requests, beams] float32: a candidate is
+    a beam and a token, its score the beam's plus the token's log probability; the lower beam, then the
+    lower token first among equals.  A beam of score -inf has none.  finished [requests, beams] bool: such
+    a beam has the one candidate `end`, at its own score.  Where fewer candidates are allowed, others
+    follow with score -inf.  A NaN or +inf among a live beam's logits, or for a score, makes the beam's
+    candidates NaN, which come first.  No gradient (token_logprobs at the chosen tokens has one)."""
+    _first("logits", logits, 3)
+    requests, beams, vocab = logits.shape
+    if min(requests, beams, vocab) < 1 or beams > MAX_TOP or requests > 65535:
+        raise ValueError(f"logits must be [requests, beams, vocab] with 1 to 65535 requests and 1 to {MAX_TOP} beams")
+    _gpu("scores", scores, _F32, (requests, beams), logits)
+    width = beams if width is None else width
+    if not 1 <= width <= min(MAX_TOP, beams * vocab):
+        raise ValueError(f"width must be 1 to {min(MAX_TOP, beams * vocab)}")
+    if finished is not None:
+        _gpu("finished", finished, (torch.bool,), (requests, beams), logits)
+        if end is None or not 0 <= end < vocab:
+            raise ValueError("end must be a token where beams may be finished")
+        finished = finished.contiguous()
+    if _wants_grad(logits, scores):
+        raise ValueError("beam_select has no gradient: call it under torch.no_grad()")
+    rows, scores = _flat(logits), scores.contiguous()
+    if rows.shape[0] > 1 and rows.stride(0) < vocab:  # one row for all
+        rows = rows.contiguous()
+    args = _BEAM.pack(_DTYPES[logits.dtype], requests, beams, width, vocab, rows.stride(0), -1 if end is None else end,
+                      rows.data_ptr(), scores.data_ptr(), _ptr(finished))
+    score = scores.new_empty((requests, width))
+    parent, token = (scores.new_empty((requests, width), dtype=torch.int32) for _ in range(2))
+    out = _BEAM_OUT.pack(score.data_ptr(), parent.data_ptr(), token.data_ptr())
+    space, size = _workspace(_lib.lib.fhe_beam_select_workspace, logits, args)
+    _run(_lib.lib.fhe_beam_select, logits, args, out, space.data_ptr(), size)
+    return BeamChoice(score, parent, token)
+
+
+def reorder_states(states, parent, *, slots=None) -> None:
+    """The states follow their beams, in place: row slots[r, j] takes what row slots[r, parent[r, j]] held.
+
+    states: a tensor [cache, ..] or a sequence of them with as many rows, of any type, contiguous; all
+    move in one launch.  parent [requests, beams] int32 (at most 32 beams) as beam_select gives it, slots
+    alike (default r * beams + j), no row twice.  A parent that is no beam leaves the row as it is; a slot
+    outside of the cache is padding.  A backward pass that needs a state as it was before raises."""
+    states = (states,) if isinstance(states, torch.Tensor) else tuple(states)
+    if not states:
+        raise ValueError("no states")
+    _axes("parent", parent, 2, "be [requests, beams]")
+    requests, beams = parent.shape
+    first = states[0]
+    if not isinstance(first, torch.Tensor) or not first.is_cuda:
+        raise ValueError("states must be tensors on the GPU")
+    if not (1 <= requests <= 65535 and 1 <= beams <= MAX_TOP):
+        raise ValueError(f"parent must be [requests, beams] with 1 to 65535 requests and 1 to {MAX_TOP} beams")
+    _gpu("parent", parent, (torch.int32,), (requests, beams), first)
+    cache = first.shape[0] if first.dim() else 0
+    if slots is not None:
+        _gpu("slots", slots, (torch.int32,), (requests, beams), first)
+        slots = slots.contiguous()
+    elif requests * beams > cache:
+        raise ValueError(f"{requests * beams} beams and {cache} rows of the states")
+    packed = []
+    for t in states:
+        if not isinstance(t, torch.Tensor) or t.device != first.device:
+            raise ValueError("states must be tensors on one GPU")
+        if not t.dim() or t.shape[0] != cache or cache < 1:
+            raise ValueError("states must have the same number of rows, one or more")
+        if not t.is_contiguous():
+            raise ValueError("states must be contiguous: they are updated in place")
+        packed.append(_ROWS.pack(t.data_ptr(), t.nbytes // cache))
+    if _wants_grad(*states):
+        raise ValueError("reorder_states has no gradient: call it under torch.no_grad()")
+    parent = parent.contiguous()
+    _run(_lib.lib.fhe_reorder_states, first, b"".join(packed), len(states), requests, beams, cache, parent.data_ptr(),
+         _ptr(slots))
+    _changed(states)

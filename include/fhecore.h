@@ -492,6 +492,148 @@ int fhe_token_logprobs_backward(const fhe_logprob_args *args,
                                 const float *dentropy, void *dlogits,
                                 void *hip_stream);
 
+/* Rows [rows][channels], `stride` elements apart. */
+typedef struct {
+  const void *data;
+  int64_t stride;
+} fhe_rows;
+
+/* y = v / sqrt(mean(v^2) + eps) * weight with v = x silu(gate), or x where there
+ * is no gate (data NULL); the mean is over each of `groups` equal parts of the
+ * channels.  x and gate in dtype, y [rows][channels] in out_dtype, which is dtype
+ * or FHE_BF16.  A part has at most FHE_MAX_ROW channels.  Squares are summed in 32
+ * bits: values over 2^63 give zeros.  A row with a value that is not finite has
+ * NaN in it. */
+enum { FHE_MAX_ROW = 32768 };
+typedef struct {
+  uint32_t dtype, out_dtype, groups;
+  float eps;
+  int64_t rows, channels;
+  fhe_rows x, gate;
+  const float *weight;
+} fhe_norm_args;
+int fhe_rms_norm(const fhe_norm_args *args, void *y, void *hip_stream);
+int fhe_rms_norm_workspace(const fhe_norm_args *args, size_t *bytes);
+/* From dy in out_dtype: dx and dgate [rows][channels] in dtype (dgate with a gate
+ * only), dweight [channels].  Sums have a fixed order. */
+typedef struct {
+  fhe_rows dy;
+  void *dx, *dgate;
+  float *dweight;
+} fhe_norm_grads;
+int fhe_rms_norm_backward(const fhe_norm_args *args,
+                          const fhe_norm_grads *grads, void *workspace,
+                          size_t bytes, void *hip_stream);
+
+/* sum = hidden + scale update (scale [channels], or NULL: 1), y the norm of the
+ * unrounded sum as above.  hidden and sum in dtype, update and y in out_dtype. */
+typedef struct {
+  uint32_t dtype, out_dtype;
+  float eps;
+  uint32_t reserved;
+  int64_t rows, channels;
+  fhe_rows hidden, update;
+  const float *scale, *weight;
+} fhe_add_norm_args;
+int fhe_add_norm(const fhe_add_norm_args *args, void *sum, void *y,
+                 void *hip_stream);
+int fhe_add_norm_workspace(const fhe_add_norm_args *args, size_t *bytes);
+/* From dy and the gradient of sum (data NULL: zeros).  sum: the forward call's, or
+ * NULL; where it serves (32 bits, no scale) hidden and update are not read.
+ * dhidden and dupdate [rows][channels] and dscale [channels] may be NULL. */
+typedef struct {
+  fhe_rows dy, dsum;
+  const void *sum;
+  void *dhidden, *dupdate;
+  float *dscale, *dweight;
+} fhe_add_norm_grads;
+int fhe_add_norm_backward(const fhe_add_norm_args *args,
+                          const fhe_add_norm_grads *grads, void *workspace,
+                          size_t bytes, void *hip_stream);
+
+/* scale [rows] = max|x| / 127 and values [rows][channels] = the integer nearest
+ * to x / scale (even among equals; both quotients rounded to 32 bits first), within
+ * -127 .. 127.  A row of zeros has scale 0; one with a value that is not finite has
+ * scale NaN and values 0.  channels <= FHE_MAX_ROW. */
+typedef struct {
+  uint32_t dtype, reserved;
+  int64_t rows, channels;
+  fhe_rows x;
+} fhe_quantize_args;
+int fhe_quantize_rows(const fhe_quantize_args *args, int8_t *values,
+                      float *scale, void *hip_stream);
+
+/* y = (q weight^T) row_scale scale + bias, q and row_scale those of x's rows as
+ * above: [rows][outputs] in dtype.  weight [outputs][inputs], scale and bias
+ * [outputs] (bias may be NULL).  The sums of products are exact. */
+typedef struct {
+  uint32_t dtype, reserved;
+  int64_t rows, inputs, outputs;
+  fhe_rows x;
+  const int8_t *weight;
+  const float *scale, *bias;
+} fhe_int8_args;
+int fhe_int8_linear_workspace(const fhe_int8_args *args, size_t *bytes);
+int fhe_int8_linear(const fhe_int8_args *args, void *y, void *workspace,
+                    size_t bytes, void *hip_stream);
+
+/* y [tokens][channels] = scale weight[id] in dtype; zeros where an id is below 0,
+ * NaN where it is vocab or more. */
+typedef struct {
+  uint32_t dtype;
+  float scale;
+  int64_t tokens, vocab, channels;
+  fhe_rows weight;
+  const int64_t *ids;
+} fhe_embed_args;
+int fhe_embed(const fhe_embed_args *args, void *y, void *hip_stream);
+int fhe_embed_workspace(const fhe_embed_args *args, size_t *bytes);
+/* dweight [vocab][channels] in dtype: scale times the sum, in 32 bits and in the
+ * tokens' order, of each id's rows of dy.  weight is not read. */
+int fhe_embed_backward(const fhe_embed_args *args, const fhe_rows *dy,
+                       void *dweight, void *workspace, size_t bytes,
+                       void *hip_stream);
+
+/* A step of a beam search: of all candidates (beam, token) of a request, which
+ * have the beam's score plus the token's log probability, the `width` <=
+ * FHE_MAX_TOP largest, in order, the lower beam and then the lower token first
+ * among equals: score, parent and token [requests][width].  logits
+ * [requests * beams][vocab], row_stride elements apart; beams <= FHE_MAX_TOP,
+ * width <= beams * vocab.  A finished beam (finished may be NULL) has the one
+ * candidate `end`, at its own score; its logits are not read, nor those of a beam
+ * of score -infinity.  Candidates that are not allowed (a logit of -infinity, a
+ * beam of score -infinity) have score -infinity.  A NaN or +infinity among a
+ * beam's logits or for its score makes its candidates NaN, which come first. */
+typedef struct {
+  uint32_t dtype, requests, beams, width;
+  int64_t vocab, row_stride, end;
+  const void *logits;
+  const float *scores;
+  const uint8_t *finished;
+} fhe_beam_args;
+typedef struct {
+  float *score;
+  int32_t *parent, *token;
+} fhe_beam_out;
+int fhe_beam_select_workspace(const fhe_beam_args *args, size_t *bytes);
+int fhe_beam_select(const fhe_beam_args *args, const fhe_beam_out *out,
+                    void *workspace, size_t bytes, void *hip_stream);
+
+/* Rows follow their beams in place: row slots[r][j] of every state takes what row
+ * slots[r][parent[r][j]] held before the call.  states [count]: an array on the
+ * host; each has `cache` contiguous rows of row_bytes <= 2^30.  parent [requests]
+ * [beams] and slots (device; slots NULL: r * beams + j).  A parent outside of
+ * [0, beams) leaves the row as it is, a slot outside of [0, cache) is padding.  No
+ * row may be named twice. */
+typedef struct {
+  void *data;
+  int64_t row_bytes;
+} fhe_state_rows;
+int fhe_reorder_states(const fhe_state_rows *states, uint32_t count,
+                       uint32_t requests, uint32_t beams, uint32_t cache,
+                       const int32_t *parent, const int32_t *slots,
+                       void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif
