@@ -164,28 +164,47 @@ struct SumArgs {
 };
 
 constexpr int COLUMNS = 4;  // pieces of 256 channels at a time
+constexpr int LOADS = 4;    // tokens whose rows are in flight
 
-// out[c] = the sum of dy over `token[0 .. count)`, for the channels that `first`
-// and up hold in this wavefront's lanes.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The sum of dy over `token[0 .. count)`, for the channels that `first` and up hold
+// in this wavefront's lanes.  count and first are the same in all lanes.
 template <class T>
 __device__ __forceinline__ void add_rows(const SumArgs& a, const int* token, int count, int first,
                                          f32x4 (&sum)[COLUMNS]) {
   const int lane = lane_id();
 #pragma unroll
   for (int k = 0; k < COLUMNS; ++k) sum[k] = f32x4{};
-  for (int i = 0; i < count; ++i) {
-    const T* row = (const T*)a.dy + (int64_t)token[i] * a.dy_row;
+  for (int base = 0; base < count; base += 64) {
+    const int some = count - base < 64 ? count - base : 64;
+    const int mine = lane < some ? token[base + lane] : 0;
+    for (int i = 0; i < some; i += LOADS) {
+      f32x4 v[LOADS][COLUMNS];
 #pragma unroll
-    for (int k = 0; k < COLUMNS; ++k) {
-      const int c = first + (k * 64 + lane) * 4;
-      if (c < a.channels) sum[k] += get4(row + c, a.channels - c);
+      for (int j = 0; j < LOADS; ++j) {
+        // past the last token the last one again, times nothing
+        const int t = __builtin_amdgcn_readlane(mine, i + j < some ? i + j : some - 1);
+        const T* row = (const T*)a.dy + (int64_t)t * a.dy_row + first;
+#pragma unroll
+        for (int k = 0; k < COLUMNS; ++k) {
+          const int c = (k * 64 + lane) * 4;
+          v[j][k] = first + k * 256 < a.channels ? get4(row + c, a.channels - first - c) : f32x4{};
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j)
+        if (i + j < some) {
+#pragma unroll
+          for (int k = 0; k < COLUMNS; ++k) sum[k] += v[j][k];
+        }
     }
   }
 }
 
 template <class T>
 __global__ __launch_bounds__(256) void k_sums(SumArgs a) {
-  const int wave = threadIdx.x >> 6, lane = lane_id();
+  const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
   if ((int)blockIdx.x < a.pieces) {
     // a row of more than `piece` tokens covers a piece's end or its begin
     const int64_t begin = (int64_t)blockIdx.x * a.piece, all = a.o.start[a.vocab];
@@ -200,7 +219,7 @@ __global__ __launch_bounds__(256) void k_sums(SumArgs a) {
       float* out = a.parts + ((int64_t)blockIdx.x * 2 + side) * a.channels;
       for (int c0 = wave * 256 * COLUMNS; c0 < a.channels; c0 += 4 * 256 * COLUMNS) {
         f32x4 sum[COLUMNS];
-        add_rows<T>(a, a.o.token + f, (int)(t - f), c0, sum);
+        add_rows<T>(a, a.o.token + f, uniform((int)(t - f)), c0, sum);
 #pragma unroll
         for (int k = 0; k < COLUMNS; ++k) {
           const int c = c0 + (k * 64 + lane) * 4;
@@ -212,7 +231,7 @@ __global__ __launch_bounds__(256) void k_sums(SumArgs a) {
   }
   const int64_t row = ((int64_t)blockIdx.x - a.pieces) * 4 + wave;
   if (row >= a.vocab) return;
-  const int from = a.o.start[row], count = a.o.start[row + 1] - from;
+  const int from = uniform(a.o.start[row]), count = uniform(a.o.start[row + 1]) - from;
   if (count > a.piece) return;
   T* out = (T*)a.dweight + row * a.channels;
   for (int c0 = 0; c0 < a.channels; c0 += 256 * COLUMNS) {
@@ -238,12 +257,13 @@ __global__ __launch_bounds__(256) void k_join(SumArgs a) {
   const int64_t last = (to - 1) / a.piece;
   for (int c = threadIdx.x; c < a.channels; c += 256) {
     float s = a.parts[((int64_t)blockIdx.x * 2 + 1) * a.channels + c];
+#pragma unroll 8
     for (int64_t i = blockIdx.x + 1; i <= last; ++i) s += a.parts[i * 2 * a.channels + c];
     ((T*)a.dweight)[(int64_t)row * a.channels + c] = (T)(s * a.scale);
   }
 }
 
-int piece_of(int64_t tokens) { return (int)std::max<int64_t>(64, (tokens + 1023) / 1024); }
+int piece_of(int64_t tokens) { return (int)std::max<int64_t>(32, (tokens + 1023) / 1024); }
 size_t line(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace

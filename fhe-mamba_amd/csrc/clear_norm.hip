@@ -220,20 +220,26 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
 }
 
 // out[c] = the sum over workgroups of parts[.][c]; blockIdx.y: of which of the outputs.
+constexpr int SUM_COLUMNS = 16;
 __global__ __launch_bounds__(1024) void k_norm_sum(const float* parts, int count, int all, float* out0, float* out1) {
-  __shared__ float lds[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
+  constexpr int LANES = 1024 / SUM_COLUMNS;
+  __shared__ float lds[LANES][SUM_COLUMNS + 1];
+  const int at = threadIdx.x % SUM_COLUMNS, lane = threadIdx.x / SUM_COLUMNS;
+  const int c = blockIdx.x * SUM_COLUMNS + at;
   parts += (int64_t)blockIdx.y * count * all;
   float s = 0.0f;
-  if (c < all)
-    for (int i = lane; i < count; i += 16) s += parts[(int64_t)i * all + c];
-  lds[lane][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (lane || c >= all) return;
+  if (c < all) {
+#pragma unroll 8
+    for (int i = lane; i < count; i += LANES) s += parts[(int64_t)i * all + c];
+  }
+  lds[lane][at] = s;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) s += lds[i][threadIdx.x];
+  for (int half = LANES / 2; half; half /= 2) {
+    __syncthreads();
+    if (lane < half) lds[lane][at] = s += lds[lane + half][at];
+  }
   float* out = blockIdx.y ? out1 : out0;
-  if (out) out[c] = s;
+  if (!lane && c < all && out) out[c] = s;
 }
 
 template <class F>
@@ -277,7 +283,7 @@ void backward(const NormArgs& p, uint32_t dtype, uint32_t out, int groups, float
     });
   });
   hip_check(hipGetLastError(), "norm gradient");
-  k_norm_sum<<<dim3((p.all + 63) / 64, p.scale ? 2 : 1), 1024, 0, stream>>>(p.parts, count, p.all, dweight, dscale);
+  k_norm_sum<<<dim3((p.all + SUM_COLUMNS - 1) / SUM_COLUMNS, p.scale ? 2 : 1), 1024, 0, stream>>>(p.parts, count, p.all, dweight, dscale);
   hip_check(hipGetLastError(), "norm gradient sums");
 }
 

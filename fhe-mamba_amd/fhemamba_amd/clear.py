@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from itertools import chain, repeat
 from typing import NamedTuple, Optional
 
 import torch
@@ -67,6 +68,7 @@ _forward_ad = torch.autograd.forward_ad
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_device_of, _size_of, _is_contiguous = torch.Tensor.get_device, torch.Tensor.size, torch.Tensor.is_contiguous
 
 
 def _run(entry, like: torch.Tensor, *args) -> None:
@@ -130,12 +132,13 @@ def _strides2(t: torch.Tensor, packed: bool) -> tuple:
 
 
 def _workspace(entry, like: torch.Tensor, *args, more: int = 0) -> tuple:
-    """(bytes that the entry point asks for and `more` behind them, how many it asks for)."""
+    """(bytes that the entry point asks for and `more` behind them, or None for none; how many it asks for)."""
     size = ctypes.c_size_t()
     code = entry(*args, ctypes.byref(size))
     if code:
         _lib.check(code)
-    return like.new_empty(size.value + more, dtype=torch.uint8), size.value
+    size = size.value
+    return like.new_empty(size + more, dtype=torch.uint8) if size + more else None, size
 
 
 def _offsets(cu_seqlens, like: torch.Tensor) -> None:
@@ -540,6 +543,11 @@ def _row(t: Optional[torch.Tensor]) -> tuple:
     return (0, 0) if t is None else (t.data_ptr(), t.stride(0))
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _eps(eps) -> float:
     if not 0.0 <= eps < 3.4e38:
         raise ValueError("eps must be 0 or more and finite")
@@ -566,7 +574,7 @@ def _pack_norm(x, weight, gate, groups, eps, dtype) -> tuple:
 
 def _norm_forward(x, weight, gate, groups, eps, dtype):
     args, held = _pack_norm(x, weight, gate, groups, eps, dtype)
-    y = x.new_empty(x.shape, dtype=dtype)
+    y = _like(x) if dtype == x.dtype else x.new_empty(x.shape, dtype=dtype)
     _run(_lib.lib.fhe_rms_norm, x, args, y.data_ptr())
     return y
 
@@ -584,8 +592,7 @@ class _Norm(torch.autograd.Function):
         x, weight, gate = ctx.saved_tensors
         args, held = _pack_norm(x, weight, gate, *ctx.options)
         dy = _flat(dy)
-        dx, dw = x.new_empty(x.shape), weight.new_empty(weight.shape)
-        dgate = None if gate is None else gate.new_empty(gate.shape)
+        dx, dw, dgate = _like(x), _like(weight), None if gate is None else _like(gate)
         grads = _NORM_GRADS.pack(*_row(dy), dx.data_ptr(), _ptr(dgate), dw.data_ptr())
         space, size = _workspace(_lib.lib.fhe_rms_norm_workspace, x, args)
         _run(_lib.lib.fhe_rms_norm_backward, x, args, grads, space.data_ptr(), size)
@@ -621,18 +628,19 @@ class AddNorm(NamedTuple):
 def _pack_add_norm(hidden, update, weight, scale, eps, dtypes, shape) -> tuple:
     """(the packed arguments, the tensors that they point to)."""
     weight = weight.contiguous()
-    hidden, update = (None if t is None else _flat(t) for t in (hidden, update))
-    scale = None if scale is None else scale.contiguous()
+    if hidden is not None:
+        hidden, update = _flat(hidden), _flat(update)
+    if scale is not None:
+        scale = scale.contiguous()
     channels = shape[-1]
-    rows = shape.numel() // channels
-    args = _ADD_NORM.pack(_DTYPES[dtypes[0]], _DTYPES[dtypes[1]], eps, rows, channels, *_row(hidden), *_row(update),
-                          _ptr(scale), weight.data_ptr())
+    args = _ADD_NORM.pack(_DTYPES[dtypes[0]], _DTYPES[dtypes[1]], eps, shape.numel() // channels, channels,
+                          *_row(hidden), *_row(update), _ptr(scale), weight.data_ptr())
     return args, (hidden, update, weight, scale)
 
 
 def _add_norm_forward(hidden, update, weight, scale, eps):
     args, held = _pack_add_norm(hidden, update, weight, scale, eps, (hidden.dtype, update.dtype), hidden.shape)
-    total, y = hidden.new_empty(hidden.shape), update.new_empty(hidden.shape)
+    total, y = _like(hidden), _like(update)
     _run(_lib.lib.fhe_add_norm, hidden, args, total.data_ptr(), y.data_ptr())
     return y, total
 
@@ -662,7 +670,7 @@ class _AddNorm(torch.autograd.Function):
         args, held = _pack_add_norm(hidden, update, weight, scale, eps, dtypes, shape)
         dy, dtotal = (None if t is None else _flat(t) for t in (dy, dtotal))
         dh, du = (weight.new_empty(shape, dtype=t) for t in dtypes)
-        dw, ds = weight.new_empty(weight.shape), None if scale is None else scale.new_empty(scale.shape)
+        dw, ds = _like(weight), None if scale is None else _like(scale)
         grads = _ADD_NORM_GRADS.pack(*_row(dy), *_row(dtotal), _ptr(total), dh.data_ptr(), du.data_ptr(), _ptr(ds),
                                      dw.data_ptr())
         space, size = _workspace(_lib.lib.fhe_add_norm_workspace, weight, args)
@@ -741,8 +749,8 @@ def int8_linear(x, weight, weight_scale, bias=None):
     y = x.new_empty((*x.shape[:-1], outputs))
     args = _INT8.pack(_DTYPES[x.dtype], rows.shape[0], inputs, outputs, *_row(rows), weight.data_ptr(),
                       weight_scale.data_ptr(), _ptr(bias))
-    space, size = _workspace(_lib.lib.fhe_int8_linear_workspace, x, args)
-    _run(_lib.lib.fhe_int8_linear, x, args, y.data_ptr(), space.data_ptr(), size)
+    space, size = _workspace(_lib.lib.fhe_int8_linear_workspace, x, args)  # none for the fewest rows
+    _run(_lib.lib.fhe_int8_linear, x, args, y.data_ptr(), _ptr(space), size)
     return y
 
 
@@ -854,29 +862,32 @@ def reorder_states(states, parent, *, slots=None) -> None:
     _axes("parent", parent, 2, "be [requests, beams]")
     requests, beams = parent.shape
     first = states[0]
-    if not isinstance(first, torch.Tensor) or not first.is_cuda:
+    # there may be two for each layer: checked in as few Python steps as can be
+    if not all(map(isinstance, states, repeat(torch.Tensor))) or not first.is_cuda:
         raise ValueError("states must be tensors on the GPU")
+    if len(set(map(_device_of, states))) > 1:
+        raise ValueError("states must be tensors on one GPU")
     if not (1 <= requests <= 65535 and 1 <= beams <= MAX_TOP):
         raise ValueError(f"parent must be [requests, beams] with 1 to 65535 requests and 1 to {MAX_TOP} beams")
     _gpu("parent", parent, (torch.int32,), (requests, beams), first)
-    cache = first.shape[0] if first.dim() else 0
+    try:
+        rows = set(map(_size_of, states, repeat(0)))
+    except IndexError:  # a tensor without axes
+        rows = ()
+    if len(rows) != 1 or (cache := rows.pop()) < 1:
+        raise ValueError("states must have the same number of rows, one or more")
     if slots is not None:
         _gpu("slots", slots, (torch.int32,), (requests, beams), first)
         slots = slots.contiguous()
     elif requests * beams > cache:
         raise ValueError(f"{requests * beams} beams and {cache} rows of the states")
-    packed = []
-    for t in states:
-        if not isinstance(t, torch.Tensor) or t.device != first.device:
-            raise ValueError("states must be tensors on one GPU")
-        if not t.dim() or t.shape[0] != cache or cache < 1:
-            raise ValueError("states must have the same number of rows, one or more")
-        if not t.is_contiguous():
-            raise ValueError("states must be contiguous: they are updated in place")
-        packed.append(_ROWS.pack(t.data_ptr(), t.nbytes // cache))
+    if not all(map(_is_contiguous, states)):
+        raise ValueError("states must be contiguous: they are updated in place")
     if _wants_grad(*states):
         raise ValueError("reorder_states has no gradient: call it under torch.no_grad()")
+    packed = struct.pack(f"={2 * len(states)}q",
+                         *chain.from_iterable((t.data_ptr(), t.nbytes // cache) for t in states))
     parent = parent.contiguous()
-    _run(_lib.lib.fhe_reorder_states, first, b"".join(packed), len(states), requests, beams, cache, parent.data_ptr(),
+    _run(_lib.lib.fhe_reorder_states, first, packed, len(states), requests, beams, cache, parent.data_ptr(),
          _ptr(slots))
     _changed(states)

@@ -132,12 +132,13 @@ def test_int8_arguments(kw, match):
 
 
 def test_int8_outputs_and_workspace():
-    size = size_of("fhe_int8_linear_workspace", int8())
-    assert size >= 2 * 8 + 8
+    args = int8(rows=200)
+    size = size_of("fhe_int8_linear_workspace", args)
+    assert size >= 200 * 8 + 800
     for y, space, given, match in ((0, 4096, size, "null output"), (4097, 4096, size, "aligned"),
                                    (4096, 4096, size - 1, "too small"), (4096, 0, size, "null workspace")):
         with pytest.raises(ValueError, match=match):
-            _lib.call("fhe_int8_linear", int8(), y, space, given, 0)
+            _lib.call("fhe_int8_linear", args, y, space, given, 0)
     with pytest.raises(ValueError, match="null output"):
         _lib.call("fhe_quantize_rows", clear._QUANTIZE.pack(0, 2, 8, 4096, 8), 0, 4096, 0)
 
