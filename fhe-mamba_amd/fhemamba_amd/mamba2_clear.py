@@ -5,18 +5,19 @@ fits the polynomials or tunes the weights to them runs and differentiates the sa
 that it leaves start the plain decode (mamba2_payload.decode_tokens); the encrypted decode starts from
 empty ones.  The layer is mamba2_payload.layer_step with exact functions
 (src/fhemamba/reference.py:182-339): RMSNorm, in_proj, causal convolution and SiLU, the selective scan,
-the gate and its norm, out_proj, the residual; the norms and projections are torch's, the rest
-clear.py's kernels.
+the gate and its norm, out_proj, the residual; the projections are torch's unless they are asked for in
+8-bit integers, the rest clear.py's kernels.
 
     python -m fhemamba_amd.mamba2_clear PAYLOAD RESULT [--prompt-tokens K] [--dtype float32|bfloat16]
-        [--top N] [--states FILE]
+        [--int8] [--top N] [--beams K] [--states FILE]
 
 runs a payload's test embeddings: the first K (default: all but one) in one call, the others token by
 token from the states that it leaves, checks every final hidden vector against the payload's exact
 reference, and writes a fhemamba-m2-clear-result-v1 report.  With a client head in the payload the
 report has the log probability of the greedy token, the entropy and the N likeliest tokens of each
-step.  --states writes the carried states (ssm_<layer> [heads][head_dim][states], fifo_<layer>
-[taps - 1][channels]) as a .npz file.  Exit code 1: a result is further than the tolerance.
+step, and with --beams the K best continuations of the payload's prompt by a beam search.  --states
+writes the carried states (ssm_<layer> [heads][head_dim][states], fifo_<layer> [taps - 1][channels]) as a
+.npz file.  Exit code 1: a result is further than the tolerance.
 """
 from __future__ import annotations
 
@@ -25,7 +26,7 @@ import json
 import sys
 import time
 from dataclasses import dataclass
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
@@ -36,6 +37,10 @@ from .mamba2_payload import ChainPayload, LayerPayload, LayerState, read_chain_p
 # Relative 2-norm error of a final hidden vector: float32 sums over a layer's thousands of terms, or
 # bfloat16 activations, each rounding 2^-8, through the layers' residuals.
 TOLERANCE = {torch.float32: 1e-4, torch.bfloat16: 5e-2}
+# The same with projections in 8 bits: an operand's error is max / (127 sqrt(12)), 0.7% of rows whose largest
+# is three times their size, both operands' 1%; two products a layer, 7% over 24 layers, and what the gates
+# and exponentials make of it.
+INT8_TOLERANCE = 2e-1
 
 
 @dataclass
@@ -46,29 +51,41 @@ class State:
     conv: torch.Tensor
 
 
+def _project(x: torch.Tensor, weight, bias=None) -> torch.Tensor:
+    """x times a table's transpose, in x's type; the table in x's type or 8-bit rows."""
+    if isinstance(weight, clear.Int8Rows):
+        return clear.int8_linear(x, weight.values, weight.scale, bias)
+    out = x @ weight.t()
+    return out if bias is None else (out.float() + bias).to(x.dtype)
+
+
+def _table(values, dtype: torch.dtype, device, int8: bool):
+    if int8:
+        return clear.quantize_rows(torch.as_tensor(values, dtype=torch.float32, device=device))
+    return torch.as_tensor(values, dtype=dtype, device=device)
+
+
 class Layer:
-    """A payload layer's weights on the GPU; projections in the model's type, the others float32."""
+    """A payload layer's weights on the GPU; projections in the model's type or 8 bits, the others float32."""
 
     PROJECTIONS = ("in_proj_w", "out_proj_w")
     OTHERS = ("conv_w", "conv_b", "dt_bias", "a_log", "d_skip", "block_norm_w", "gated_norm_w")
 
-    def __init__(self, lay: LayerPayload, dtype: torch.dtype, device):
+    def __init__(self, lay: LayerPayload, dtype: torch.dtype, device, int8: bool = False):
         self.shape = lay
-        self.weights = {k: torch.as_tensor(lay.t(k), dtype=dtype, device=device) for k in self.PROJECTIONS}
+        self.weights = {k: _table(lay.t(k), dtype, device, int8) for k in self.PROJECTIONS}
         self.weights.update({k: torch.as_tensor(lay.t(k), dtype=torch.float32, device=device) for k in self.OTHERS})
 
-    def __call__(self, hidden: torch.Tensor, state: Optional[State], mixer) -> tuple:
-        """hidden [.., d_model] float32 -> (hidden, state); `mixer` runs the convolution and the scan."""
+    def __call__(self, normed: torch.Tensor, state: Optional[State], mixer) -> tuple:
+        """normed [.., d_model], the layer's input behind its norm -> (what the layer adds to the residual, state);
+        `mixer` runs the convolution and the scan."""
         w, s = self.weights, self.shape
-        dtype = w["in_proj_w"].dtype
-        normed = hidden * torch.rsqrt(hidden.square().mean(-1, keepdim=True) + s.eps_block) * w["block_norm_w"]
-        proj = normed.to(dtype) @ w["in_proj_w"].t()
+        proj = _project(normed, w["in_proj_w"])
         z, inputs, dt = torch.split(proj, [s.d_inner, s.conv_dim, s.num_heads], dim=-1)
         write = torch.nn.functional.softplus(dt.float() + w["dt_bias"])
         y, state = mixer(self, inputs, write, write * -torch.exp(w["a_log"]), state)
-        gated = y.flatten(-2).float() * torch.nn.functional.silu(z.float())
-        gated = gated * torch.rsqrt(gated.square().mean(-1, keepdim=True) + s.eps_gated) * w["gated_norm_w"]
-        return hidden + (gated.to(dtype) @ w["out_proj_w"].t()).float(), state
+        gated = clear.rms_norm(y.flatten(-2), w["gated_norm_w"], gate=z, eps=s.eps_gated)
+        return _project(gated, w["out_proj_w"]), state
 
     def split(self, conv: torch.Tensor) -> tuple:
         """x, B and C as views of the convolution's output."""
@@ -77,27 +94,39 @@ class Layer:
         return x.unflatten(-1, (s.num_heads, s.head_dim)), B.unsqueeze(-2), C.unsqueeze(-2)
 
 
-class ClearMamba2:
-    """The layers and the final norm of a chain payload, and its client head if it has one."""
+class BeamResult(NamedTuple):
+    """tokens [requests, beams, steps] int64 and score [requests, beams] float32, best first."""
+    tokens: torch.Tensor
+    score: torch.Tensor
 
-    def __init__(self, chain: ChainPayload, dtype: torch.dtype = torch.float32, device="cuda"):
+
+class ClearMamba2:
+    """The layers and the final norm of a chain payload, and its client head if it has one.
+
+    int8: the projections and the head in 8-bit integers with a scale for each output and token, for serving."""
+
+    def __init__(self, chain: ChainPayload, dtype: torch.dtype = torch.float32, device="cuda", int8: bool = False):
         if dtype not in TOLERANCE:
             raise ValueError(f"dtype must be float32 or bfloat16, not {dtype}")
-        self.dtype, self.device = dtype, torch.device(device)
-        self.layers = [Layer(lay, dtype, device) for lay in chain.layers]
+        self.dtype, self.device, self.int8 = dtype, torch.device(device), int8
+        self.layers = [Layer(lay, dtype, device, int8) for lay in chain.layers]
         self.norm_eps = chain.final_norm_eps
         self.norm_w = torch.as_tensor(chain.final_norm_w, dtype=torch.float32, device=device)
         self.embedding = self.head = self.head_bias = None
         ar = chain.autoregressive
         if ar is not None:
             self.embedding = torch.as_tensor(ar.embedding_w, dtype=torch.float32, device=device)
-            tied = ar.lm_head_w is None
-            self.head = self.embedding.to(dtype) if tied else torch.as_tensor(ar.lm_head_w, dtype=dtype, device=device)
+            if ar.lm_head_w is None and not int8:
+                self.head = self.embedding.to(dtype)
+            else:
+                self.head = _table(ar.embedding_w if ar.lm_head_w is None else ar.lm_head_w, dtype, device, int8)
             if ar.lm_head_b is not None:
                 self.head_bias = torch.as_tensor(ar.lm_head_b, dtype=torch.float32, device=device)
 
     def parameters(self) -> list:
         """The layers' and the final norm's weights (the head and the embeddings stay as they are)."""
+        if self.int8:
+            raise ValueError("a model in 8-bit integers is not trained")
         return [v for lay in self.layers for v in lay.weights.values()] + [self.norm_w]
 
     def zero_states(self, rows: int) -> list:
@@ -109,8 +138,20 @@ class ClearMamba2:
                              torch.zeros(rows, s.conv_kernel - 1, s.conv_dim, dtype=self.dtype, device=self.device)))
         return out
 
-    def _final(self, hidden):
-        return hidden * torch.rsqrt(hidden.square().mean(-1, keepdim=True) + self.norm_eps) * self.norm_w
+    def _run(self, hidden, states, mixer) -> tuple:
+        """Residual stream [.., d_model] -> (final normed hidden, states), both of 32 bits."""
+        hidden, update, out = hidden.float(), None, []
+        for i, lay in enumerate(self.layers):
+            w, eps = lay.weights["block_norm_w"], lay.shape.eps_block
+            if update is None:
+                normed = clear.rms_norm(hidden, w, eps=eps, dtype=self.dtype)
+            else:
+                normed, hidden = clear.add_norm(hidden, update, w, eps=eps)
+            update, state = lay(normed, None if states is None else states[i], mixer)
+            out.append(state)
+        if update is None:
+            return clear.rms_norm(hidden, self.norm_w, eps=self.norm_eps), out
+        return clear.add_norm(hidden, update.float(), self.norm_w, eps=self.norm_eps).normed, out
 
     def forward(self, embeddings, states=None, *, cu_seqlens=None) -> tuple:
         """Whole sequences [sequences, tokens, d_model] float32, or packed [tokens, d_model] with cu_seqlens,
@@ -124,11 +165,7 @@ class ClearMamba2:
                                     return_state=True)
             return y, State(ssm, last)
 
-        hidden, out = embeddings, []
-        for i, lay in enumerate(self.layers):
-            hidden, state = lay(hidden, None if states is None else states[i], mixer)
-            out.append(state)
-        return self._final(hidden), out
+        return self._run(embeddings, states, mixer)
 
     @staticmethod
     def _scan_inputs(lay, conv, write, log_decay):
@@ -145,25 +182,55 @@ class ClearMamba2:
                                slots=slots)
             return y, state
 
-        hidden = embeddings
-        for lay, state in zip(self.layers, states):
-            hidden, _ = lay(hidden, state, mixer)
-        return self._final(hidden)
+        return self._run(embeddings, states, mixer)[0]
 
     def logits(self, hidden):
         if self.head is None:
             raise ValueError("the payload has no client head")
-        out = hidden.to(self.dtype) @ self.head.t()
-        return out if self.head_bias is None else (out.float() + self.head_bias).to(self.dtype)
+        return _project(hidden.to(self.dtype), self.head, self.head_bias)
 
     def score(self, hidden, targets, top: int = 0) -> clear.TokenLogprobs:
         """Log probabilities of target tokens, entropies and likeliest tokens at each hidden vector."""
         return clear.token_logprobs(self.logits(hidden), targets, top=top)
 
+    def embed(self, ids):
+        """Embeddings of token ids; those below 0 count from the table's end."""
+        return clear.embed(self.embedding, torch.where(ids < 0, ids + self.embedding.shape[0], ids))
+
+    @torch.no_grad()
+    def beam_search(self, ids, steps: int, *, beams: int = 4, end: Optional[int] = None, cu_seqlens=None) -> BeamResult:
+        """The `beams` (at most 32) continuations of `steps` tokens of each prompt that a beam search finds.
+
+        ids [requests, tokens], or packed [tokens] with cu_seqlens, each prompt one token or more.  A beam that
+        has taken the token `end` goes on with it at no cost.  The score is the sum of the tokens' log
+        probabilities."""
+        if self.head is None:
+            raise ValueError("the payload has no client head")
+        if steps < 1 or ids.shape[-1] < 1:
+            raise ValueError("steps must be 1 or more, and so must a prompt's tokens")
+        hidden, states = self.forward(self.embed(ids), cu_seqlens=cu_seqlens)
+        last = hidden[:, -1] if cu_seqlens is None else hidden[cu_seqlens[1:].long() - 1]
+        requests = last.shape[0]
+        score, parent, token = clear.beam_select(self.logits(last).unsqueeze(1), last.new_zeros(requests, 1), beams)
+        states = [State(s.ssm.repeat_interleave(beams, 0), s.conv.repeat_interleave(beams, 0)) for s in states]
+        held = [t for s in states for t in (s.ssm, s.conv)]
+        tokens = token.long().unsqueeze(-1)
+        finished = None if end is None else token == end
+        for _ in range(steps - 1):
+            hidden = self.step(self.embed(tokens[..., -1].reshape(-1)), states)
+            score, parent, token = clear.beam_select(self.logits(hidden).unflatten(0, (requests, beams)), score,
+                                                     finished=finished, end=end)
+            clear.reorder_states(held, parent)
+            parent, token = parent.long(), token.long()
+            tokens = torch.cat([tokens.gather(1, parent.unsqueeze(-1).expand(tokens.shape)), token.unsqueeze(-1)], -1)
+            if end is not None:
+                finished = token == end  # a finished beam's only token is `end`
+        return BeamResult(tokens, score)
+
     def loss(self, ids, *, cu_seqlens=None):
         """Mean negative log probability of each token's successor; ids [sequences, tokens], or packed, where
         tokens outside of every sequence take no part."""
-        hidden, _ = self.forward(self.embedding[ids], cu_seqlens=cu_seqlens)
+        hidden, _ = self.forward(self.embed(ids), cu_seqlens=cu_seqlens)
         targets = torch.cat([ids[..., 1:], torch.full_like(ids[..., :1], -1)], dim=-1)
         if cu_seqlens is not None:  # neither a sequence's last token nor one outside of all has a successor
             begins, ends = cu_seqlens[:-1].long(), cu_seqlens[1:].long()
@@ -180,8 +247,11 @@ def layer_states(states, row: int = 0) -> list:
 
 
 def run(chain: ChainPayload, *, prompt_tokens: Optional[int] = None, dtype=torch.float32, top: int = 5,
-        states_file: Optional[str] = None) -> dict:
-    model = ClearMamba2(chain, dtype)
+        states_file: Optional[str] = None, int8: bool = False, beams: int = 0) -> dict:
+    model = ClearMamba2(chain, dtype, int8=int8)
+    if beams and chain.autoregressive is None:
+        raise ValueError("a beam search needs the payload's client head and prompt")
+    tolerance = INT8_TOLERANCE if int8 else TOLERANCE[dtype]
     tokens = torch.as_tensor(chain.input_embeddings, dtype=torch.float32, device=model.device)
     n = tokens.shape[0]
     k = max(n - 1, 1) if prompt_tokens is None else prompt_tokens
@@ -204,15 +274,22 @@ def run(chain: ChainPayload, *, prompt_tokens: Optional[int] = None, dtype=torch
         report = {"format": "fhemamba-m2-clear-result-v1", "dtype": str(dtype).replace("torch.", ""),
                   "layers": len(model.layers), "prompt_tokens": k, "step_tokens": n - k, "seconds_prompt": prompt_s,
                   "seconds_per_step": step_s / (n - k) if n > k else None,
-                  "relative_errors": [float(e) for e in errors], "tolerance": TOLERANCE[dtype],
-                  "passed": bool(np.all(errors <= TOLERANCE[dtype]))}
+                  "relative_errors": [float(e) for e in errors], "tolerance": tolerance,
+                  "passed": bool(np.all(errors <= tolerance))}
+        if int8:
+            report["int8"] = True
         if model.head is not None:
             greedy = model.logits(final).argmax(-1)
-            scored = model.score(final, greedy, min(top, model.head.shape[0], clear.MAX_TOP))
+            scored = model.score(final, greedy, min(top, chain.autoregressive.vocab, clear.MAX_TOP))
             report["head"] = {"greedy": greedy.tolist(), "logprob": scored.logprob.tolist(),
                               "entropy": scored.entropy.tolist()}
             if scored.top_index is not None:
                 report["head"].update(top_index=scored.top_index.tolist(), top_logprob=scored.top_logprob.tolist())
+        if beams:
+            ar = chain.autoregressive
+            found = model.beam_search(torch.as_tensor([ar.prompt_ids], device=model.device), ar.generate_tokens,
+                                      beams=beams)
+            report["beams"] = {"tokens": found.tokens[0].tolist(), "score": found.score[0].tolist()}
         if states_file:
             arrays = {}
             for i, s in enumerate(layer_states(states)):
@@ -228,11 +305,14 @@ def main(argv=None) -> int:
     ap.add_argument("result")
     ap.add_argument("--prompt-tokens", type=int, default=None)
     ap.add_argument("--dtype", choices=("float32", "bfloat16"), default="float32")
+    ap.add_argument("--int8", action="store_true", help="projections and head in 8-bit integers")
     ap.add_argument("--top", type=int, default=5)
+    ap.add_argument("--beams", type=int, default=0, help="continuations of the payload's prompt by a beam search")
     ap.add_argument("--states", default=None)
     args = ap.parse_args(argv)
     report = run(read_chain_payload(args.payload), prompt_tokens=args.prompt_tokens,
-                 dtype=getattr(torch, args.dtype), top=args.top, states_file=args.states)
+                 dtype=getattr(torch, args.dtype), top=args.top, states_file=args.states, int8=args.int8,
+                 beams=args.beams)
     with open(args.result, "w") as f:
         json.dump(report, f, indent=1)
     print(json.dumps({k: v for k, v in report.items() if k != "head"}))
