@@ -124,7 +124,7 @@ int channels_of(int64_t channels, int64_t most, const char* msg) {
 }
 
 int64_t rows_of(int64_t rows) {
-  need(rows >= 0 && rows <= (1 << 24), "rows must be 0 .. 2^24");
+  need(rows >= 0 && rows <= INT32_MAX, "rows must be 0 .. 2^31 - 1");
   return rows;
 }
 

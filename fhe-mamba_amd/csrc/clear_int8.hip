@@ -79,21 +79,25 @@ __device__ __forceinline__ float round_row(const T* x, int channels, int lane, i
   for (int k = 0; k < PER; ++k) {
     const int c = (k * LANES + lane) * 4;
     if (c >= pitch) continue;
-    float r[4];
-    bool near = !plain;
+    // 1.5 2^23 + r in 32 bits rounds to an integer as the quotient would be rounded,
+    // and holds it in its low byte
+    float off = 0.0f;
+    uint32_t t[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      r[i] = rintf(v[k][i] * inverse);
-      near |= fabsf(v[k][i] * inverse - r[i]) > 0.4998f;
+      const float sum = __builtin_fmaf(v[k][i], inverse, 0x1.8p23f);
+      t[i] = __builtin_bit_cast(uint32_t, sum);
+      off = fmaxf(off, fabsf(__builtin_fmaf(v[k][i], inverse, 0x1.8p23f - sum)));
     }
-    if (near) {
+    uint32_t bytes = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400) | __builtin_amdgcn_perm(t[3], t[2], 0x04000c0c);
+    if (!plain || off > 0.4998f) {
+      bytes = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        r[i] = some ? fminf(fmaxf(rintf(v[k][i] / scale), -127.0f), 127.0f) : 0.0f;
+      for (int i = 0; i < 4; ++i) {
+        const float r = some ? fminf(fmaxf(rintf(v[k][i] / scale), -127.0f), 127.0f) : 0.0f;
+        bytes |= (uint32_t)((int)r & 255) << 8 * i;
+      }
     }
-    uint32_t bytes = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bytes |= (uint32_t)((int)r[i] & 255) << 8 * i;
     if (c + 4 <= pitch) {
       __builtin_memcpy(q + c, &bytes, 4);
     } else {
@@ -124,18 +128,21 @@ __global__ __launch_bounds__(threads_of(W)) void k_quantize(const T* x, int64_t 
 }
 
 void quantize(const Quantize& z, int8_t* values, int64_t pitch, float* scale, hipStream_t stream) {
-  if (!z.rows) return;
-  auto run = [&](auto zero) {
+  constexpr int64_t MOST = 1 << 20;  // rows of a launch, which has fewer than 2^32 threads
+  auto run = [&](auto zero, int64_t first) {
     using T = decltype(zero);
+    const int64_t rows = std::min(z.rows - first, MOST);
     by_shape((int)pitch, [&](auto w, auto per, auto) {
       const int at = threads_of(w()) / (64 * w());
-      k_quantize<T, w(), per()><<<(uint32_t)((z.rows + at - 1) / at), threads_of(w()), 0, stream>>>(
-          (const T*)z.x.p, z.x.row, z.rows, z.channels, values, pitch, scale);
+      k_quantize<T, w(), per()><<<(uint32_t)((rows + at - 1) / at), threads_of(w()), 0, stream>>>(
+          (const T*)z.x.p + first * z.x.row, z.x.row, rows, z.channels, values + first * pitch, pitch, scale + first);
     });
   };
-  if (z.dtype == BF16) run(bf16{});
-  else run(float{});
-  hip_check(hipGetLastError(), "rounding of rows");
+  for (int64_t first = 0; first < z.rows; first += MOST) {
+    if (z.dtype == BF16) run(bf16{}, first);
+    else run(float{}, first);
+    hip_check(hipGetLastError(), "rounding of rows");
+  }
 }
 
 // ----------------------------------------------------------------- products
@@ -184,8 +191,8 @@ __device__ __forceinline__ void put_outputs(const ProductArgs& p, int64_t m, int
 }
 
 // The fewest rows, of at most 1536 inputs: every workgroup rounds them itself, which
-// saves a launch, while its weights are on their way.  16 outputs a workgroup, a part
-// of the summed index a wavefront.
+// saves a launch, while its weights are on their way.  A wavefront has 16 outputs, and
+// all of their weights in its registers.
 constexpr int FEWEST = 8;
 
 template <class O, int PER, bool WIDE>
@@ -193,14 +200,13 @@ __global__ __launch_bounds__(256) void k_fewest(ProductArgs p, const O* x, int64
   constexpr int WIDTH = PER * 256, PITCH = WIDTH + 16;  // rows begin in banks four apart
   __shared__ alignas(16) int8_t rows[FEWEST * PITCH];
   __shared__ float scales[FEWEST];
-  __shared__ i32x4 lds[3][64];
   const int wave = threadIdx.x >> 6, lane = lane_id(), q = lane >> 4, l = lane & 15;
-  const int n0 = blockIdx.x * 16, count = (int)p.rows;
+  const int n0 = (blockIdx.x * 4 + wave) * 16, count = (int)p.rows;
   const int8_t* w = p.weight + (int64_t)min(n0 + l, p.outputs - 1) * p.inputs;
-  i32x4 a[PER];
+  i32x4 a[4 * PER];
 #pragma unroll
-  for (int s = 0; s < PER; ++s) {
-    const int k = (4 * s + wave) * 64 + 16 * q;
+  for (int s = 0; s < 4 * PER; ++s) {
+    const int k = 64 * s + 16 * q;
     a[s] = k < p.inputs ? weight16<WIDE>(w, k, p.inputs) : i32x4{};
   }
   for (int r = wave; r < count; r += 4) {
@@ -209,19 +215,14 @@ __global__ __launch_bounds__(256) void k_fewest(ProductArgs p, const O* x, int64
     if (lane == 0) scales[r] = scale;
   }
   __syncthreads();
-  i32x4 sum{};
+  i32x4 sum[2] = {};
   const int8_t* row = rows + min(l, count - 1) * PITCH;
 #pragma unroll
-  for (int s = 0; s < PER; ++s) {
-    const i32x4 b = *reinterpret_cast<const i32x4*>(row + (4 * s + wave) * 64 + 16 * q);
-    sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], b, sum, 0, 0, 0);
+  for (int s = 0; s < 4 * PER; ++s) {
+    const i32x4 b = *reinterpret_cast<const i32x4*>(row + 64 * s + 16 * q);
+    sum[s % 2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], b, sum[s % 2], 0, 0, 0);
   }
-  if (wave) lds[wave - 1][lane] = sum;
-  __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int o = 0; o < 3; ++o) sum += lds[o][lane];
-  if (l < count) put_outputs<O>(p, l, n0 + 4 * q, sum, scales[l]);
+  if (l < count) put_outputs<O>(p, l, n0 + 4 * q, sum[0] + sum[1], scales[l]);
 }
 
 // Few rows: a workgroup has 16 outputs and MT times 16 rows, its four wavefronts
@@ -539,10 +540,10 @@ int64_t tiles_of(int64_t rows, int64_t outputs, int tile) {
 }
 
 // In us, here and with rows rounded by a launch of their own: 768 inputs and 3352
-// outputs 4.1 and 6.0 for one row, 5.3 and 6.8 for 8, 6.5 and 6.7 for 12; 50280 outputs
-// 10.7 and 13.2 for one, 12.9 and 13.1 for 4, 16.5 and 13.0 for 8.
+// outputs 4.7 and 6.1 for one row, 6.0 and 6.5 for 8, 7.4 and 6.7 for 12; 50280 outputs
+// 9.8 and 13.3 for one, 11.7 and 13.4 for 8.
 bool is_fewest(const Int8& p) {
-  return p.rows <= (p.outputs <= 16384 ? FEWEST : 4) && rows_at_once(p.inputs) > 1;
+  return p.rows <= FEWEST && rows_at_once(p.inputs) > 1;
 }
 
 }  // namespace
@@ -576,7 +577,7 @@ void int8_linear(const Int8& p, void* y, void* workspace, hipStream_t stream) {
       using O = decltype(zero);
       by_shape(p.inputs, [&](auto w, auto per, auto) {
         if constexpr (w() == 1) {
-          const uint32_t grid = (uint32_t)((p.outputs + 15) / 16);
+          const uint32_t grid = (uint32_t)((p.outputs + 63) / 64);
           if (wide) k_fewest<O, per(), true><<<grid, 256, 0, stream>>>(a, (const O*)p.x.p, p.x.row);
           else k_fewest<O, per(), false><<<grid, 256, 0, stream>>>(a, (const O*)p.x.p, p.x.row);
         }

@@ -34,7 +34,7 @@ def norm(**kw):
 @pytest.mark.parametrize("kw,match", [
     ({"dtype": 2}, "dtype"), ({"out": 3}, "dtype"), ({"dtype": 1, "out": 0}, "out_dtype"), ({"groups": 0}, "groups"),
     ({"groups": 3}, "groups"), ({"eps": -1.0}, "eps"), ({"eps": math.nan}, "eps"), ({"eps": math.inf}, "eps"),
-    ({"rows": -1}, "rows"), ({"rows": 2 ** 24 + 1}, "rows"), ({"channels": 0}, "channels"),
+    ({"rows": -1}, "rows"), ({"rows": 2 ** 31}, "rows"), ({"channels": 0}, "channels"),
     ({"channels": 32769}, "32768"), ({"channels": 2 ** 20 + 2, "groups": 2 ** 10 + 2}, "channels"), ({"x": 0}, "null"),
     ({"x": 4097, "dtype": 1, "out": 1}, "aligned"), ({"x_row": -8}, "negative"), ({"gate": 4098}, "aligned"),
     ({"weight": 0}, "null weight"), ({"weight": 2}, "aligned"),
@@ -75,7 +75,7 @@ def add_norm(**kw):
 
 
 @pytest.mark.parametrize("kw,match", [
-    ({"dtype": 1, "out": 0}, "out_dtype"), ({"eps": -1.0}, "eps"), ({"rows": 2 ** 25}, "rows"),
+    ({"dtype": 1, "out": 0}, "out_dtype"), ({"eps": -1.0}, "eps"), ({"rows": 2 ** 31}, "rows"),
     ({"channels": 32769}, "channels"), ({"hidden": 0}, "null"), ({"update": 0}, "null"), ({"update": 4097}, "aligned"),
     ({"update_row": -1}, "negative"), ({"weight": 0}, "null weight"), ({"scale": 6}, "aligned"),
 ])
@@ -121,7 +121,7 @@ def int8(**kw):
 
 
 @pytest.mark.parametrize("kw,match", [
-    ({"dtype": 2}, "dtype"), ({"rows": 2 ** 24 + 1}, "rows"), ({"inputs": 0}, "inputs"), ({"inputs": 40000}, "inputs"),
+    ({"dtype": 2}, "dtype"), ({"rows": 2 ** 31}, "rows"), ({"inputs": 0}, "inputs"), ({"inputs": 40000}, "inputs"),
     ({"outputs": 0}, "outputs"), ({"outputs": 2 ** 25}, "outputs"), ({"rows": 2 ** 24, "outputs": 2 ** 12}, "too many"),
     ({"x": 0}, "null"), ({"x": 4097}, "aligned"), ({"weight": 0}, "null weight"), ({"scale": 0}, "null weight"),
     ({"scale": 6}, "aligned"), ({"bias": 6}, "aligned"),

@@ -123,6 +123,21 @@ def test_views_and_default_width():
         assert torch.equal(a, b)
 
 
+def test_logits_past_32_bits():
+    from fhemamba_amd import clear
+
+    requests, beams, vocab = 1400, 32, 50280
+    logits = torch.zeros(requests, beams, vocab, dtype=BF, device="cuda")
+    scores = torch.full((requests, beams), -1.0, device="cuda")
+    some, own = make(8, 1, beams, vocab, BF)
+    logits[-1], scores[-1] = some[0].cuda(), own[0].cuda()
+    got, alone = clear.beam_select(logits, scores, 4), clear.beam_select(some.cuda(), own.cuda(), 4)
+    for a, b in zip(got, alone):
+        assert torch.equal(a[-1], b[0])
+    assert got.token[0].tolist() == [0, 1, 2, 3] and got.parent[0].tolist() == [0] * 4
+    assert bool((got.token[:-1] == got.token[0]).all())
+
+
 def test_refusals():
     from fhemamba_amd import clear
 

@@ -117,6 +117,28 @@ def test_largest_sums(rows):
     assert float((got.double() - want).abs().max()) <= 4 * 2.0 ** -24 * want
 
 
+def test_results_past_32_bits():
+    """2.5e9 results; and more rows than a launch rounds."""
+    from fhemamba_amd import clear
+
+    gen = torch.Generator().manual_seed(3)
+    rows, outputs = 50000, 50280
+    x, w = rows_of(gen, 8, 64, BF), torch.randint(-127, 128, (outputs, 64), generator=gen, dtype=torch.int8)
+    wide = torch.zeros(rows, 64, dtype=BF, device="cuda")
+    picked = [0, 1, 42700, 42711, 42712, 49151, 49998, 49999]
+    wide[picked] = x.cuda()
+    ws = torch.rand(outputs, generator=gen)
+    got = clear.int8_linear(wide, w.cuda(), ws.cuda())
+    want = L.int8_linear(x, w, ws, None)
+    assert float((got[picked].cpu().double() - want).norm()) <= R.BF16 * float(want.norm())
+    assert not bool(got[2:42700].any()) and not bool(got[49152:49998].any())
+    rows = (1 << 20) + 5
+    many = torch.arange(rows, device="cuda").float()[:, None].expand(rows, 3)
+    q = clear.quantize_rows(many)
+    assert bool((q.values[1:] == 127).all()) and not bool(q.values[0].any())
+    assert torch.equal(q.scale, torch.arange(rows).div(127.0).cuda())
+
+
 def test_views_axes_and_alignment():
     from fhemamba_amd import clear
 

@@ -210,9 +210,20 @@ def test_offsets_past_32_bits():
     some = n(gen, 4, channels, dtype=BF)
     x[picked] = some.cuda()
     w = n(gen, channels)
-    y = clear.rms_norm(x, w.cuda())
-    check(y[picked], L.norm(some.double(), w.double(), None, 1, 1e-5), BF)
+    leaf = x.requires_grad_(True)
+    y = clear.rms_norm(leaf, w.cuda())
+    ref = some.double().requires_grad_(True)
+    want = L.norm(ref, w.double(), None, 1, 1e-5)
+    check(y[picked], want, BF)
     assert not bool(y[1:65535].any())
+    dn = n(gen, 4, channels, dtype=BF)
+    (grad,) = torch.autograd.grad(want, ref, dn.double())
+    dy = torch.zeros_like(x)
+    dy[picked] = dn.cuda()
+    (back,) = torch.autograd.grad(y, leaf, dy)
+    # the terms are about as large as the gradient: rows of 32768 are hardly along it
+    check(back[picked], grad, BF, grad)
+    assert not bool(back[1:65535].any())
 
 
 def test_differences():
