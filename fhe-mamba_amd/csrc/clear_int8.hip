@@ -606,17 +606,17 @@ void int8_linear(const Int8& p, void* y, void* workspace, hipStream_t stream) {
     });
   } else {
     // workgroups: as many as there are tiles, but no more than run at once
-    auto tiles = [&](int tile, int at_once) {
-      a.row_tiles = (int)((p.rows + tile - 1) / tile);
-      a.out_tiles = (p.outputs + tile - 1) / tile;
+    auto tiles = [&](int rows, int outs, int at_once) {
+      a.row_tiles = (int)((p.rows + rows - 1) / rows);
+      a.out_tiles = (p.outputs + outs - 1) / outs;
       const int64_t share = ((int64_t)a.row_tiles * a.out_tiles + 7) / 8;
       return (uint32_t)(8 * std::min<int64_t>(share, at_once / 8));
     };
     by_type([&](auto zero) {
       using O = decltype(zero);
-      if (!wide) k_many_narrow<O><<<tiles(128, 1 << 30), 256, 0, stream>>>(a);
-      else if (tiles_of(p.rows, p.outputs, 256) >= 256) k_many<O, 2, 4, 8><<<tiles(256, 256), 512, 0, stream>>>(a);
-      else k_many<O, 2, 2, 4><<<tiles(128, 512), 256, 0, stream>>>(a);
+      if (!wide) k_many_narrow<O><<<tiles(128, 128, 1 << 30), 256, 0, stream>>>(a);
+      else if (tiles_of(p.rows, p.outputs, 256) >= 256) k_many<O, 2, 4, 8><<<tiles(256, 256, 256), 512, 0, stream>>>(a);
+      else k_many<O, 2, 2, 4><<<tiles(128, 128, 512), 256, 0, stream>>>(a);
     });
   }
   hip_check(hipGetLastError(), "8-bit product");

@@ -32,6 +32,7 @@ from __future__ import annotations
 import ctypes
 import struct
 from itertools import chain, repeat
+from operator import attrgetter
 from typing import NamedTuple, Optional
 
 import torch
@@ -69,6 +70,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _device_of, _size_of, _is_contiguous = torch.Tensor.get_device, torch.Tensor.size, torch.Tensor.is_contiguous
+_requires_grad = attrgetter("requires_grad")
 
 
 def _run(entry, like: torch.Tensor, *args) -> None:
@@ -894,8 +896,9 @@ def reorder_states(states, parent, *, slots=None) -> None:
         raise ValueError(f"{requests * beams} beams and {cache} rows of the states")
     if not all(map(_is_contiguous, states)):
         raise ValueError("states must be contiguous: they are updated in place")
-    if _wants_grad(*states):
-        raise ValueError("reorder_states has no gradient: call it under torch.no_grad()")
+    if getattr(_forward_ad, "_current_level", 0) >= 0 or any(map(_requires_grad, states)):
+        if _wants_grad(*states):
+            raise ValueError("reorder_states has no gradient: call it under torch.no_grad()")
     packed = struct.pack(f"={2 * len(states)}q",
                          *chain.from_iterable((t.data_ptr(), t.nbytes // cache) for t in states))
     parent = parent.contiguous()
