@@ -36,21 +36,23 @@ __global__ __launch_bounds__(256) void k_embed(Embed e, T* y) {
       continue;
     }
     const T* row = (const T*)e.weight + id * e.weight_row;
+    if (e.channels < VEC) {
+      const int c = lane_id();
+      if (c < e.channels) out[c] = (T)((float)row[c] * e.scale);
+      continue;
+    }
     for (int c = lane_id() * VEC; c < e.channels; c += 64 * VEC) {
-      if (c + VEC <= e.channels) {
-        union {
-          u32x4 w;
-          T v[VEC];
-        } u;
-        __builtin_memcpy(&u.w, row + c, 16);
-        if (e.scale != 1.0f) {
+      const int at = min(c, e.channels - VEC);  // the last piece over the end of the one before
+      union {
+        u32x4 w;
+        T v[VEC];
+      } u;
+      __builtin_memcpy(&u.w, row + at, 16);
+      if (e.scale != 1.0f) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) u.v[i] = (T)((float)u.v[i] * e.scale);
-        }
-        __builtin_memcpy(out + c, &u.w, 16);
-      } else {
-        for (int i = c; i < e.channels; ++i) out[i] = (T)((float)row[i] * e.scale);
+        for (int i = 0; i < VEC; ++i) u.v[i] = (T)((float)u.v[i] * e.scale);
       }
+      __builtin_memcpy(out + at, &u.w, 16);
     }
   }
 }
@@ -170,7 +172,7 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 
 // The sum of dy over `token[0 .. count)`, for the channels that `first` and up hold
 // in this wavefront's lanes.  count and first are the same in all lanes.
-template <class T>
+template <class T, int COVER>
 __device__ __forceinline__ void add_rows(const SumArgs& a, const int* token, int count, int first,
                                          f32x4 (&sum)[COLUMNS]) {
   const int lane = lane_id();
@@ -185,11 +187,11 @@ __device__ __forceinline__ void add_rows(const SumArgs& a, const int* token, int
       for (int j = 0; j < LOADS; ++j) {
         // past the last token the last one again, times nothing
         const int t = __builtin_amdgcn_readlane(mine, i + j < some ? i + j : some - 1);
-        const T* row = (const T*)a.dy + (int64_t)t * a.dy_row + first;
+        const T* row = (const T*)a.dy + (int64_t)t * a.dy_row;
 #pragma unroll
         for (int k = 0; k < COLUMNS; ++k) {
-          const int c = (k * 64 + lane) * 4;
-          v[j][k] = first + k * 256 < a.channels ? get4(row + c, a.channels - first - c) : f32x4{};
+          const int c = first + k * 256;
+          v[j][k] = c < a.channels ? Piece<COVER>(c + 4 * lane, a.channels).get(row) : f32x4{};
         }
       }
 #pragma unroll
@@ -202,7 +204,7 @@ __device__ __forceinline__ void add_rows(const SumArgs& a, const int* token, int
   }
 }
 
-template <class T>
+template <class T, int COVER>
 __global__ __launch_bounds__(256) void k_sums(SumArgs a) {
   const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
   if ((int)blockIdx.x < a.pieces) {
@@ -219,11 +221,11 @@ __global__ __launch_bounds__(256) void k_sums(SumArgs a) {
       float* out = a.parts + ((int64_t)blockIdx.x * 2 + side) * a.channels;
       for (int c0 = wave * 256 * COLUMNS; c0 < a.channels; c0 += 4 * 256 * COLUMNS) {
         f32x4 sum[COLUMNS];
-        add_rows<T>(a, a.o.token + f, uniform((int)(t - f)), c0, sum);
+        add_rows<T, COVER>(a, a.o.token + f, uniform((int)(t - f)), c0, sum);
 #pragma unroll
         for (int k = 0; k < COLUMNS; ++k) {
-          const int c = c0 + (k * 64 + lane) * 4;
-          if (c < a.channels) put4(out + c, sum[k], a.channels - c);
+          const int c = c0 + k * 256;
+          if (c < a.channels) Piece<COVER>(c + 4 * lane, a.channels).put(out, sum[k]);
         }
       }
     }
@@ -236,11 +238,11 @@ __global__ __launch_bounds__(256) void k_sums(SumArgs a) {
   T* out = (T*)a.dweight + row * a.channels;
   for (int c0 = 0; c0 < a.channels; c0 += 256 * COLUMNS) {
     f32x4 sum[COLUMNS];
-    add_rows<T>(a, a.o.token + from, count, c0, sum);
+    add_rows<T, COVER>(a, a.o.token + from, count, c0, sum);
 #pragma unroll
     for (int k = 0; k < COLUMNS; ++k) {
-      const int c = c0 + (k * 64 + lane) * 4;
-      if (c < a.channels) put4(out + c, sum[k] * a.scale, a.channels - c);
+      const int c = c0 + k * 256;
+      if (c < a.channels) Piece<COVER>(c + 4 * lane, a.channels).put(out, sum[k] * a.scale);
     }
   }
 }
@@ -319,8 +321,14 @@ void embed_backward(const Embed& e, const Rows& dy, void* dweight, void* workspa
   k_sort<<<(uint32_t)((e.vocab + SPAN - 1) / SPAN), 64 * SORT_WAVES, 0, stream>>>(e.ids, e.tokens, e.vocab, a.o);
   hip_check(hipGetLastError(), "order of tokens");
   const uint32_t grid = (uint32_t)(a.pieces + (e.vocab + 3) / 4);
-  if (e.dtype == BF16) k_sums<bf16><<<grid, 256, 0, stream>>>(a);
-  else k_sums<float><<<grid, 256, 0, stream>>>(a);
+  auto sums = [&](auto zero) {
+    using T = decltype(zero);
+    if (e.channels % 256 == 0) k_sums<T, WHOLE><<<grid, 256, 0, stream>>>(a);
+    else if (e.channels >= 4) k_sums<T, MOVED><<<grid, 256, 0, stream>>>(a);
+    else k_sums<T, SHORT><<<grid, 256, 0, stream>>>(a);
+  };
+  if (e.dtype == BF16) sums(bf16{});
+  else sums(float{});
   hip_check(hipGetLastError(), "embedding gradient");
   if (!a.pieces) return;
   if (e.dtype == BF16) k_join<bf16><<<a.pieces, 64 * JOIN_WAVES, 0, stream>>>(a);

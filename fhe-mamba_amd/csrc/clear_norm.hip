@@ -62,9 +62,8 @@ __device__ __forceinline__ void row_sums(float (&s)[COUNT], float (*lds)[2][COUN
   }
 }
 
-// W wavefronts a row, PER pieces of four channels a lane; FULL: they are all of
-// the row.  blockIdx.y is the group.
-template <class A, class O, int MODE, int W, int PER, bool FULL>
+// W wavefronts a row, PER pieces of four channels a lane.  blockIdx.y is the group.
+template <class A, class O, int MODE, int W, int PER, int COVER>
 __global__ __launch_bounds__(threads_of(W)) void k_norm(NormArgs p) {
   using B = std::conditional_t<MODE == ADDED, O, A>;
   constexpr int LANES = 64 * W, ROWS = threads_of(W) / LANES;
@@ -72,14 +71,13 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm(NormArgs p) {
   const int lane = threadIdx.x % LANES;
   const int64_t first = (int64_t)blockIdx.y * p.channels;
   const float mean = 1.0f / (float)p.channels;
-  int count[PER];
+  Piece<COVER> piece[PER];
   f32x4 w[PER], scale[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int c = (k * LANES + lane) * 4;
-    count[k] = FULL ? 4 : p.channels - c;
-    w[k] = get4(p.weight + first + c, count[k]);
-    if constexpr (MODE == ADDED) scale[k] = p.scale ? get4(p.scale + first + c, count[k]) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+    piece[k] = Piece<COVER>((k * LANES + lane) * 4, p.channels);
+    w[k] = piece[k].get(p.weight + first);
+    if constexpr (MODE == ADDED) scale[k] = p.scale ? piece[k].get(p.scale + first) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
   }
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < p.rows;
@@ -89,32 +87,30 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm(NormArgs p) {
     f32x4 v[PER], other[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int c = (k * LANES + lane) * 4;
-      v[k] = get4(a + c, count[k]);
-      if constexpr (MODE != PLAIN) other[k] = get4(b + c, count[k]);
+      v[k] = piece[k].get(a);
+      if constexpr (MODE != PLAIN) other[k] = piece[k].get(b);
     }
     float s[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       if constexpr (MODE == ADDED) {
         v[k] += scale[k] * other[k];
-        put4((A*)p.sum + row * p.all + first + (k * LANES + lane) * 4, v[k], count[k]);
+        piece[k].put((A*)p.sum + row * p.all + first, v[k]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (MODE == GATED) v[k][i] *= other[k][i] * sigmoid(other[k][i]);
-        s[0] += v[k][i] * v[k][i];
+        s[0] += piece[k].mine(i, v[k][i] * v[k][i]);
       }
     }
     row_sums<W>(s, lds, turn ^= 1);
     const float r = rsqrtf(s[0] * mean + p.eps);
 #pragma unroll
-    for (int k = 0; k < PER; ++k)
-      put4((O*)p.y + row * p.all + first + (k * LANES + lane) * 4, v[k] * r * w[k], count[k]);
+    for (int k = 0; k < PER; ++k) piece[k].put((O*)p.y + row * p.all + first, v[k] * r * w[k]);
   }
 }
 
-template <class A, class O, int MODE, int W, int PER, bool FULL>
+template <class A, class O, int MODE, int W, int PER, int COVER>
 __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
   using B = std::conditional_t<MODE == ADDED || MODE == SUMMED, O, A>;
   constexpr int LANES = 64 * W, ROWS = threads_of(W) / LANES;
@@ -123,14 +119,13 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
   const int lane = threadIdx.x % LANES;
   const int64_t first = (int64_t)blockIdx.y * p.channels;
   const float mean = 1.0f / (float)p.channels;
-  int count[PER];
+  Piece<COVER> piece[PER];
   f32x4 w[PER], scale[PER], dw[PER], ds[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int c = (k * LANES + lane) * 4;
-    count[k] = FULL ? 4 : p.channels - c;
-    w[k] = get4(p.weight + first + c, count[k]);
-    if constexpr (MODE == ADDED) scale[k] = p.scale ? get4(p.scale + first + c, count[k]) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+    piece[k] = Piece<COVER>((k * LANES + lane) * 4, p.channels);
+    w[k] = piece[k].get(p.weight + first);
+    if constexpr (MODE == ADDED) scale[k] = p.scale ? piece[k].get(p.scale + first) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
     dw[k] = ds[k] = f32x4{};
   }
   int turn = 0;
@@ -142,10 +137,9 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
     f32x4 v[PER], other[PER], g[PER], act[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int c = (k * LANES + lane) * 4;
-      v[k] = get4(a + c, count[k]);
-      if constexpr (MODE == GATED || MODE == ADDED) other[k] = get4(b + c, count[k]);
-      g[k] = p.dy ? get4(dy + c, count[k]) : f32x4{};
+      v[k] = piece[k].get(a);
+      if constexpr (MODE == GATED || MODE == ADDED) other[k] = piece[k].get(b);
+      g[k] = p.dy ? piece[k].get(dy) : f32x4{};
     }
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -158,8 +152,8 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
           act[k][i] = other[k][i] * sigmoid(other[k][i]);
           t *= act[k][i];
         }
-        s[0] += t * t;
-        s[1] += t * g[k][i] * w[k][i];
+        s[0] += piece[k].mine(i, t * t);
+        s[1] += piece[k].mine(i, t * g[k][i] * w[k][i]);
       }
     }
     row_sums<W>(s, lds, turn ^= 1);
@@ -167,31 +161,30 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
     const float back = r * r * r * (s[1] * mean);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int c = (k * LANES + lane) * 4;
-      const int64_t at = row * p.all + first + c;
+      const int64_t at = row * p.all + first;
       f32x4 t = v[k];
       if constexpr (MODE == GATED) t *= act[k];
       f32x4 d = r * (g[k] * w[k]) - t * back;
       dw[k] += g[k] * (t * r);
       if constexpr (MODE == PLAIN) {
-        put4((A*)p.da + at, d, count[k]);
+        piece[k].put((A*)p.da + at, d);
       } else if constexpr (MODE == GATED) {
-        put4((A*)p.da + at, d * act[k], count[k]);
+        piece[k].put((A*)p.da + at, d * act[k]);
         f32x4 dz;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float sig = sigmoid(other[k][i]);
           dz[i] = d[i] * v[k][i] * (sig + act[k][i] * (1.0f - sig));
         }
-        put4((A*)p.db + at, dz, count[k]);
+        piece[k].put((A*)p.db + at, dz);
       } else {
-        if (p.dsum) d += get4((const A*)p.dsum + row * p.dsum_row + first + c, count[k]);
-        if (p.da) put4((A*)p.da + at, d, count[k]);
+        if (p.dsum) d += piece[k].get((const A*)p.dsum + row * p.dsum_row + first);
+        if (p.da) piece[k].put((A*)p.da + at, d);
         if constexpr (MODE == ADDED) {
           ds[k] += d * other[k];
           d *= scale[k];
         }
-        if (p.db) put4((B*)p.db + at, d, count[k]);
+        if (p.db) piece[k].put((B*)p.db + at, d);
       }
     }
   }
@@ -213,7 +206,7 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
         for (int o = 0; o < ROWS - 1; ++o) t[k] += *reinterpret_cast<const f32x4*>(&totals[o][(k * 64 + lane) * 4]);
     }
 #pragma unroll
-    for (int k = 0; k < PER; ++k) put4(out + (k * LANES + lane) * 4, t[k], count[k]);
+    for (int k = 0; k < PER; ++k) piece[k].put(out, t[k]);
   };
   total(dw, p.parts);
   if constexpr (MODE == ADDED) {
@@ -269,8 +262,8 @@ void forward(const NormArgs& p, uint32_t dtype, uint32_t out, int groups, hipStr
   if (!p.rows) return;
   const dim3 grid(forward_grid(p.rows, p.channels), groups);
   by_type(dtype, out, [&](auto a, auto o) {
-    by_shape(p.channels, [&](auto w, auto per, auto full) {
-      k_norm<decltype(a), decltype(o), MODE, w(), per(), full()><<<grid, threads_of(w()), 0, stream>>>(p);
+    by_shape(p.channels, [&](auto w, auto per, auto cover) {
+      k_norm<decltype(a), decltype(o), MODE, w(), per(), cover()><<<grid, threads_of(w()), 0, stream>>>(p);
     });
   });
   hip_check(hipGetLastError(), "norm");
@@ -281,8 +274,8 @@ void backward(const NormArgs& p, uint32_t dtype, uint32_t out, int groups, float
               hipStream_t stream) {
   const int count = backward_grid(p.rows, p.channels);
   by_type(dtype, out, [&](auto a, auto o) {
-    by_shape(p.channels, [&](auto w, auto per, auto full) {
-      k_norm_back<decltype(a), decltype(o), MODE, w(), per(), full()>
+    by_shape(p.channels, [&](auto w, auto per, auto cover) {
+      k_norm_back<decltype(a), decltype(o), MODE, w(), per(), cover()>
           <<<dim3(count, groups), threads_of(w()), 0, stream>>>(p);
     });
   });

@@ -71,12 +71,38 @@ constexpr int MAX_ROW = 16 * 256 * 8;
 constexpr int threads_of(int w) { return w == 16 ? 1024 : 256; }
 inline int rows_at_once(int channels) { return channels <= 6 * 256 ? 4 : 1; }  // of a workgroup
 
-// f(W, PER, FULL) for rows of at most MAX_ROW; FULL: the pieces are all of the row.
+// How the pieces of the lanes cover a row: just so; with a last piece moved back to the
+// row's end, over elements of the piece before it; or a row shorter than a piece.
+enum Cover { WHOLE, MOVED, SHORT };
+
+// A lane's piece of four elements that begins at element c.
+template <int COVER>
+struct Piece {
+  int at, own;  // where it lies; how many of its elements are no other piece's: the last ones, or of a short row the first
+
+  __device__ __forceinline__ Piece(int c, int channels)
+      : at(COVER == MOVED ? min(c, channels - 4) : c), own(COVER == WHOLE ? 4 : max(0, min(4, channels - c))) {}
+  Piece() = default;
+
+  template <class T>
+  __device__ __forceinline__ f32x4 get(const T* row) const {
+    return get4(row + at, COVER == SHORT ? own : 4);
+  }
+  // A moved piece writes its neighbour's elements too: the same values from the same inputs.
+  template <class T>
+  __device__ __forceinline__ void put(T* row, f32x4 v) const {
+    if (COVER == WHOLE || own > 0) put4(row + at, v, COVER == SHORT ? own : 4);
+  }
+  // v where element i is the piece's own, else 0
+  __device__ __forceinline__ float mine(int i, float v) const { return COVER == MOVED && i < 4 - own ? 0.0f : v; }
+};
+
+// f(W, PER, COVER) for rows of at most MAX_ROW.
 template <class F>
 void by_shape(int channels, F&& f) {
   auto go = [&](auto w, auto per) {
-    if (channels == 256 * w() * per()) f(w, per, std::true_type{});
-    else f(w, per, std::false_type{});
+    if (channels == 256 * w() * per()) f(w, per, std::integral_constant<int, WHOLE>{});
+    else f(w, per, std::integral_constant<int, MOVED>{});
   };
   const int pieces = (channels + 255) / 256;  // of 64 lanes
   std::integral_constant<int, 1> one;
@@ -86,7 +112,8 @@ void by_shape(int channels, F&& f) {
   std::integral_constant<int, 6> six;
   std::integral_constant<int, 8> eight;
   std::integral_constant<int, 16> sixteen;
-  if (pieces <= 1) go(one, one);
+  if (channels < 4) f(one, one, std::integral_constant<int, SHORT>{});
+  else if (pieces <= 1) go(one, one);
   else if (pieces <= 2) go(one, two);
   else if (pieces <= 3) go(one, three);
   else if (pieces <= 4) go(one, four);
