@@ -477,6 +477,7 @@ int fhe_add_norm_backward(const fhe_add_norm_args* args, const fhe_add_norm_grad
                           size_t bytes, void* hip_stream) {
   return guard([&] {
     need(args && grads && grads->dweight, "null output");
+    need(!grads->dscale || args->scale, "a gradient of a scale that is not there");
     const bool whole = grads->sum && args->dtype == FHE_F32 && !args->scale;  // as add_norm_backward
     const clear::AddNorm n = to_add_norm(args, !whole);
     clear::AddNormGrads g{};

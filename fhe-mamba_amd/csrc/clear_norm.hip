@@ -280,7 +280,8 @@ void backward(const NormArgs& p, uint32_t dtype, uint32_t out, int groups, float
     });
   });
   hip_check(hipGetLastError(), "norm gradient");
-  k_norm_sum<<<dim3((p.all + SUM_COLUMNS - 1) / SUM_COLUMNS, p.scale ? 2 : 1), 1024, 0, stream>>>(p.parts, count, p.all, dweight, dscale);
+  const dim3 sums((p.all + SUM_COLUMNS - 1) / SUM_COLUMNS, p.scale ? 2 : 1);
+  k_norm_sum<<<sums, 1024, 0, stream>>>(p.parts, count, p.all, dweight, dscale);
   hip_check(hipGetLastError(), "norm gradient sums");
 }
 

@@ -78,7 +78,8 @@ enum Cover { WHOLE, MOVED, SHORT };
 // A lane's piece of four elements that begins at element c.
 template <int COVER>
 struct Piece {
-  int at, own;  // where it lies; how many of its elements are no other piece's: the last ones, or of a short row the first
+  int at;   // where it lies
+  int own;  // how many of its elements are no other piece's: the last ones, or of a short row the first
 
   __device__ __forceinline__ Piece(int c, int channels)
       : at(COVER == MOVED ? min(c, channels - 4) : c), own(COVER == WHOLE ? 4 : max(0, min(4, channels - c))) {}

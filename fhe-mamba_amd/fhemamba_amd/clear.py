@@ -10,9 +10,12 @@ the clear (the reference does it in PyTorch on the host, src/fhemamba/reference.
   causal_conv_step
   token_logprobs  log probabilities of given tokens, entropy and likeliest tokens, with gradients
   embed           embeddings of tokens, with the table's gradient
-  rms_norm, add_norm  norms with the gate or the residual before them, with gradients
-  quantize_rows, int8_linear  projections in 8-bit integers, for serving
-  beam_select, reorder_states  a step of a beam search, and its states
+  rms_norm        the norm with or without a gate before it, with gradients
+  add_norm        the residual and the next layer's norm, with gradients
+  quantize_rows   rows as 8-bit integers and a scale
+  int8_linear     projections in 8-bit integers, for serving
+  beam_select     the best continuations of a search's beams
+  reorder_states  their states follow them
 
 They take torch tensors on the GPU, run libfhecore's kernels on torch's current stream and return
 without waiting; inputs made on another stream need the usual synchronisation.  Activations are

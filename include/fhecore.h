@@ -540,7 +540,8 @@ int fhe_add_norm(const fhe_add_norm_args *args, void *sum, void *y,
 int fhe_add_norm_workspace(const fhe_add_norm_args *args, size_t *bytes);
 /* From dy and the gradient of sum (data NULL: zeros).  sum: the forward call's, or
  * NULL; where it serves (32 bits, no scale) hidden and update are not read.
- * dhidden and dupdate [rows][channels] and dscale [channels] may be NULL. */
+ * dhidden and dupdate [rows][channels] and dscale [channels] may be NULL; dscale
+ * is where there is no scale. */
 typedef struct {
   fhe_rows dy, dsum;
   const void *sum;

@@ -102,6 +102,9 @@ def test_add_norm_outputs():
             _lib.call("fhe_add_norm_backward", args, clear._ADD_NORM_GRADS.pack(*bad), 4096, size, 0)
     with pytest.raises(ValueError, match="too small"):
         _lib.call("fhe_add_norm_backward", args, clear._ADD_NORM_GRADS.pack(*ok), 4096, size - 1, 0)
+    ok[7] = 4096
+    with pytest.raises(ValueError, match="a scale that is not there"):
+        _lib.call("fhe_add_norm_backward", args, clear._ADD_NORM_GRADS.pack(*ok), 4096, size, 0)
 
 
 @pytest.mark.parametrize("kw,match", [({"dtype": 7}, "dtype"), ({"rows": -1}, "rows"), ({"channels": 0}, "channels"),
