@@ -76,13 +76,13 @@ __global__ __launch_bounds__(THREADS) void k_beam_parts(BeamArgs a) {
   float m = -INFINITY;
   double s = 0.0;
   Sixteen<T> x;
-  x.read(row, start, a.b.vocab);
+  x.template read<false>(row, start, a.b.vocab);
   for (int t = 0; t < a.tiles; ++t) {
     const int64_t base = start + (int64_t)t * TILE;
     if (base >= a.b.vocab) break;
     float v[16];
     x.widen(v);
-    if (t + 1 < a.tiles) x.read(row, base + TILE, a.b.vocab);  // in flight meanwhile
+    if (t + 1 < a.tiles) x.template read<false>(row, base + TILE, a.b.vocab);  // in flight meanwhile
     float most = m, sum = 0.0f;
     bool nan = false;
 #pragma unroll

@@ -10,7 +10,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int THREADS = 256, TILE = 16 * THREADS;  // logits of a workgroup at a time
 
 // Sixteen logits of a thread in a tile that begins at column `base` (it may be
-// negative; read fastest at a multiple of 16 bytes), as they lie in memory.  -inf outside of the
+// negative; ALIGNED: at a multiple of 16 bytes), as they lie in memory.  -inf outside of the
 // row.
 template <class T>
 struct Sixteen {
@@ -23,12 +23,14 @@ struct Sixteen {
   static __device__ __forceinline__ int64_t column(int64_t base, int j) {
     return base + (int64_t)(j / VEC) * THREADS * VEC + threadIdx.x * VEC + j % VEC;
   }
+  template <bool ALIGNED>
   __device__ __forceinline__ void read(const T* row, int64_t base, int64_t vocab) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int64_t c = column(base, p * VEC);
       if (c >= 0 && c + VEC <= vocab) {
-        __builtin_memcpy(&w[p], row + c, 16);
+        if constexpr (ALIGNED) w[p] = *reinterpret_cast<const u32x4*>(row + c);
+        else __builtin_memcpy(&w[p], row + c, 16);
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) e[p * VEC + i] = c + i >= 0 && c + i < vocab ? row[c + i] : (T)-INFINITY;

@@ -90,13 +90,13 @@ __global__ __launch_bounds__(THREADS) void k_row_parts(RowArgs a) {
   Stats st{-INFINITY, 0.0f, 0.0f};
   const int64_t start = (int64_t)split * a.tiles * TILE - lead;
   Sixteen<T> x;
-  x.read(row, start, a.l.vocab);
+  x.template read<true>(row, start, a.l.vocab);
   for (int t = 0; t < a.tiles; ++t) {
     const int64_t base = start + (int64_t)t * TILE;
     if (base >= a.l.vocab) break;
     float v[16];
     x.widen(v);
-    if (t + 1 < a.tiles) x.read(row, base + TILE, a.l.vocab);  // in flight meanwhile
+    if (t + 1 < a.tiles) x.template read<true>(row, base + TILE, a.l.vocab);  // in flight meanwhile
     st = add16(st, v);
     if constexpr (TOP) {
       const uint64_t key = set_key<T>(v, base, a.l.vocab);
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(THREADS) void k_row_back(BackArgs a) {
   const float gb = a.dentropy ? a.dentropy[row_i] : 0.0f;
   const bool none = peak == -INFINITY;
   Sixteen<T> x;
-  x.read(row, base, a.l.vocab);
+  x.template read<true>(row, base, a.l.vocab);
   float v[16];
   x.widen(v);
 #pragma unroll
