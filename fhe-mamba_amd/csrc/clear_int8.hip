@@ -50,6 +50,15 @@ constexpr int STEP = 128;  // bytes of a row at a time; rows of q are whole step
 int64_t pitch_of(int64_t inputs) { return (inputs + STEP - 1) / STEP * STEP; }
 
 // ----------------------------------------------------------------- rounding rows
+template <class T, int LANES, int PER>
+__device__ __forceinline__ void load_row(f32x4 (&v)[PER], const T* x, int channels, int lane) {
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int c = (k * LANES + lane) * 4;
+    v[k] = get4(x + c, channels - c);
+  }
+}
+
 // A row in registers as integers, to bytes c .. of q for c below `pitch`; its scale.
 // `all`: the largest of the lanes' numbers for the whole row.
 //
@@ -57,14 +66,11 @@ int64_t pitch_of(int64_t inputs) { return (inputs + STEP - 1) / STEP * STEP; }
 // the same integer unless the product lies that near to the middle of two: then, or
 // for a scale whose reciprocal is no good, the quotient itself is taken.  Dividing
 // each takes 30011 rows of 768 from 20 to 22 us.
-template <class T, int LANES, int PER, class All>
-__device__ __forceinline__ float round_row(const T* x, int channels, int lane, int8_t* q, int64_t pitch, All&& all) {
-  f32x4 v[PER];
+template <int LANES, int PER, class All>
+__device__ __forceinline__ float round_row(const f32x4 (&v)[PER], int lane, int8_t* q, int64_t pitch, All&& all) {
   uint32_t most = 0;  // |x| as a number orders as its bits do, infinity and NaN above all
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int c = (k * LANES + lane) * 4;
-    v[k] = get4(x + c, channels - c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float e = v[k][i];  // a cast of the vector's element itself takes its first
@@ -127,7 +133,9 @@ __global__ __launch_bounds__(threads_of(W)) void k_quantize(const T* x, int64_t 
     }
     return most;
   };
-  const float scale = round_row<T, LANES, PER>(x + row * x_row, channels, lane, q + row * pitch, pitch, all);
+  f32x4 v[PER];
+  load_row<T, LANES>(v, x + row * x_row, channels, lane);
+  const float scale = round_row<LANES>(v, lane, q + row * pitch, pitch, all);
   if (lane == 0) scales[row] = scale;
 }
 
@@ -197,13 +205,14 @@ __device__ __forceinline__ void put_outputs(const ProductArgs& p, int64_t m, int
 // The fewest rows, of at most 1536 inputs: every workgroup rounds them itself, which
 // saves a launch, while its weights are on their way.  A wavefront has 16 outputs, and
 // all of their weights in its registers.
-constexpr int FEWEST = 8;
+constexpr int FEWEST = 16;
 
-template <class O, int PER, bool WIDE>
+// EACH: rows of a wavefront.
+template <class O, int PER, int EACH, bool WIDE>
 __global__ __launch_bounds__(256) void k_fewest(ProductArgs p, const O* x, int64_t x_row) {
   constexpr int WIDTH = PER * 256, PITCH = WIDTH + 16;  // rows begin in banks four apart
-  __shared__ alignas(16) int8_t rows[FEWEST * PITCH];
-  __shared__ float scales[FEWEST];
+  __shared__ alignas(16) int8_t rows[4 * EACH * PITCH];
+  __shared__ float scales[4 * EACH];
   const int wave = threadIdx.x >> 6, lane = lane_id(), q = lane >> 4, l = lane & 15;
   const int n0 = (blockIdx.x * 4 + wave) * 16, count = (int)p.rows;
   const int8_t* w = p.weight + (int64_t)min(n0 + l, p.outputs - 1) * p.inputs;
@@ -213,9 +222,14 @@ __global__ __launch_bounds__(256) void k_fewest(ProductArgs p, const O* x, int64
     const int k = 64 * s + 16 * q;
     a[s] = k < p.inputs ? weight16<WIDE>(w, k, p.inputs) : i32x4{};
   }
-  for (int r = wave; r < count; r += 4) {
-    const float scale = round_row<O, 64, PER>(x + r * x_row, p.inputs, lane, rows + r * PITCH, WIDTH,
-                                              [](uint32_t most) { return most; });
+  f32x4 v[EACH][PER];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)  // rows past the last are the last again
+    load_row<O, 64>(v[i], x + min(wave + 4 * i, count - 1) * x_row, p.inputs, lane);
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int r = wave + 4 * i;
+    const float scale = round_row<64>(v[i], lane, rows + r * PITCH, WIDTH, [](uint32_t most) { return most; });
     if (lane == 0) scales[r] = scale;
   }
   __syncthreads();
@@ -551,11 +565,14 @@ int64_t tiles_of(int64_t rows, int64_t outputs, int tile) {
   return ((rows + tile - 1) / tile) * ((outputs + tile - 1) / tile);
 }
 
-// In us, here and with rows rounded by a launch of their own: 768 inputs and 3352
-// outputs 4.7 and 6.1 for one row, 6.0 and 6.5 for 8, 7.4 and 6.7 for 12; 50280 outputs
-// 9.8 and 13.3 for one, 11.7 and 13.4 for 8.
+// In us, here and with rows rounded by a launch of their own, kernels alone: 768 inputs
+// and 3352 outputs 4.6 and 6.1 for one row, 6.2 and 6.6 for 8, 8.5 and 6.7 for 16; 50280
+// outputs 10.2 and 13.3 for one, 11.7 and 13.1 for 8, 15.0 and 13.3 for 16; 1536 inputs
+// and 768 outputs 9.4 and 8.6 for 8.  One after another from Python, where a launch and a
+// workspace more are 4 us: 8.7 and 13.1 for 16 rows of 768 inputs and 3352 outputs, 14.7
+// and 13.1 of 50280 outputs, 12.8 and 13.5 of 1536 inputs and 768 outputs.
 bool is_fewest(const Int8& p) {
-  return p.rows <= FEWEST && rows_at_once(p.inputs) > 1;
+  return rows_at_once(p.inputs) > 1 && p.rows <= (p.inputs <= 768 && p.outputs <= 16384 ? FEWEST : 8);
 }
 
 }  // namespace
@@ -590,8 +607,14 @@ void int8_linear(const Int8& p, void* y, void* workspace, hipStream_t stream) {
       by_shape(p.inputs, [&](auto w, auto per, auto) {
         if constexpr (w() == 1) {
           const uint32_t grid = (uint32_t)((p.outputs + 63) / 64);
-          if (wide) k_fewest<O, per(), true><<<grid, 256, 0, stream>>>(a, (const O*)p.x.p, p.x.row);
-          else k_fewest<O, per(), false><<<grid, 256, 0, stream>>>(a, (const O*)p.x.p, p.x.row);
+          auto go = [&](auto each) {
+            const O* x = (const O*)p.x.p;
+            if (wide) k_fewest<O, per(), each(), true><<<grid, 256, 0, stream>>>(a, x, p.x.row);
+            else k_fewest<O, per(), each(), false><<<grid, 256, 0, stream>>>(a, x, p.x.row);
+          };
+          if (p.rows <= 4) go(std::integral_constant<int, 1>{});
+          else if (p.rows <= 8) go(std::integral_constant<int, 2>{});
+          else go(std::integral_constant<int, 4>{});
         }
       });
     });

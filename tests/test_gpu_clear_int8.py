@@ -91,7 +91,7 @@ def compare(rows, inputs, outputs, dtype, bias=True, seed=0):
 
 
 @pytest.mark.parametrize("inputs", [1, 15, 16, 17, 63, 64, 65, 96, 128, 129, 255, 333, 768, 1001, 1536, 4100])
-@pytest.mark.parametrize("rows,outputs", [(1, 1), (1, 643), (2, 17), (15, 16), (17, 15), (33, 64), (64, 65), (65, 3),
+@pytest.mark.parametrize("rows,outputs", [(1, 1), (1, 643), (2, 17), (7, 130), (8, 64), (15, 16), (16, 643), (17, 15), (33, 64), (64, 65), (65, 3),
                                           (100, 130), (250, 768)])
 def test_few_rows(rows, outputs, inputs):
     compare(rows, inputs, outputs, BF if (rows + inputs) % 2 else F32, bias=outputs % 2 == 0)
