@@ -318,7 +318,7 @@ void embed_backward(const Embed& e, const Rows& dy, void* dweight, void* workspa
   a.tokens = e.tokens;
   a.channels = e.channels;
   a.piece = piece_of(e.tokens);
-  a.pieces = (int)((e.tokens + a.piece - 1) / a.piece);
+  a.pieces = e.tokens > a.piece ? (int)((e.tokens + a.piece - 1) / a.piece) : 0;  // no row has more than a piece
   a.scale = e.scale;
   k_sort<<<(uint32_t)((e.vocab + SPAN - 1) / SPAN), 64 * SORT_WAVES, 0, stream>>>(e.ids, e.tokens, e.vocab, a.o);
   hip_check(hipGetLastError(), "order of tokens");

@@ -146,16 +146,20 @@ def test_refusals():
     parent = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
     state = torch.zeros(6, 4, device="cuda")
     bad = [(lambda: clear.beam_select(logits.half(), scores), "float32 or bfloat16"),
-           (lambda: clear.beam_select(logits[0], scores), "axes"), (lambda: clear.beam_select(logits, scores[:1]), "shape"),
-           (lambda: clear.beam_select(logits, scores, 33), "width"), (lambda: clear.beam_select(logits, scores, 0), "width"),
+           (lambda: clear.beam_select(logits[0], scores), "axes"),
+           (lambda: clear.beam_select(logits, scores[:1]), "shape"),
+           (lambda: clear.beam_select(logits, scores, 33), "width"),
+           (lambda: clear.beam_select(logits, scores, 0), "width"),
            (lambda: clear.beam_select(logits[..., :2], scores, 7), "width"),
            (lambda: clear.beam_select(logits, scores, finished=none), "end"),
            (lambda: clear.beam_select(logits, scores, finished=none, end=10), "end"),
            (lambda: clear.beam_select(logits, scores, finished=none.int(), end=1), "type"),
            (lambda: clear.beam_select(logits[:0], scores[:0]), "requests"),
+
            (lambda: clear.beam_select(torch.zeros(1, 33, 4, device="cuda"), torch.zeros(1, 33, device="cuda")), "32 beams"),
            (lambda: clear.beam_select(logits, scores.clone().requires_grad_(True)), "no gradient"),
-           (lambda: clear.reorder_states([], parent), "no states"), (lambda: clear.reorder_states(state, parent.long()), "type"),
+           (lambda: clear.reorder_states([], parent), "no states"),
+           (lambda: clear.reorder_states(state, parent.long()), "type"),
            (lambda: clear.reorder_states(state[:5], parent), "6 beams and 5 rows"),
            (lambda: clear.reorder_states(state, parent[0]), "requests"),
            (lambda: clear.reorder_states(state.t(), parent, slots=parent), "contiguous"),

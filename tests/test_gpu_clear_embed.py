@@ -145,7 +145,8 @@ def test_refusals():
     from fhemamba_amd import clear
 
     w, ids = torch.randn(5, 4, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
-    for call, match in [(lambda: clear.embed(w.half(), ids), "float32 or bfloat16"), (lambda: clear.embed(w[0], ids), "axes"),
+    for call, match in [(lambda: clear.embed(w.half(), ids), "float32 or bfloat16"),
+                        (lambda: clear.embed(w[0], ids), "axes"),
                         (lambda: clear.embed(w, ids.int()), "type"), (lambda: clear.embed(w, ids.cpu()), "cpu"),
                         (lambda: clear.embed(w, [1]), "tensor"), (lambda: clear.embed(w[:0], ids), "vocabulary"),
                         (lambda: clear.embed(w, ids, scale=float("inf")), "finite")]:

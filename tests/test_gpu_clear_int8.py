@@ -91,8 +91,8 @@ def compare(rows, inputs, outputs, dtype, bias=True, seed=0):
 
 
 @pytest.mark.parametrize("inputs", [1, 15, 16, 17, 63, 64, 65, 96, 128, 129, 255, 333, 768, 1001, 1536, 4100])
-@pytest.mark.parametrize("rows,outputs", [(1, 1), (1, 643), (2, 17), (7, 130), (8, 64), (15, 16), (16, 643), (17, 15), (33, 64), (64, 65), (65, 3),
-                                          (100, 130), (250, 768)])
+@pytest.mark.parametrize("rows,outputs", [(1, 1), (1, 643), (2, 17), (7, 130), (8, 64), (15, 16), (16, 643),
+                                          (17, 15), (33, 64), (64, 65), (65, 3), (100, 130), (250, 768)])
 def test_few_rows(rows, outputs, inputs):
     compare(rows, inputs, outputs, BF if (rows + inputs) % 2 else F32, bias=outputs % 2 == 0)
 
@@ -191,10 +191,12 @@ def test_refusals():
 
     x, w = torch.randn(3, 16, device="cuda"), torch.zeros(4, 16, dtype=torch.int8, device="cuda")
     ws = torch.ones(4, device="cuda")
-    bad = [(lambda: clear.int8_linear(x.half(), w, ws), "float32 or bfloat16"), (lambda: clear.int8_linear(x, w.int(), ws), "type"),
+    bad = [(lambda: clear.int8_linear(x.half(), w, ws), "float32 or bfloat16"),
+           (lambda: clear.int8_linear(x, w.int(), ws), "type"),
            (lambda: clear.int8_linear(x, w[:, :8], ws), "shape"), (lambda: clear.int8_linear(x, w, ws[:2]), "shape"),
            (lambda: clear.int8_linear(x, w[0], ws), "outputs"), (lambda: clear.int8_linear(x, w, ws, ws[:2]), "shape"),
-           (lambda: clear.int8_linear(x, w[:0], ws[:0]), "no outputs"), (lambda: clear.int8_linear(x, w, ws.double()), "type"),
+           (lambda: clear.int8_linear(x, w[:0], ws[:0]), "no outputs"),
+           (lambda: clear.int8_linear(x, w, ws.double()), "type"),
            (lambda: clear.int8_linear(x.clone().requires_grad_(True), w, ws), "no gradient"),
            (lambda: clear.int8_linear(x, w, ws.clone().requires_grad_(True)), "no gradient"),
            (lambda: clear.int8_linear(x, w.cpu(), ws), "cpu"), (lambda: clear.quantize_rows(x.int()), "float32"),

@@ -272,11 +272,13 @@ def test_refusals():
            (lambda: clear.rms_norm(x, w.to(BF)), "type"), (lambda: clear.rms_norm(x, w, groups=3), "groups"),
            (lambda: clear.rms_norm(x, w, groups=0), "groups"), (lambda: clear.rms_norm(x, w, gate=x.to(BF)), "type"),
            (lambda: clear.rms_norm(x, w, gate=x[:2]), "shape"), (lambda: clear.rms_norm(x, w, eps=-1.0), "eps"),
-           (lambda: clear.rms_norm(x, w, eps=math.nan), "eps"), (lambda: clear.rms_norm(x.to(BF), w, dtype=F32), "dtype"),
+           (lambda: clear.rms_norm(x, w, eps=math.nan), "eps"),
+           (lambda: clear.rms_norm(x.to(BF), w, dtype=F32), "dtype"),
            (lambda: clear.rms_norm(x, w.cpu()), "cpu"), (lambda: clear.rms_norm(x[:, :0], w[:0]), "channels"),
            (lambda: clear.rms_norm(x.new_empty(1, 32769), x.new_empty(32769)), "32768"),
            (lambda: clear.add_norm(x.to(BF), x, w), "type"), (lambda: clear.add_norm(x, x[:2], w), "shape"),
-           (lambda: clear.add_norm(x, x, w, scale=w[:3]), "shape"), (lambda: clear.add_norm(x, x, w, eps=math.inf), "eps"),
+           (lambda: clear.add_norm(x, x, w, scale=w[:3]), "shape"),
+           (lambda: clear.add_norm(x, x, w, eps=math.inf), "eps"),
            (lambda: clear.add_norm(x.new_empty(1, 32769), x.new_empty(1, 32769), x.new_empty(32769)), "32768")]
     for call, match in bad:
         with pytest.raises(ValueError, match=match):
