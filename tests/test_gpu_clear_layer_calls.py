@@ -159,8 +159,8 @@ def test_tangents_are_refused():
     ids, parent = torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(1, 2, dtype=torch.int32, device="cuda")
     table = torch.zeros(4, 8, dtype=torch.int8, device="cuda")
     with fwd.dual_level(), torch.no_grad():
-        for call in
-                    (lambda: clear.rms_norm(z(2, 8), dual(z(8))), lambda: clear.rms_norm(z(2, 8), z(8), gate=dual(z(2, 8))),
+        for call in (lambda: clear.rms_norm(z(2, 8), dual(z(8))),
+                     lambda: clear.rms_norm(z(2, 8), z(8), gate=dual(z(2, 8))),
                      lambda: clear.add_norm(z(2, 8), dual(z(2, 8)), z(8)), lambda: clear.quantize_rows(dual(z(2, 8))),
                      lambda: clear.int8_linear(dual(z(2, 8)), table, z(4)), lambda: clear.embed(dual(z(4, 8)), ids),
                      lambda: clear.beam_select(dual(z(1, 2, 8)), z(1, 2)),
