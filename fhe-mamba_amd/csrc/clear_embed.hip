@@ -5,6 +5,7 @@
 // gradient of 8192 in a table of 50280 11 + 42 + 5 (3.8 TB/s of reads and writes in the
 // second of its kernels).  The gradient adds each row's tokens in their order,
 // so that equal inputs give equal bits; no atomic addition of floats:
+//   k_direct does all for few tokens; for more
 //   k_sort   a workgroup for each 256 rows of the table reads all ids, counts those
 //            of its rows and those before them, and writes its tokens in order of
 //            (id, token).  The ids are few beside the table: reading them once a
@@ -249,6 +250,44 @@ __global__ __launch_bounds__(256) void k_sums(SumArgs a) {
   }
 }
 
+// Few tokens, in one launch and without a workspace: a wavefront a row looks through
+// all of them for its own.  Lookup and gradient of 128 tokens take 25 us in a table of
+// 50280 x 768 (31 by their order), 6 in one of 93 x 768 (11); of 128 tokens of one row
+// 37 and 33, of 256 63 and 33.
+constexpr int DIRECT = 128;
+
+template <class T, int COVER>
+__global__ __launch_bounds__(256) void k_direct(SumArgs a, const int64_t* ids) {
+  __shared__ int rows[DIRECT], mine[4][DIRECT];
+  const int wave = uniform(threadIdx.x >> 6), lane = lane_id();
+  for (int t = threadIdx.x; t < DIRECT; t += 256) {
+    const int64_t id = t < a.tokens ? ids[t] : -1;
+    rows[t] = id >= 0 && id < a.vocab ? (int)id : -1;
+  }
+  __syncthreads();
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  if (row >= a.vocab) return;
+  int count = 0;
+#pragma unroll
+  for (int j = 0; j < DIRECT; j += 64) {
+    const bool own = rows[j + lane] == (int)row;
+    const uint64_t found = __ballot(own);
+    if (own) mine[wave][count + __popcll(found & ((1ull << lane) - 1))] = j + lane;
+    count += __popcll(found);
+  }
+  wave_sync();
+  T* out = (T*)a.dweight + row * a.channels;
+  for (int c0 = 0; c0 < a.channels; c0 += 256 * COLUMNS) {
+    f32x4 sum[COLUMNS];
+    add_rows<T, COVER>(a, mine[wave], uniform(count), c0, sum);
+#pragma unroll
+    for (int k = 0; k < COLUMNS; ++k) {
+      const int c = c0 + k * 256;
+      if (c < a.channels) Piece<COVER>(c + 4 * lane, a.channels).put(out, sum[k] * a.scale);
+    }
+  }
+}
+
 // A workgroup a piece: if a long row begins in it, the sum of that row's parts, every
 // sixteenth of them in one of its wavefronts.
 constexpr int JOIN_WAVES = 16;
@@ -297,6 +336,7 @@ void embed(const Embed& e, void* y, hipStream_t stream) {
 }
 
 size_t embed_workspace(const Embed& e) {
+  if (e.tokens <= DIRECT) return 0;
   const int piece = piece_of(e.tokens);
   const int64_t pieces = (e.tokens + piece - 1) / piece;
   return line(4 * ((size_t)e.vocab + 1)) + 2 * line(4 * (size_t)e.tokens) + (size_t)pieces * 2 * e.channels * 4;
@@ -304,6 +344,30 @@ size_t embed_workspace(const Embed& e) {
 
 void embed_backward(const Embed& e, const Rows& dy, void* dweight, void* workspace, hipStream_t stream) {
   SumArgs a{};
+  a.dy = dy.p;
+  a.dy_row = dy.row;
+  a.dweight = dweight;
+  a.vocab = e.vocab;
+  a.tokens = e.tokens;
+  a.channels = e.channels;
+  a.scale = e.scale;
+  // f(type, cover)
+  auto by_cover = [&](auto&& f) {
+    auto go = [&](auto zero) {
+      if (e.channels % 256 == 0) f(zero, std::integral_constant<int, WHOLE>{});
+      else if (e.channels >= 4) f(zero, std::integral_constant<int, MOVED>{});
+      else f(zero, std::integral_constant<int, SHORT>{});
+    };
+    if (e.dtype == BF16) go(bf16{});
+    else go(float{});
+  };
+  if (e.tokens <= DIRECT) {
+    by_cover([&](auto zero, auto cover) {
+      k_direct<decltype(zero), cover()><<<(uint32_t)((e.vocab + 3) / 4), 256, 0, stream>>>(a, e.ids);
+    });
+    hip_check(hipGetLastError(), "embedding gradient of few tokens");
+    return;
+  }
   char* w = (char*)workspace;
   a.o.start = (int*)w;
   w += line(4 * ((size_t)e.vocab + 1));
@@ -311,28 +375,13 @@ void embed_backward(const Embed& e, const Rows& dy, void* dweight, void* workspa
   w += line(4 * (size_t)e.tokens);
   a.o.row = (int*)w;
   a.parts = (float*)(w + line(4 * (size_t)e.tokens));
-  a.dy = dy.p;
-  a.dy_row = dy.row;
-  a.dweight = dweight;
-  a.vocab = e.vocab;
-  a.tokens = e.tokens;
-  a.channels = e.channels;
   a.piece = piece_of(e.tokens);
-  a.pieces = e.tokens > a.piece ? (int)((e.tokens + a.piece - 1) / a.piece) : 0;  // no row has more than a piece
-  a.scale = e.scale;
+  a.pieces = (int)((e.tokens + a.piece - 1) / a.piece);
   k_sort<<<(uint32_t)((e.vocab + SPAN - 1) / SPAN), 64 * SORT_WAVES, 0, stream>>>(e.ids, e.tokens, e.vocab, a.o);
   hip_check(hipGetLastError(), "order of tokens");
   const uint32_t grid = (uint32_t)(a.pieces + (e.vocab + 3) / 4);
-  auto sums = [&](auto zero) {
-    using T = decltype(zero);
-    if (e.channels % 256 == 0) k_sums<T, WHOLE><<<grid, 256, 0, stream>>>(a);
-    else if (e.channels >= 4) k_sums<T, MOVED><<<grid, 256, 0, stream>>>(a);
-    else k_sums<T, SHORT><<<grid, 256, 0, stream>>>(a);
-  };
-  if (e.dtype == BF16) sums(bf16{});
-  else sums(float{});
+  by_cover([&](auto zero, auto cover) { k_sums<decltype(zero), cover()><<<grid, 256, 0, stream>>>(a); });
   hip_check(hipGetLastError(), "embedding gradient");
-  if (!a.pieces) return;
   if (e.dtype == BF16) k_join<bf16><<<a.pieces, 64 * JOIN_WAVES, 0, stream>>>(a);
   else k_join<float><<<a.pieces, 64 * JOIN_WAVES, 0, stream>>>(a);
   hip_check(hipGetLastError(), "embedding gradient of frequent tokens");

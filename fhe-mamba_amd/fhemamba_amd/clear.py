@@ -796,8 +796,8 @@ class _Embed(torch.autograd.Function):
         ids, dy = ids.contiguous(), _flat(dy)
         args = _pack_embed(None, ids, *ctx.options)
         dw = dy.new_empty(ctx.options[2:])
-        space, size = _workspace(_lib.lib.fhe_embed_workspace, dy, args)
-        _run(_lib.lib.fhe_embed_backward, dy, args, _ROWS.pack(*_row(dy)), dw.data_ptr(), space.data_ptr(), size)
+        space, size = _workspace(_lib.lib.fhe_embed_workspace, dy, args)  # none for few tokens
+        _run(_lib.lib.fhe_embed_backward, dy, args, _ROWS.pack(*_row(dy)), dw.data_ptr(), _ptr(space), size)
         return dw, None, None
 
 

@@ -169,13 +169,14 @@ def test_embed_outputs_and_workspace():
                          ({"dtype": 1}, 4097, "aligned")):
         with pytest.raises(ValueError, match=match):
             _lib.call("fhe_embed", embed(**kw), y, 0)
-    size = size_of("fhe_embed_workspace", embed(weight=0))
-    dy = clear._ROWS.pack(4096, 8)
-    for d, dw, space, given, match in ((dy, 0, 4096, size, "null"), (None, 4096, 4096, size, "null"),
-                                       (clear._ROWS.pack(0, 8), 4096, 4096, size, "null"), (dy, 4098, 4096, size, "aligned"),
-                                       (dy, 4096, 4096, size - 1, "too small")):
+    args = embed(weight=0, tokens=4000)
+    size = size_of("fhe_embed_workspace", args)
+    assert size >= 4 * 11 + 8 * 4000 and size_of("fhe_embed_workspace", embed(weight=0)) == 0
+    dy, none = clear._ROWS.pack(4096, 8), clear._ROWS.pack(0, 8)
+    for d, dw, given, match in ((dy, 0, size, "null"), (None, 4096, size, "null"), (none, 4096, size, "null"),
+                                (dy, 4098, size, "aligned"), (dy, 4096, size - 1, "too small")):
         with pytest.raises(ValueError, match=match):
-            _lib.call("fhe_embed_backward", embed(weight=0), d, dw, space, given, 0)
+            _lib.call("fhe_embed_backward", args, d, dw, 4096, given, 0)
 
 
 def beam(**kw):

@@ -37,7 +37,7 @@ def compare(weight, ids, scale, seed=0):
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("vocab,channels", [(1, 1), (2, 3), (93, 64), (255, 5), (256, 256), (257, 333), (513, 1100),
                                             (9973, 8), (50280, 16)])
-@pytest.mark.parametrize("tokens", [1, 2, 63, 64, 65, 129, 1000, 5001])
+@pytest.mark.parametrize("tokens", [1, 2, 63, 64, 65, 128, 129, 1000, 5001])
 def test_lookup_and_gradient(tokens, vocab, channels, dtype):
     print(f"[embed] {tokens} of {vocab} x {channels} {dtype}", flush=True)
     gen = torch.Generator().manual_seed(tokens + vocab)
@@ -67,6 +67,9 @@ def test_many_tokens():
     ids[torch.rand(150001, generator=gen) < 0.5] = 300
     compare(weight, ids, 1.0)
     compare(weight, torch.full((500,), -1), 1.0)
+    for n in (100, 128, 129):  # of one row, and of none
+        compare(weight, torch.full((n,), 999), 1.0)
+        compare(weight, torch.full((n,), -1), 1.0)
 
 
 def test_axes_strides_and_no_tokens():
