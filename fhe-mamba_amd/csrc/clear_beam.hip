@@ -123,7 +123,7 @@ __global__ __launch_bounds__(THREADS) void k_beam_rows(BeamArgs a) {
   const float score = a.b.scores[row_i];
   if (!is_read(a.b, row_i)) {
     if (i >= a.list) return;
-    const bool finished = a.b.finished && a.b.finished[row_i];
+    const bool finished = score != -INFINITY;  // else a beam without candidates, finished or not
     // behind the end token the others in order, which are not allowed
     const int end = finished ? (int)a.b.end : -1;
     total[i] = finished && i == 0 ? (double)score : -INFINITY;

@@ -8,8 +8,8 @@
 //   k_direct does all for few tokens; for more
 //   k_sort   a workgroup for each 256 rows of the table reads all ids, counts those
 //            of its rows and those before them, and writes its tokens in order of
-//            (id, token).  The ids are few beside the table: reading them once a
-//            workgroup costs less than the launches of a sort in passes.
+//            (id, token).  The ids are few beside the table, so that each workgroup
+//            can read all of them, and nothing waits for a sort's passes.
 //   k_sums   a wavefront a row of the table adds the row's tokens, or writes zeros.
 //            Rows of more than `piece` tokens are left out here; a workgroup each
 //            `piece` tokens of the order adds what of it belongs to such rows.

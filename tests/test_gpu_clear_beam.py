@@ -55,7 +55,8 @@ def test_finished_dead_and_masked_beams():
     logits, scores = make(1, 6, 4, 300, F32, masked=0.2)
     finished = torch.zeros(6, 4, dtype=torch.bool)
     scores[0, 1:] = -math.inf                      # the first step: one live beam
-    scores[1] = -math.inf                          # none
+    scores[1] = -math.inf                          # none, and one of them is finished
+    finished[1, 0] = True
     finished[2, 1] = finished[2, 3] = True
     finished[3] = True                             # all
     logits[4, 0] = -math.inf                       # no token is allowed
