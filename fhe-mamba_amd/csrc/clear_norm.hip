@@ -1,7 +1,7 @@
 // Root mean square norms fused with what stands before them in a layer, and
 // their gradients:
 //   v = x, x silu(z) or h + s u;   r = (mean v^2 + eps)^(-1/2);   n = v r w
-//   g = dn w,   dv = r g - v r^3 mean(g v) (+ the gradient of h + s u itself)
+//   g = dn w,   dv = r (g - v r (r mean(g v))) (+ the gradient of h + s u itself)
 //   dx = dv silu(z),  dz = dv x silu'(z);   dh = dv,  du = s dv
 //   dw = sum over rows of dn v r,   ds = sum over rows of dv u
 // A row is held in registers by one wavefront, four or sixteen, so that each
@@ -157,15 +157,17 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
       }
     }
     row_sums<W>(s, lds, turn ^= 1);
-    const float r = rsqrtf(s[0] * mean + p.eps);
-    const float back = r * r * r * (s[1] * mean);
+    // v is made a unit before it is weighed: powers of r above the first leave 32 bits
+    // for rows as small as 1e-13 or as large as 1e14
+    const float r = rsqrtf(s[0] * mean + p.eps), back = r * (s[1] * mean);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int64_t at = row * p.all + first;
-      f32x4 t = v[k];
-      if constexpr (MODE == GATED) t *= act[k];
-      f32x4 d = r * (g[k] * w[k]) - t * back;
-      dw[k] += g[k] * (t * r);
+      f32x4 unit = v[k];
+      if constexpr (MODE == GATED) unit *= act[k];
+      unit *= r;
+      f32x4 d = r * (g[k] * w[k] - unit * back);
+      dw[k] += g[k] * unit;
       if constexpr (MODE == PLAIN) {
         piece[k].put((A*)p.da + at, d);
       } else if constexpr (MODE == GATED) {

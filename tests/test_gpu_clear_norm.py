@@ -287,3 +287,46 @@ def test_refusals():
     (g,) = torch.autograd.grad(clear.rms_norm(leaf, w).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+# (size of the values, eps): r = 1 / size leaves r^3 no room in 32 bits from about 1e13 on, or below 1e-12
+RANGES = [(1e13, 1e-5), (1e15, 1e-5), (1e17, 1e-5), (1e18, 0.0), (1e-13, 0.0), (1e-13, 1e-30), (1e-16, 1e-30), (0.0, 1e-30)]
+
+
+@pytest.mark.parametrize("size,eps", RANGES)
+@pytest.mark.parametrize("form", ["plain", "gated", "sum", "scaled"])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_gradients_of_very_large_and_very_small_rows(dtype, form, size, eps):
+    """The squares' sum is far from 32 bits' ends, and so are the gradients, of the size of r g."""
+    from fhemamba_amd import clear
+
+    rows, channels = 5, 97
+    gen = torch.Generator().manual_seed(7)
+    x, other = (size * n(gen, rows, channels)).to(dtype), n(gen, rows, channels, dtype=dtype)
+    w, s, dn = 1 + 0.2 * n(gen, channels), 0.5 + 0.1 * n(gen, channels), n(gen, rows, channels, dtype=dtype)
+    if form == "gated":
+        tensors, call = (x, w, other), lambda a, b, c: clear.rms_norm(a, b, gate=c, eps=eps)
+        plain = lambda a, b, c: L.norm(a, b, c, 1, eps)  # noqa: E731
+        v = x.double() * other.double() * torch.sigmoid(other.double())
+    elif form == "plain":
+        tensors, call = (x, w), lambda a, b: clear.rms_norm(a, b, eps=eps)
+        plain = lambda a, b: L.norm(a, b, None, 1, eps)  # noqa: E731
+        v = x.double()
+    else:
+        update = (size * other.double()).to(dtype)
+        scaled = form == "scaled"
+        tensors = (x, update, w, s) if scaled else (x, update, w)
+        call = lambda a, b, c, d=None: clear.add_norm(a, b, c, scale=d, eps=eps).normed  # noqa: E731
+        plain = lambda a, b, c, d=None: L.add_norm(a, b, c, d, eps)[0]  # noqa: E731
+        v = x.double() + update.double() * (s.double() if scaled else 1.0)
+    ref, mine = [leaf(t) for t in tensors], [t.cuda().requires_grad_(True) for t in tensors]
+    want, got = plain(*ref), call(*mine)
+    check(got, want, dtype)
+    # both terms of the gradient of v are as large as r g
+    rg = dn.double() * w.double() / torch.sqrt((v * v).mean(-1, keepdim=True) + eps)
+    act = other.double() * torch.sigmoid(other.double())
+    terms = {"plain": (rg, None), "gated": (rg * act, None, rg * x.double()), "sum": (rg, rg, None),
+             "scaled": (rg, rg * s.double(), None, (rg * other.double() * size).norm(dim=0))}[form]
+    grads = torch.autograd.grad(want, ref, dn.double())
+    for g, e, t, term in zip(torch.autograd.grad(got, mine, dn.cuda()), grads, tensors, terms):
+        check(g, e, t.dtype, term)
