@@ -37,8 +37,16 @@ struct NormArgs {
   float eps;
 };
 
+// 1 / (1 + e^-v).  The product -v log2 e is rounded to 32 bits, up to 2^-18 off at v = -80,
+// which would be as much of a closed gate; what the rounding took off, and the constant's own,
+// goes in as a factor.  2^x and the reciprocal are the hardware's, good to a unit.
 __device__ __forceinline__ float sigmoid(float v) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+  constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
+  constexpr float HIGH = (float)LOG2E, LOW = (float)((LOG2E - (double)HIGH) * LN2);
+  v = __builtin_amdgcn_fmed3f(v, -128.0f, 128.0f);  // 0 or 1 beyond
+  const float x = v * -HIGH, off = __builtin_fmaf(v, -HIGH, -x);
+  const float factor = __builtin_fmaf(v, -LOW, __builtin_fmaf(off, (float)LN2, 1.0f));
+  return __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_exp2f(x), factor, 1.0f));
 }
 
 // The sums of W wavefronts' lanes; `lds` is free again after the next call's barrier.
@@ -84,11 +92,21 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm(NormArgs p) {
        row += (int64_t)gridDim.x * ROWS) {
     const A* a = (const A*)p.a + row * p.a_row + first;
     const B* b = (const B*)p.b + (MODE == PLAIN ? 0 : row * p.b_row + first);
+    Raw4<A> raw_a[PER];
+    Raw4<B> raw_b[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      raw_a[k] = piece[k].raw(a);
+      if constexpr (MODE != PLAIN) raw_b[k] = piece[k].raw(b);
+    }
+    // all on their way: left to itself the compiler may widen each before the next is
+    // asked for (a call of 30011 rows of 1536 with a gate in bfloat16: 72 us for 51)
+    __builtin_amdgcn_sched_barrier(0);
     f32x4 v[PER], other[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      v[k] = piece[k].get(a);
-      if constexpr (MODE != PLAIN) other[k] = piece[k].get(b);
+      v[k] = widen(raw_a[k]);
+      if constexpr (MODE != PLAIN) other[k] = widen(raw_b[k]);
     }
     float s[1] = {0.0f};
 #pragma unroll

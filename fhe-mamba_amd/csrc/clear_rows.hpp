@@ -32,6 +32,25 @@ __device__ __forceinline__ f32x4 get4(const bf16* p, int count) {
   for (int i = 0; i < 4; ++i) v[i] = i < count ? (float)p[i] : 0.0f;
   return v;
 }
+
+// The same in two steps, so that loads can all be on their way before the first is widened.
+__device__ __forceinline__ f32x4 raw4(const float* p, int count) { return get4(p, count); }
+__device__ __forceinline__ u32x2 raw4(const bf16* p, int count) {
+  u32x2 u{};
+  if (count >= 4) {
+    __builtin_memcpy(&u, p, 8);
+    return u;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < count) u[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << 16 * (i % 2);
+  return u;
+}
+__device__ __forceinline__ f32x4 widen(f32x4 v) { return v; }
+__device__ __forceinline__ f32x4 widen(u32x2 u) { return {low2(u[0]), high2(u[0]), low2(u[1]), high2(u[1])}; }
+template <class T>
+using Raw4 = decltype(raw4((const T*)nullptr, 4));
+
 __device__ __forceinline__ void put4(float* p, f32x4 v, int count) {
   if (count >= 4) {
     __builtin_memcpy(p, &v, 16);
@@ -88,6 +107,10 @@ struct Piece {
   template <class T>
   __device__ __forceinline__ f32x4 get(const T* row) const {
     return get4(row + at, COVER == SHORT ? own : 4);
+  }
+  template <class T>
+  __device__ __forceinline__ Raw4<T> raw(const T* row) const {
+    return raw4(row + at, COVER == SHORT ? own : 4);
   }
   // A moved piece writes its neighbour's elements too: the same values from the same inputs.
   template <class T>

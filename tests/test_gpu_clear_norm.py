@@ -330,3 +330,39 @@ def test_gradients_of_very_large_and_very_small_rows(dtype, form, size, eps):
     grads = torch.autograd.grad(want, ref, dn.double())
     for g, e, t, term in zip(torch.autograd.grad(got, mine, dn.cuda()), grads, tensors, terms):
         check(g, e, t.dtype, term)
+
+
+@pytest.mark.parametrize("low,high", [(-8, -4), (-20, -10), (-60, -40), (-85, -75), (-2, 2), (4, 40)])
+def test_gates_element_by_element(low, high):
+    """Each result for itself: a closed gate's is as exact as an open one's.
+
+    In steps of 2^-24 of a result: the sigmoid's exponential 2 (a unit of the hardware's), its factor 2, 1 + e 1, the
+    reciprocal 2, the products with the gate and x 2, together 9; the row's size as much from its
+    products, 5.5 from ten sums and a square, 0.5 from eps, the root's unit 2; two more products: 28."""
+    from fhemamba_amd import clear
+
+    gen = torch.Generator().manual_seed(-low)
+    rows, channels = 400, 64
+    z = low + (high - low) * torch.rand(rows, channels, generator=gen)
+    # so that the row's values are all of the same size
+    x = (torch.exp(-z.double().clamp(max=0)) * (1 + torch.rand(rows, channels, generator=gen))).float()
+    w = 1 + torch.rand(channels, generator=gen)
+    got = clear.rms_norm(x.cuda(), w.cuda(), gate=z.cuda()).cpu().double()
+    want = L.norm(x.double(), w.double(), z.double(), 1, 1e-5)
+    off = ((got - want) / want).abs().max().item() * 2.0 ** 24
+    assert off <= 28, off
+
+
+def test_gates_at_the_ends_of_their_type():
+    """Open ones pass x on, closed ones nothing, and one that is no number spoils its row."""
+    from fhemamba_amd import clear
+
+    w = torch.ones(8, device="cuda")
+    z = torch.tensor([[3e38, 1e4, 200.0, 89.0, 0.0, -200.0, -1e4, -3e38], [1.0] * 7 + [math.nan],
+                      [1.0] * 7 + [-math.inf], [-104.0] * 8, [0.0] * 8], device="cuda")
+    x = torch.full((5, 8), 1e-38, device="cuda")
+    x[0, 1:] = 1.0
+    got = clear.rms_norm(x, w, gate=z)
+    assert bool(torch.isfinite(got[0]).all()) and not bool(got[0, 4:].any()) and bool((got[0, :4] > 0).all())
+    assert bool(torch.isnan(got[1]).all()) and bool(torch.isnan(got[2]).all())
+    assert not bool(got[3:].any())
