@@ -837,7 +837,8 @@ def beam_select(logits, scores, width: Optional[int] = None, *, finished=None, e
     A beam of score -inf has none.  finished [requests, beams] bool: such
     a beam has the one candidate `end`, at its own score.  Where fewer candidates are allowed, others
     follow with score -inf.  A NaN or +inf among a live beam's logits, or for a score, makes the beam's
-    candidates NaN, which come first.  No gradient (token_logprobs at the chosen tokens has one)."""
+    candidates NaN, which come first.  No gradient (token_logprobs at the chosen tokens has one).  Where the
+    width is not the number of beams, reorder_states has to be told how many beams there were."""
     _first("logits", logits, 3)
     requests, beams, vocab = logits.shape
     if min(requests, beams, vocab) < 1 or beams > MAX_TOP or requests > 65535:
@@ -866,27 +867,35 @@ def beam_select(logits, scores, width: Optional[int] = None, *, finished=None, e
     return BeamChoice(score, parent, token)
 
 
-def reorder_states(states, parent, *, slots=None) -> None:
+def reorder_states(states, parent, *, slots=None, beams: Optional[int] = None) -> None:
     """The states follow their beams, in place: row slots[r, j] takes what row slots[r, parent[r, j]] held.
 
-    states: a tensor [cache, ..] or a sequence of them with as many rows, of any type, contiguous; all
-    move in one launch.  parent [requests, beams] int32 (at most 32 beams) as beam_select gives it, slots
-    alike (default r * beams + j), no row twice.  A parent that is no beam leaves the row as it is; a slot
+    states: a tensor [cache, ..] or a sequence of them with as many rows, of any type, contiguous.  parent
+    [requests, width] int32 as beam_select gives it; `beams` (at most 32) is how many beams each request had
+    before, which beam_select's caller has to say where that is not the width.  slots [requests, the larger of
+    width and beams] (default: rows in order, as many for each request), no row twice: the first `width` of
+    them are written, the others stay as they were.  A parent that is no beam leaves the row as it is; a slot
     outside of the cache is padding.  A backward pass that needs a state as it was before raises."""
     states = (states,) if isinstance(states, torch.Tensor) else tuple(states)
     if not states:
         raise ValueError("no states")
     _axes("parent", parent, 2, "be [requests, beams]")
-    requests, beams = parent.shape
+    requests, width = parent.shape
+    beams = width if beams is None else beams
     first = states[0]
     # there may be two for each layer: checked in as few Python steps as can be
     if not all(map(isinstance, states, repeat(torch.Tensor))) or not first.is_cuda:
         raise ValueError("states must be tensors on the GPU")
     if len(set(map(_device_of, states))) > 1:
         raise ValueError("states must be tensors on one GPU")
-    if not (1 <= requests <= 65535 and 1 <= beams <= MAX_TOP):
+    if not (1 <= requests <= 65535 and 1 <= width <= MAX_TOP and 1 <= beams <= MAX_TOP):
         raise ValueError(f"parent must be [requests, beams] with 1 to 65535 requests and 1 to {MAX_TOP} beams")
-    _gpu("parent", parent, (torch.int32,), (requests, beams), first)
+    _gpu("parent", parent, (torch.int32,), (requests, width), first)
+    if width < beams:  # rows without a parent stay
+        parent = torch.nn.functional.pad(parent, (0, beams - width), value=-1)
+    elif width > beams:  # and those whose parent is none of the beams that were
+        parent = parent.masked_fill(parent >= beams, -1)
+        beams = width
     try:
         rows = set(map(_size_of, states, repeat(0)))
     except IndexError:  # a tensor without axes

@@ -626,7 +626,8 @@ int fhe_beam_select(const fhe_beam_args *args, const fhe_beam_out *out,
  * host; each has `cache` contiguous rows of row_bytes <= 2^30.  parent [requests]
  * [beams] and slots (device; slots NULL: r * beams + j).  A parent outside of
  * [0, beams) leaves the row as it is, a slot outside of [0, cache) is padding.  No
- * row may be named twice. */
+ * row may be named twice.  `beams` counts the beams before and after: behind a
+ * choice of fewer (its width less than its beams) parent goes on with -1. */
 typedef struct {
   void *data;
   int64_t row_bytes;

@@ -232,3 +232,37 @@ def test_a_saved_state_that_moved_is_seen():
     clear.reorder_states([state], torch.tensor([[1, 0]], dtype=torch.int32, device="cuda"))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("B,width", [(4, 2), (8, 1), (32, 5), (2, 3), (1, 4), (3, 32)])
+def test_states_follow_into_another_number_of_beams(B, width):
+    """A choice that keeps fewer beams, or more, than there were: the states in the first rows, or slots, of each
+    request; the other rows as they were."""
+    from fhemamba_amd import clear
+
+    gen = torch.Generator().manual_seed(B)
+    R, pitch = 3, max(B, width)
+    cache = R * pitch + 2
+    choice = clear.beam_select(torch.randn(R, B, 50, generator=gen).cuda(), torch.randn(R, B, generator=gen).cuda(), width)
+    for slots in (None, torch.randperm(cache, generator=gen)[: R * pitch].reshape(R, pitch).to(torch.int32)):
+        states = [torch.randn(cache, 3, 8, generator=gen), torch.randn(cache, 7, generator=gen).to(BF)]
+        at = torch.arange(R * pitch).reshape(R, pitch) if slots is None else slots.long()
+        mine = [s.cuda() for s in states]
+        clear.reorder_states(mine, choice.parent, beams=B, slots=None if slots is None else slots.cuda())
+        for got, s in zip(mine, states):
+            want = s.clone()
+            for r in range(R):
+                for j in range(width):
+                    want[at[r, j]] = s[at[r, int(choice.parent[r, j])]]
+            assert torch.equal(got.cpu(), want)
+    state = torch.randn(6, 4, device="cuda")  # a parent that is no beam of those that were
+    want = state[[1, 0, 2, 3, 4, 3]].clone()
+    clear.reorder_states(state, torch.tensor([[1, 0, 2], [0, -1, 0]], dtype=torch.int32, device="cuda"), beams=2)
+    assert torch.equal(state, want)
+    state, parent = torch.zeros(12, 4, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    for call, match in [(lambda: clear.reorder_states(state, parent, beams=33), "32 beams"),
+                        (lambda: clear.reorder_states(state, parent, beams=0), "32 beams"),
+                        (lambda: clear.reorder_states(state, parent, beams=7), "14 beams and 12 rows"),
+                        (lambda: clear.reorder_states(state, parent, beams=4, slots=parent), "shape")]:
+        with pytest.raises(ValueError, match=match):
+            call()
