@@ -1,7 +1,9 @@
 // extern "C" boundary of the operators in the clear (include/fhecore.h):
 // validation of everything that the host can see, and their descriptors as the
 // kernels take them.
+#include <algorithm>
 #include <cstdint>
+#include <functional>
 #include <vector>
 
 #include "clear.hpp"
@@ -598,6 +600,15 @@ int fhe_reorder_states(const fhe_state_rows* states, uint32_t count, uint32_t re
       need(states[i].data || !states[i].row_bytes, "null state");
       need(states[i].row_bytes >= 0 && states[i].row_bytes <= (1 << 30), "row_bytes must be 0 .. 2^30");
       moved.push_back({states[i].data, states[i].row_bytes});
+    }
+    // two threads would move the same bytes
+    std::vector<clear::Moved> by_place = moved;
+    std::sort(by_place.begin(), by_place.end(), [](auto& a, auto& b) { return std::less<>()(a.state, b.state); });
+    const char* end = nullptr;
+    for (const clear::Moved& m : by_place) {
+      if (!m.row_bytes) continue;
+      need(!std::less<>()((const char*)m.state, end), "two of the states share memory");
+      end = (const char*)m.state + m.row_bytes * cache;
     }
     clear::reorder_states(moved.data(), (int)count, (int)requests, (int)beams, (int)cache, parent, slots,
                           (hipStream_t)hip_stream);

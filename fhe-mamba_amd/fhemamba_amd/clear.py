@@ -870,12 +870,13 @@ def beam_select(logits, scores, width: Optional[int] = None, *, finished=None, e
 def reorder_states(states, parent, *, slots=None, beams: Optional[int] = None) -> None:
     """The states follow their beams, in place: row slots[r, j] takes what row slots[r, parent[r, j]] held.
 
-    states: a tensor [cache, ..] or a sequence of them with as many rows, of any type, contiguous.  parent
-    [requests, width] int32 as beam_select gives it; `beams` (at most 32) is how many beams each request had
-    before, which beam_select's caller has to say where that is not the width.  slots [requests, the larger of
-    width and beams] (default: rows in order, as many for each request), no row twice: the first `width` of
-    them are written, the others stay as they were.  A parent that is no beam leaves the row as it is; a slot
-    outside of the cache is padding.  A backward pass that needs a state as it was before raises."""
+    states: a tensor [cache, ..] or a sequence of them with as many rows, of any type, contiguous, none of
+    which shares memory with another.  parent [requests, width] int32 as beam_select gives it; `beams` (at
+    most 32) is how many beams each request had before, to be given where that is not the width.  slots
+    [requests, the larger of width and beams] (default: rows in order, as many for each request), no row
+    twice: the first `width` of them are written, the others stay as they were.  A parent that is no beam
+    leaves the row as it is; a slot outside of the cache is padding.  A backward pass that needs a state as
+    it was before raises."""
     states = (states,) if isinstance(states, torch.Tensor) else tuple(states)
     if not states:
         raise ValueError("no states")

@@ -623,11 +623,12 @@ int fhe_beam_select(const fhe_beam_args *args, const fhe_beam_out *out,
 
 /* Rows follow their beams in place: row slots[r][j] of every state takes what row
  * slots[r][parent[r][j]] held before the call.  states [count]: an array on the
- * host; each has `cache` contiguous rows of row_bytes <= 2^30.  parent [requests]
- * [beams] and slots (device; slots NULL: r * beams + j).  A parent outside of
- * [0, beams) leaves the row as it is, a slot outside of [0, cache) is padding.  No
- * row may be named twice.  `beams` counts the beams before and after: behind a
- * choice of fewer (its width less than its beams) parent goes on with -1. */
+ * host; each has `cache` contiguous rows of row_bytes <= 2^30, and no two share
+ * memory.  parent [requests][beams] and slots (device; slots NULL: r * beams + j).
+ * A parent outside of [0, beams) leaves the row as it is, a slot outside of
+ * [0, cache) is padding.  No row may be named twice.  `beams` counts the beams
+ * before and after: behind a choice of fewer (its width less than its beams) parent
+ * goes on with -1. */
 typedef struct {
   void *data;
   int64_t row_bytes;

@@ -231,3 +231,12 @@ def test_tensors_off_the_gpu_are_refused():
                  lambda: clear.reorder_states(z(2, 8), z(1, 2, dtype=torch.int32))):
         with pytest.raises(ValueError, match="on the GPU"):
             call()
+
+
+@pytest.mark.parametrize("states", [[(4096, 64), (4096, 64)], [(8192, 16), (4096, 64), (4096 + 6 * 64 - 1, 4)],
+                                    [(4096, 64), (4096 + 64, 8)]])
+def test_states_that_share_memory_are_refused(states):
+    """Rows of one that are rows of another would be moved twice, at once."""
+    packed = b"".join(clear._ROWS.pack(*s) for s in states)
+    with pytest.raises(ValueError, match="share memory"):
+        _lib.call("fhe_reorder_states", packed, len(states), 2, 3, 6, 4096, 0, 0)
