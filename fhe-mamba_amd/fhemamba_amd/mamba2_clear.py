@@ -59,6 +59,16 @@ def _project(x: torch.Tensor, weight, bias=None) -> torch.Tensor:
     return out if bias is None else (out.float() + bias).to(x.dtype)
 
 
+def _next_norm(hidden, update, weight, eps: float, dtype: torch.dtype) -> tuple:
+    """(the norm of hidden + update in dtype, the sum); no update yet: None."""
+    if hidden.dtype == torch.float64:  # a caller's own: the kernels' streams are of 32 bits or 16
+        hidden = hidden if update is None else hidden + update
+        return (hidden * torch.rsqrt(hidden.square().mean(-1, keepdim=True) + eps) * weight).to(dtype), hidden
+    if update is None:
+        return clear.rms_norm(hidden, weight, eps=eps, dtype=dtype), hidden
+    return clear.add_norm(hidden, update, weight, eps=eps)
+
+
 def _table(values, dtype: torch.dtype, device, int8: bool):
     if int8:
         return clear.quantize_rows(torch.as_tensor(values, dtype=torch.float32, device=device))
@@ -139,23 +149,21 @@ class ClearMamba2:
         return out
 
     def _run(self, hidden, states, mixer) -> tuple:
-        """Residual stream [.., d_model] -> (final normed hidden, states), both of 32 bits."""
-        hidden, update, out = hidden.float(), None, []
+        """Residual stream [.., d_model] -> (final normed hidden, states), both of 32 bits; a stream of 64 stays one."""
+        hidden = hidden if hidden.dtype == torch.float64 else hidden.float()
+        update, out = None, []
         for i, lay in enumerate(self.layers):
-            w, eps = lay.weights["block_norm_w"], lay.shape.eps_block
-            if update is None:
-                normed = clear.rms_norm(hidden, w, eps=eps, dtype=self.dtype)
-            else:
-                normed, hidden = clear.add_norm(hidden, update, w, eps=eps)
+            normed, hidden = _next_norm(hidden, update, lay.weights["block_norm_w"], lay.shape.eps_block, self.dtype)
             update, state = lay(normed, None if states is None else states[i], mixer)
             out.append(state)
-        if update is None:
-            return clear.rms_norm(hidden, self.norm_w, eps=self.norm_eps), out
-        return clear.add_norm(hidden, update.float(), self.norm_w, eps=self.norm_eps).normed, out
+        if update is not None:
+            update = update.float()
+        return _next_norm(hidden, update, self.norm_w, self.norm_eps, hidden.dtype)[0], out
 
     def forward(self, embeddings, states=None, *, cu_seqlens=None) -> tuple:
         """Whole sequences [sequences, tokens, d_model] float32, or packed [tokens, d_model] with cu_seqlens,
-        from `states` (default zeros): (final normed hidden, the states behind the last tokens)."""
+        from `states` (default zeros): (final normed hidden, the states behind the last tokens).  Embeddings of
+        float64 make a residual stream, its norms and the result of 64 bits; what a layer adds is of 32 or 16."""
         def mixer(lay, inputs, write, log_decay, state):
             conv, last = clear.causal_conv(inputs, lay.weights["conv_w"], lay.weights["conv_b"],
                                            initial_state=None if state is None else state.conv,
