@@ -201,9 +201,31 @@ class ClearMamba2:
         """Log probabilities of target tokens, entropies and likeliest tokens at each hidden vector."""
         return clear.token_logprobs(self.logits(hidden), targets, top=top)
 
+    def _rows(self, ids):
+        """Rows of the embeddings' table: ids below 0 count from its end.  Those that then are below 0 still become very
+        large numbers: no row, rather than padding."""
+        if ids.dtype != torch.int64:
+            raise ValueError(f"ids must be of type torch.int64, not {ids.dtype}")
+        return torch.where(ids < 0, (ids + self.embedding.shape[0]) & (2 ** 63 - 1), ids)
+
     def embed(self, ids):
-        """Embeddings of token ids; those below 0 count from the table's end."""
-        return clear.embed(self.embedding, torch.where(ids < 0, ids + self.embedding.shape[0], ids))
+        """Embeddings of token ids; those below 0 count from the table's end.  One outside of it gives NaN."""
+        return clear.embed(self.embedding, self._rows(ids))
+
+    def _check(self, rows):
+        """Starts to look for rows that the table does not have; a call of what is returned waits for the answer, not
+        for work begun in between, and raises ValueError.  A capture waits for nothing: no check in there."""
+        if rows.numel() == 0 or torch.cuda.is_current_stream_capturing():
+            return lambda: None
+        largest = torch.empty((), dtype=torch.int64, pin_memory=True)
+        largest.copy_(rows.max(), non_blocking=True)
+        answered = torch.cuda.current_stream(rows.device).record_event()
+
+        def wait():
+            answered.synchronize()
+            if largest >= self.embedding.shape[0]:
+                raise ValueError(f"ids outside of the table of {self.embedding.shape[0]} embeddings")
+        return wait
 
     @torch.no_grad()
     def beam_search(self, ids, steps: int, *, beams: int = 4, end: Optional[int] = None, cu_seqlens=None) -> BeamResult:
@@ -211,12 +233,14 @@ class ClearMamba2:
 
         ids [requests, tokens], or packed [tokens] with cu_seqlens, each prompt one token or more.  A beam that
         has taken the token `end` goes on with it at no cost.  The score is the sum of the tokens' log
-        probabilities."""
+        probabilities.  Ids outside of the table raise ValueError."""
         if self.head is None:
             raise ValueError("the payload has no client head")
         if steps < 1 or ids.shape[-1] < 1:
             raise ValueError("steps must be 1 or more, and so must a prompt's tokens")
-        hidden, states = self.forward(self.embed(ids), cu_seqlens=cu_seqlens)
+        rows = self._rows(ids)
+        self._check(rows)()
+        hidden, states = self.forward(clear.embed(self.embedding, rows), cu_seqlens=cu_seqlens)
         last = hidden[:, -1] if cu_seqlens is None else hidden[cu_seqlens[1:].long() - 1]
         requests = last.shape[0]
         score, parent, token = clear.beam_select(self.logits(last).unsqueeze(1), last.new_zeros(requests, 1), beams)
@@ -225,7 +249,7 @@ class ClearMamba2:
         tokens = token.long().unsqueeze(-1)
         finished = None if end is None else token == end
         for _ in range(steps - 1):
-            hidden = self.step(self.embed(tokens[..., -1].reshape(-1)), states)
+            hidden = self.step(clear.embed(self.embedding, tokens[..., -1].reshape(-1)), states)
             score, parent, token = clear.beam_select(self.logits(hidden).unflatten(0, (requests, beams)), score,
                                                      finished=finished, end=end)
             clear.reorder_states(held, parent)
@@ -237,8 +261,11 @@ class ClearMamba2:
 
     def loss(self, ids, *, cu_seqlens=None):
         """Mean negative log probability of each token's successor; ids [sequences, tokens], or packed, where
-        tokens outside of every sequence take no part."""
-        hidden, _ = self.forward(self.embed(ids), cu_seqlens=cu_seqlens)
+        tokens outside of every sequence take no part.  Ids outside of the table raise ValueError, for which the
+        call waits until the GPU has seen them (in a capture: NaN)."""
+        rows = self._rows(ids)
+        checked = self._check(rows)
+        hidden, _ = self.forward(clear.embed(self.embedding, rows), cu_seqlens=cu_seqlens)
         targets = torch.cat([ids[..., 1:], torch.full_like(ids[..., :1], -1)], dim=-1)
         if cu_seqlens is not None:  # neither a sequence's last token nor one outside of all has a successor
             begins, ends = cu_seqlens[:-1].long(), cu_seqlens[1:].long()
@@ -246,6 +273,7 @@ class ClearMamba2:
             own = torch.searchsorted(ends, at, right=True).clamp(max=ends.shape[0] - 1)  # the first that ends behind it
             targets = torch.where((at >= begins[own]) & (at + 1 < ends[own]), targets, -1)
         scored = self.score(hidden, targets).logprob
+        checked()
         return -scored.sum() / (targets >= 0).sum().clamp(min=1)
 
 

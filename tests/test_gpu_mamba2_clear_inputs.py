@@ -42,3 +42,46 @@ def test_a_stream_of_64_bits_stays_one(chain, dtype):
     (g,) = torch.autograd.grad(got, leaf, way.cuda())
     # two sums of some tens of terms each, 2^-53 a term
     assert float((g.cpu() - e).norm() / e.norm()) <= 1e-13
+
+
+def test_ids_outside_of_the_table_are_refused(chain):
+    from fhemamba_amd import mamba2_clear as C
+
+    model, vocab = C.ClearMamba2(chain), chain.autoregressive.vocab
+    good = torch.tensor([[1, 0, vocab - 1], [-1, 2, -vocab]], device="cuda")
+    cu = torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda")
+    assert bool(torch.isfinite(model.loss(good))) and bool(torch.isfinite(model.loss(good.reshape(-1), cu_seqlens=cu)))
+    found = model.beam_search(good, 2, beams=2)
+    for bad in (vocab, -vocab - 1, 2 ** 62, -2 ** 63):
+        ids = good.clone()
+        ids[1, 1] = bad
+        for call in (lambda: model.loss(ids), lambda: model.loss(ids.reshape(-1), cu_seqlens=cu),
+                     lambda: model.beam_search(ids, 2, beams=2),
+                     lambda: model.beam_search(ids.reshape(-1), 2, beams=2, cu_seqlens=cu)):
+            with pytest.raises(ValueError, match="outside of the table"):
+                call()
+        rows = model.embed(ids)  # without a wait: no row of the table, and none of zeros
+        assert bool(torch.isnan(rows[1, 1]).all()) and torch.equal(rows[0], model.embed(good[0]))
+    again = model.beam_search(good, 2, beams=2)
+    assert torch.equal(found.tokens, again.tokens) and torch.equal(found.score, again.score)
+
+
+def test_captured_loss(chain):
+    """A capture waits for nothing: there the ids are not looked at."""
+    from fhemamba_amd import mamba2_clear as C
+
+    model, vocab = C.ClearMamba2(chain), chain.autoregressive.vocab
+    ids = torch.tensor([[1, 2, 0, 3]], device="cuda") % vocab
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        model.loss(ids)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        loss = model.loss(ids)
+    for turn in range(3):
+        ids.copy_((ids + 1) % vocab)
+        graph.replay()
+        with torch.no_grad():
+            assert torch.equal(loss, model.loss(ids))
