@@ -233,13 +233,20 @@ class ClearMamba2:
 
         ids [requests, tokens], or packed [tokens] with cu_seqlens, each prompt one token or more.  A beam that
         has taken the token `end` goes on with it at no cost.  The score is the sum of the tokens' log
-        probabilities.  Ids outside of the table raise ValueError."""
+        probabilities.  Prompts without a token and ids outside of the table raise ValueError, for which the call
+        waits for the GPU before the search (not in a capture)."""
         if self.head is None:
             raise ValueError("the payload has no client head")
         if steps < 1 or ids.shape[-1] < 1:
             raise ValueError("steps must be 1 or more, and so must a prompt's tokens")
         rows = self._rows(ids)
-        self._check(rows)()
+        checked = self._check(rows)
+        if cu_seqlens is not None and not torch.cuda.is_current_stream_capturing():
+            clear._offsets(cu_seqlens, ids)
+            ends = cu_seqlens.tolist()
+            if ends[0] < 0 or ends[-1] > ids.shape[0] or any(a >= b for a, b in zip(ends, ends[1:])):
+                raise ValueError(f"cu_seqlens must give each prompt one token or more of the {ids.shape[0]}")
+        checked()
         hidden, states = self.forward(clear.embed(self.embedding, rows), cu_seqlens=cu_seqlens)
         last = hidden[:, -1] if cu_seqlens is None else hidden[cu_seqlens[1:].long() - 1]
         requests = last.shape[0]

@@ -66,6 +66,16 @@ def test_ids_outside_of_the_table_are_refused(chain):
     assert torch.equal(found.tokens, again.tokens) and torch.equal(found.score, again.score)
 
 
+@pytest.mark.parametrize("ends", [[0, 0, 3], [0, 3, 3], [0, 1, 1, 3], [2, 1, 3], [0, 4], [-1, 3]])
+def test_prompts_without_a_token_are_refused(chain, ends):
+    from fhemamba_amd import mamba2_clear as C
+
+    model = C.ClearMamba2(chain)
+    ids = torch.tensor([1, 2, 0], device="cuda")
+    with pytest.raises(ValueError, match="one token or more"):
+        model.beam_search(ids, 2, beams=2, cu_seqlens=torch.tensor(ends, dtype=torch.int32, device="cuda"))
+
+
 def test_captured_loss(chain):
     """A capture waits for nothing: there the ids are not looked at."""
     from fhemamba_amd import mamba2_clear as C
