@@ -7,13 +7,13 @@
 // alone, at its score; a beam of score -inf with none.  The `width` largest of a
 // request's totals, the lower beam and then the lower token first among equals.
 // A beam's best tokens are those of its logits, so each row's are found as the
-// likeliest tokens are, and beams times width candidates remain of a request.  Totals
-// are of 64 bits, and so are the sums above a thread's 16 terms: which of two near
-// totals of different beams is larger should not depend on how a row was cut.  Rows
-// are cut by columns whatever their alignment, so that equal beams have equal totals.
-// Four beams of 50280 tokens take 6 + 8 + 2 us, the chains of three launches; 256 beams
-// in 16 bits with a third of them masked 18 + 8 + 5, the first bound by its vector
-// instructions as the likeliest tokens' is.
+// likeliest tokens are, and beams times width candidates remain of a request.
+// Exponentials, sums and totals are of 64 bits: which of two near totals of different
+// beams is larger should depend neither on 32 bits' rounding nor on how a row was cut.
+// Rows are cut by columns whatever their alignment, so that equal beams have equal
+// totals.  Four beams of 50280 tokens take 6 + 8 + 2 us, the chains of three launches;
+// 256 beams in 16 bits with a third of them masked 18 + 8 + 5, the first bound by its
+// vector instructions as the likeliest tokens' is.
 #pragma clang fp contract(fast)
 #include <algorithm>
 
@@ -42,6 +42,24 @@ struct BeamArgs {
   double* total;       // [rows][list]
   int* token;
 };
+
+// e^d for d <= 0, to 2^-45 of it, the library's function in half of its instructions: 2^n 2^f
+// with n the integer nearest to d log2 e and 2^f from the polynomial that meets it at the ten
+// Chebyshev nodes of [-1/2, 1/2].  Below -700, and for -inf, as at -700, which is nothing
+// beside the largest term's 1.
+__device__ __forceinline__ double exp_low(double d) {
+  constexpr double LOG2_E = 1.4426950408889634, INTEGER = 0x1.8p52;
+  constexpr double C[10] = {0x1.000000000003dp+0,  0x1.62e42fefa39f7p-1,  0x1.ebfbdff8149f2p-3,  0x1.c6b08d7044119p-5,
+                            0x1.3b2ab72b175eep-7,  0x1.5d87fe908f88ap-10, 0x1.43088e257f341p-13, 0x1.ffcb76789860fp-17,
+                            0x1.63ef969a64d3cp-20, 0x1.b6571de2f2351p-24};
+  d = fmax(d, -700.0);
+  const double s = __builtin_fma(d, LOG2_E, INTEGER), f = __builtin_fma(d, LOG2_E, INTEGER - s);
+  double p = C[9];
+#pragma unroll
+  for (int i = 8; i >= 0; --i) p = __builtin_fma(p, f, C[i]);
+  // n lies in the low bits of s, and goes to the exponent
+  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + (__builtin_bit_cast(uint64_t, s) << 52));
+}
 
 __device__ __forceinline__ double raise(float m, float most, double s) {
   return s == 0.0 ? 0.0 : s * exp((double)m - (double)most);
@@ -83,7 +101,8 @@ __global__ __launch_bounds__(THREADS) void k_beam_parts(BeamArgs a) {
     float v[16];
     x.widen(v);
     if (t + 1 < a.tiles) x.template read<false>(row, base + TILE, a.b.vocab);  // in flight meanwhile
-    float most = m, sum = 0.0f;
+    float most = m;
+    double sum = 0.0;
     bool nan = false;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -93,7 +112,7 @@ __global__ __launch_bounds__(THREADS) void k_beam_parts(BeamArgs a) {
     if (nan) most = NAN;
     if (most != -INFINITY) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum += __builtin_amdgcn_exp2f((v[j] - most) * LOG2E);
+      for (int j = 0; j < 16; ++j) sum += exp_low((double)v[j] - (double)most);
       s = raise(m, most, s) + sum;
       m = max_nan(m, most);
     }

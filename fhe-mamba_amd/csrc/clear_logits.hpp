@@ -25,6 +25,11 @@ struct Sixteen {
   }
   template <bool ALIGNED>
   __device__ __forceinline__ void read(const T* row, int64_t base, int64_t vocab) {
+    if (!ALIGNED && base >= 0 && base + TILE <= vocab) {  // all pieces on their way at once
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) __builtin_memcpy(&w[p], row + column(base, p * VEC), 16);
+      return;
+    }
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int64_t c = column(base, p * VEC);

@@ -833,8 +833,8 @@ def beam_select(logits, scores, width: Optional[int] = None, *, finished=None, e
 
     logits [requests, beams, vocab] (at most 32 beams) and scores [requests, beams] float32: a candidate is
     a beam and a token, its score the beam's plus the token's log probability; the lower beam, then the
-    lower token first among equals.  Two beams' scores are told apart from a difference of about 2^-24 on.
-    A beam of score -inf has none.  finished [requests, beams] bool: such
+    lower token first among equals.  Scores are 64-bit numbers, of two beams good to about 2^-40, until they
+    are rounded for the result.  A beam of score -inf has none.  finished [requests, beams] bool: such
     a beam has the one candidate `end`, at its own score.  Where fewer candidates are allowed, others
     follow with score -inf.  A NaN or +inf among a live beam's logits, or for a score, makes the beam's
     candidates NaN, which come first.  No gradient (token_logprobs at the chosen tokens has one).  Where the

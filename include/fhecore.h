@@ -598,8 +598,8 @@ int fhe_embed_backward(const fhe_embed_args *args, const fhe_rows *dy,
 /* A step of a beam search: of all candidates (beam, token) of a request, which
  * have the beam's score plus the token's log probability, the `width` <=
  * FHE_MAX_TOP largest, in order, the lower beam and then the lower token first
- * among equals (scores of two beams are told apart from a difference of about
- * 2^-24 on): score, parent and token [requests][width].  logits
+ * among equals (scores are 64-bit numbers, good to about 2^-40, until they are
+ * rounded for the result): score, parent and token [requests][width].  logits
  * [requests * beams][vocab], row_stride elements apart; beams <= FHE_MAX_TOP,
  * width <= beams * vocab.  A finished beam (finished may be NULL) has the one
  * candidate `end`, at its own score; its logits are not read, nor those of a beam

@@ -266,3 +266,39 @@ def test_states_follow_into_another_number_of_beams(B, width):
                         (lambda: clear.reorder_states(state, parent, beams=4, slots=parent), "shape")]:
         with pytest.raises(ValueError, match=match):
             call()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("V", [40, 300, 5000, 50280])
+def test_beams_whose_totals_are_near(V, dtype):
+    """Two beams with the same logits in another order, but one: their best tokens' totals differ by 2^-33 at least
+    and 2^-28 at most, either way, which the reference's sums, good to 2^-44, tell apart."""
+    R = 60
+    gen = torch.Generator().manual_seed(V)
+    logits, scores = make(V, R, 2, V, dtype)
+    for r in range(R):
+        logits[r, 1] = logits[r, 0][torch.randperm(V, generator=gen)]
+        sums = torch.exp(logits[r, 0].double()).sum().item()
+        # one token of one of the beams gives way: its part of the sum is what the totals differ by
+        want = sums * 2.0 ** (-33 + 5 * float(torch.rand((), generator=gen)))
+        both = [logits[r, b].argmin() for b in range(2)]
+        for b in range(2):
+            logits[r, b, both[b]] = -math.inf
+        logits[r, r % 2, both[r % 2]] = math.log(want)
+    scores[:] = -2.0
+    totals = logits.double().log_softmax(-1).amax(-1)
+    apart = (totals[:, 0] - totals[:, 1]).abs()
+    assert bool((apart > 2.0 ** -34).all()) and bool((apart < 2.0 ** -27).all())
+    compare(logits, scores, 2)
+
+
+def test_logits_far_apart():
+    """One token far above the others of its thread and row, at any size: the sum is its own 1."""
+    for top in (50.0, 800.0, 1e5, 1e30):
+        for V in (3, 500, 5000):
+            logits, scores = make(V, 4, 2, V, F32)
+            logits[0, 0, 1], logits[1, 1, 0], logits[2, 0, 2], logits[3, :, V - 1] = top, top, top, top
+            logits[2, 1] = -top
+            compare(logits, scores, 1)
+            if top <= 1e5:  # of 1e30 numbers of 64 bits keep nothing smaller than 1e14: the others would be ties there
+                compare(logits, scores, 3)
