@@ -155,3 +155,32 @@ def test_refusals():
                         (lambda: clear.embed(w, ids, scale=float("inf")), "finite")]:
         with pytest.raises(ValueError, match=match):
             call()
+
+
+def ids_of(counts):
+    return torch.cat([torch.full((n,), 3 * i, dtype=torch.int64) for i, n in enumerate(counts)])
+
+
+# 129 to 32768 tokens are cut into pieces of 32: a row of as many, one more and one less, at a piece's begin, at its
+# end and across it
+@pytest.mark.parametrize("counts", [(32,) * 5, (33,) * 5, (31,) * 6, (32, 33, 31, 64, 65, 63, 96), (1, 31, 32, 33, 32, 96),
+                                    (1, 32, 31, 32, 33, 31, 40), (16, 32, 16, 33, 63, 64, 65), (31, 33, 31, 33, 1, 64),
+                                    (95, 33, 32, 97, 1), (32, 0, 160, 32), (128, 1, 128, 31, 1)])
+def test_rows_as_long_as_a_piece(counts):
+    ids = ids_of(counts)
+    assert 128 < len(ids) <= 32768
+    gen = torch.Generator().manual_seed(len(ids))
+    weight = torch.randn(3 * len(counts) + 2, 70, generator=gen)
+    compare(weight, ids, 1.0)
+    compare(weight, ids[torch.randperm(len(ids), generator=gen)], 1.0)
+    compare(weight.to(BF), torch.cat([ids, torch.full((9,), -1)]), 2.0)
+
+
+@pytest.mark.parametrize("last,piece", [(1, 63), (500, 64)])
+def test_rows_as_long_as_a_longer_piece(last, piece):
+    """Over 64000 tokens: rows of one less, as many and one more."""
+    counts = [62, 63, 64, 65, 1, 62, 63, 126, 127, 128, 129] * 72 + [last]
+    ids = ids_of(counts)
+    assert (len(ids) + 1023) // 1024 == piece
+    weight = torch.randn(3 * len(counts), 12, generator=torch.Generator().manual_seed(last))
+    compare(weight, ids, 1.0)
