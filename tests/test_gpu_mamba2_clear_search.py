@@ -152,3 +152,30 @@ def test_refusals(chain):
         bare.beam_search(ids, 2)
     with pytest.raises(ValueError, match="client head"):
         C.run(M.read_chain_payload(os.path.join(GOLDEN, "m2_chain_tiny")), beams=2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_model_in_8_bits_is_the_model_of_its_integers(chain, dtype, monkeypatch):
+    """The same layers with the plain form of each 8-bit product.  The two round alike but where a quotient lies within
+    32 bits' rounding of the middle of two integers, which moves one entry of a row by a 127th of the largest."""
+    import layer_reference as L
+    from fhemamba_amd import clear, mamba2_clear as C
+
+    model = C.ClearMamba2(chain, dtype, int8=True)
+    ids = torch.randint(0, chain.autoregressive.vocab, (3, 11), generator=torch.Generator().manual_seed(5)).cuda()
+
+    def plain(x, weight, scale, bias=None):
+        rows = x.cpu().reshape(-1, x.shape[-1])
+        y = L.int8_linear(rows, weight.cpu(), scale.cpu(), None if bias is None else bias.cpu())
+        return y.to(x.dtype).cuda().reshape(*x.shape[:-1], -1)
+
+    with torch.no_grad():
+        got = model.forward(model.embed(ids))[0]
+        logits = model.logits(got)
+        monkeypatch.setattr(clear, "int8_linear", plain)
+        want = model.forward(model.embed(ids))[0]
+        assert float((got - want).norm() / want.norm()) <= 2.0 ** -7
+        want = model.logits(got)
+        # each from the same hidden vectors: exact sums, then two 32-bit products and the type's rounding
+        off = 2.0 ** -8 if dtype == torch.bfloat16 else 4 * 2.0 ** -24
+        assert float((logits.float() - want.float()).norm() / want.float().norm()) <= 2 * off
