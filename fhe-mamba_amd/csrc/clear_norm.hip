@@ -37,15 +37,25 @@ struct NormArgs {
   float eps;
 };
 
-// 1 / (1 + e^-v).  The product -v log2 e is rounded to 32 bits, up to 2^-18 off at v = -80,
-// which would be as much of a closed gate; what the rounding took off, and the constant's own,
-// goes in as a factor.  2^x and the reciprocal are the hardware's, good to a unit.
+// 1 / (1 + e^-v) of a gate in T.  The product -v log2 e rounded to 32 bits would be up to
+// 2^-18 off at v = -80, and a closed gate as much of itself; so what is missing from it goes
+// in as a factor.  For 16 bits that is one instruction: eight bits of v times sixteen of
+// log2 e are exact, and the rest of log2 e times v is 2^-11 or less, its square nothing.
+// 2^x and the reciprocal are the hardware's, good to a unit.
+template <class T>
 __device__ __forceinline__ float sigmoid(float v) {
   constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
-  constexpr float HIGH = (float)LOG2E, LOW = (float)((LOG2E - (double)HIGH) * LN2);
-  v = __builtin_amdgcn_fmed3f(v, -128.0f, 128.0f);  // 0 or 1 beyond
-  const float x = v * -HIGH, off = __builtin_fmaf(v, -HIGH, -x);
-  const float factor = __builtin_fmaf(v, -LOW, __builtin_fmaf(off, (float)LN2, 1.0f));
+  float x, factor;
+  if constexpr (sizeof(T) == 2) {
+    constexpr float HIGH = 47274.0f / 32768.0f, LOW = (float)((LOG2E - (double)HIGH) * LN2);
+    x = v * -HIGH;
+    factor = __builtin_fmaf(v, -LOW, 1.0f);
+  } else {
+    constexpr float HIGH = (float)LOG2E, LOW = (float)((LOG2E - (double)HIGH) * LN2);
+    v = __builtin_amdgcn_fmed3f(v, -128.0f, 128.0f);  // 0 or 1 beyond
+    x = v * -HIGH;
+    factor = __builtin_fmaf(v, -LOW, __builtin_fmaf(__builtin_fmaf(v, -HIGH, -x), (float)LN2, 1.0f));
+  }
   return __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_exp2f(x), factor, 1.0f));
 }
 
@@ -99,9 +109,12 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm(NormArgs p) {
       raw_a[k] = piece[k].raw(a);
       if constexpr (MODE != PLAIN) raw_b[k] = piece[k].raw(b);
     }
-    // all on their way: left to itself the compiler may widen each before the next is
-    // asked for (a call of 30011 rows of 1536 with a gate in bfloat16: 72 us for 51)
-    __builtin_amdgcn_sched_barrier(0);
+    // All on their way: left to itself the compiler may widen each before the next is asked
+    // for (a call of 30011 rows of 1536 with a gate in bfloat16: 72 us for 51).  Where
+    // several wavefronts have a row and the last pieces are moved it does not, and its own
+    // order is better (2^25 elements in rows of 2048: 43 us for 45; of 16384, not moved, 38
+    // for 32).
+    if constexpr (W == 1 || COVER == WHOLE) __builtin_amdgcn_sched_barrier(0);
     f32x4 v[PER], other[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
@@ -117,7 +130,7 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm(NormArgs p) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (MODE == GATED) v[k][i] *= other[k][i] * sigmoid(other[k][i]);
+        if constexpr (MODE == GATED) v[k][i] *= other[k][i] * sigmoid<B>(other[k][i]);
         s[0] += piece[k].mine(i, v[k][i] * v[k][i]);
       }
     }
@@ -167,7 +180,7 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
       for (int i = 0; i < 4; ++i) {
         float t = v[k][i];
         if constexpr (MODE == GATED) {
-          act[k][i] = other[k][i] * sigmoid(other[k][i]);
+          act[k][i] = other[k][i] * sigmoid<B>(other[k][i]);
           t *= act[k][i];
         }
         s[0] += piece[k].mine(i, t * t);
@@ -193,7 +206,7 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
         f32x4 dz;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float sig = sigmoid(other[k][i]);
+          const float sig = sigmoid<B>(other[k][i]);
           dz[i] = d[i] * v[k][i] * (sig + act[k][i] * (1.0f - sig));
         }
         piece[k].put((A*)p.db + at, dz);

@@ -366,3 +366,20 @@ def test_gates_at_the_ends_of_their_type():
     assert bool(torch.isfinite(got[0]).all()) and not bool(got[0, 4:].any()) and bool((got[0, :4] > 0).all())
     assert bool(torch.isnan(got[1]).all()) and bool(torch.isnan(got[2]).all())
     assert not bool(got[3:].any())
+
+
+@pytest.mark.parametrize("low,high", [(-8, -4), (-60, -40), (-85, -75), (-2, 2), (4, 40)])
+def test_gates_of_16_bits_element_by_element(low, high):
+    """The 28 steps of 2^-24 above beneath the rounding to 16 bits: half a step of the result's own size."""
+    from fhemamba_amd import clear
+
+    gen = torch.Generator().manual_seed(-low)
+    rows, channels = 400, 64
+    z = (low + (high - low) * torch.rand(rows, channels, generator=gen)).to(BF)
+    x = (torch.exp(-z.double().clamp(max=0)) * (1 + torch.rand(rows, channels, generator=gen))).to(BF)
+    w = 1 + torch.rand(channels, generator=gen)
+    got = clear.rms_norm(x.cuda(), w.cuda(), gate=z.cuda()).cpu().double()
+    want = L.norm(x.double(), w.double(), z.double(), 1, 1e-5)
+    step = torch.exp2(torch.floor(torch.log2(want.abs())) - 7)
+    over = ((got - want).abs() - step / 2) / want.abs()
+    assert over.max().item() * 2.0 ** 24 <= 28, over.max().item() * 2.0 ** 24
