@@ -11,9 +11,9 @@
 // Exponentials, sums and totals are of 64 bits: which of two near totals of different
 // beams is larger should depend neither on 32 bits' rounding nor on how a row was cut.
 // Rows are cut by columns whatever their alignment, so that equal beams have equal
-// totals.  Four beams of 50280 tokens take 6 + 8 + 2 us, the chains of three launches;
-// 256 beams in 16 bits with a third of them masked 18 + 8 + 5, the first bound by its
-// vector instructions as the likeliest tokens' is.
+// totals.  Four beams of 50280 tokens take 7 + 8 + 3 us, the chains of three launches;
+// 256 beams in 16 bits with a third of them masked 22 + 8 + 5, the first bound by its
+// vector instructions, the exponentials among them.
 #pragma clang fp contract(fast)
 #include <algorithm>
 
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(THREADS) void k_beam_parts(BeamArgs a) {
     if (base >= a.b.vocab) break;
     float v[16];
     x.widen(v);
-    if (t + 1 < a.tiles) x.template read<false>(row, base + TILE, a.b.vocab);  // in flight meanwhile
+    if (t + 1 < a.tiles) x.template read<false>(row, base + TILE, a.b.vocab);  // waited for in its branches
     float most = m;
     double sum = 0.0;
     bool nan = false;
@@ -200,8 +200,9 @@ __global__ __launch_bounds__(THREADS) void k_beam_pick(BeamArgs a) {
 // A thread has one piece of all the beams' rows of a request: it reads those that
 // move and then writes them, so that rows may change places without a copy, and a
 // beam that goes on where it lies costs nothing.  Bound by memory: 256 beams' states of
-// two layers, 0.8 MB each, take 126 us (5.7 TB/s), four beams' of 24 layers 21 us in one
-// launch.
+// two layers, 0.8 MB each, take 125 us (5.7 TB/s) in searches of eight, four beams' of 24
+// layers 22 us in one launch.  With more than eight beams the 16-byte pieces pass through
+// scratch memory, one load at a time: 3.2 TB/s in searches of 16, 2.5 of 32.
 constexpr int MAX_MOVED = 64;               // tensors of a launch
 constexpr uint32_t MAX_BLOCKS = 1u << 22;  // as many has a row of 2^30 bytes in the narrowest pieces
 

@@ -195,7 +195,8 @@ clear::Int8 to_int8(const fhe_int8_args* a) {
   p.rows = rows_of(a->rows);
   p.inputs = channels_of(a->inputs, FHE_MAX_ROW, "inputs must be 1 .. 32768");
   p.outputs = channels_of(a->outputs, 1 << 24, "outputs must be 1 .. 2^24");
-  // as many tiles of 16 outputs and 64 rows as a launch takes
+  // Below this the largest products, of 128 x 128 tiles or more, have fewer than 2^24 workgroups
+  // or tiles to number; a result has fewer than 2^34 elements.
   need((p.rows + 63) / 64 * ((a->outputs + 15) / 16) < (1 << 24), "too many outputs for one call");
   if (p.rows) p.x = rows_at(a->x, size);
   need(a->weight && a->scale, "null weight or scale");

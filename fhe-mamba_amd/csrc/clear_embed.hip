@@ -2,9 +2,11 @@
 //   y_t = scale weight[id_t];   dweight[v] = scale sum over t with id_t = v of dy_t
 // Bound by memory: the rows read, the rows written, and for the gradient, which
 // is dense, the whole table: 30011 tokens of 768 channels in 32 bits take 24 us, the
-// gradient of 8192 in a table of 50280 11 + 42 + 5 (3.8 TB/s of reads and writes in the
-// second of its kernels).  The gradient adds each row's tokens in their order,
-// so that equal inputs give equal bits; no atomic addition of floats:
+// gradient of 8192 in a table of 50280 11 + 43 + 5 (3.7 TB/s of reads and writes in the
+// second of its kernels).  The gradient adds each row's tokens in an order that the ids
+// fix, so that equal inputs give equal bits; no atomic addition of floats.  It is the
+// tokens' own order but for frequent rows, which are cut where pieces of the order of all
+// tokens end, so that their bits depend on how many tokens of lower ids there are:
 //   k_direct does all for few tokens; for more
 //   k_sort   a workgroup for each 256 rows of the table reads all ids, counts those
 //            of its rows and those before them, and writes its tokens in order of
@@ -169,7 +171,9 @@ struct SumArgs {
 };
 
 constexpr int COLUMNS = 4;  // pieces of 256 channels at a time
-constexpr int LOADS = 4;    // tokens whose rows are in flight
+// Tokens whose rows are asked for together.  In 32 bits all of them are in flight; in 16
+// the widening stands in the branch on the channel, and each 256 channels are waited for.
+constexpr int LOADS = 4;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 

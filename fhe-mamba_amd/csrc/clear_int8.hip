@@ -4,7 +4,7 @@
 // The sums are of 32-bit integers and exact.  The quotient is rounded to 32 bits
 // before it is rounded to an integer (even among equals), so that q is the same
 // on any machine with IEEE division.  Few rows are bound by the weights' bytes: one
-// row of 768 inputs and 50280 outputs takes 10.5 us (3.7 TB/s).  Many are bound by the
+// row of 768 inputs and 50280 outputs takes 11 us (3.5 TB/s).  Many are bound by the
 // way through LDS, the matrix units and the bytes of y together: 30011 rows of 768
 // inputs and 3352 outputs in bfloat16 take 20 us to round (3.5 TB/s) and 104 to
 // multiply (1.48 POP/s), 8192 rows of 8192 inputs and outputs 476 (2.31 POP/s).
@@ -244,7 +244,9 @@ __global__ __launch_bounds__(256) void k_fewest(ProductArgs p, const O* x, int64
 }
 
 // Few rows: a workgroup has 16 outputs and MT times 16 rows, its four wavefronts
-// a part of the summed index each; operands straight from memory.
+// a part of the summed index each; operands straight from memory.  A step's operands
+// are waited for before its products, in a chain of six for 1536 inputs: 250 rows of
+// those and 768 outputs take 7.6 us, their bytes 0.5.
 template <class O, int MT, bool WIDE>
 __global__ __launch_bounds__(256) void k_few(ProductArgs p) {
   __shared__ i32x4 lds[3][MT][64];
@@ -283,9 +285,9 @@ __global__ __launch_bounds__(256) void k_few(ProductArgs p) {
 // ----------------------------------------------------------------- many rows
 // Tiles of WM WN wavefronts, 16 MI rows and 64 outputs each, STEP indices at a time.
 // 256 x 256 in eight wavefronts need the fewest bytes from the caches and from LDS for
-// a product: 30011 x 768 x 3352 takes 123 us of them, 129 of 192 x 256, 133 of 128 x
-// 256 or 256 x 128, 131 of 128 x 128 in four.  Steps of 64 indices, half a cache line,
-// take 137, although their loads can be three steps ahead.
+// a product.  With the rows' rounding, in bfloat16: 30011 x 768 x 3352 takes 122 - 125 us
+// in them, 128 in 192 x 256, 131 - 133 in 256 x 128 or 128 x 256, 125 in 128 x 128 in
+// four wavefronts; 8192 x 8192 x 8192 494, 539, 606 - 618 and 587.
 template <int WM, int WN, int MI>
 struct Shape {
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, ROWS = 16 * WM * MI, OUTS = 64 * WN;
@@ -411,9 +413,11 @@ __device__ __forceinline__ bool put_tile(const ProductArgs& p, int64_t m0, int n
 // row of steps.  A wavefront's loads and stores are done in the order of their issue,
 // so that the first step of a tile, whose loads are older than the last tile's stores,
 // need not wait for those.  Of 104 us the matrix units work 33 (8-bit products at
-// their full rate); in a form that took 132 us, 109 were left without the loads, 87
-// without the products and 86 without the stores, so the rest is what these three do
-// not hide of each other.
+// their full rate).  The 24 outputs behind the last multiple of 256 of 3352 are 118 tiles
+// of their own, and take the 1652 tiles from 5.99 rounds of the 256 CUs to 6.45, which is
+// seven.  The rest is what loads, products and stores do not hide of each other: in an
+// earlier form that took 132 us, 109 were left without the loads, 87 without the products
+// and 86 without the stores.
 template <class O, int WM, int WN, int MI>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_many(ProductArgs p) {
   using S = Shape<WM, WN, MI>;
@@ -512,7 +516,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_many(ProductArgs p) {
   }
 }
 
-// The same for weights that are not aligned to 16 bytes, through registers.
+// The same for weights that are not aligned to 16 bytes, through registers.  With the
+// rows' rounding, in bfloat16: 30011 rows of 333 inputs and 1280 outputs take 73 us (of
+// 320 inputs, aligned, 45), of 1001 inputs and 643 outputs 83 (1008: 70).
 template <class O>
 __global__ __launch_bounds__(256) void k_many_narrow(ProductArgs p) {
   using S = Shape<2, 2, 4>;
@@ -627,7 +633,7 @@ void int8_linear(const Int8& p, void* y, void* workspace, hipStream_t stream) {
   a.q = q;
   a.row_scale = row_scale;
   // Tiles that few CUs would have are cut finer.  128 rows of 768 inputs and 3352
-  // outputs (27 tiles) take 10.5 us here and 11.3 in tiles, 192 (54 tiles) 12.3 and 11.5.
+  // outputs (27 tiles) take 10.4 us here and 11.4 in tiles, 192 (54 tiles) 12.4 and 11.4.
   if (tiles_of(p.rows, p.outputs, 128) < 32) {
     by_type([&](auto zero) {
       using O = decltype(zero);
@@ -651,8 +657,9 @@ void int8_linear(const Int8& p, void* y, void* workspace, hipStream_t stream) {
     };
     by_type([&](auto zero) {
       using O = decltype(zero);
-      // Large tiles as soon as every CU has one: of 3352 outputs 22.0 us and 16.8 in small
-      // ones for 2048 rows, 42.0 and 42.9 for 8192, 134 and 137 for 30011.
+      // Large tiles as soon as every CU has one.  With the rows' rounding, of 768 inputs and
+      // 3352 outputs: 2048 rows 22.2 us and 16.8 in small ones, 4096 26.3 and 26.1, 8192 41.4
+      // and 40.3, 30011 122 and 125; of 8192 inputs and outputs 8192 rows 492 and 587.
       if (!wide) k_many_narrow<O><<<tiles(128, 128, 1 << 30), 256, 0, stream>>>(a);
       else if (tiles_of(p.rows, p.outputs, 256) >= 256) k_many<O, 2, 4, 8><<<tiles(256, 256, 256), 512, 0, stream>>>(a);
       else k_many<O, 2, 2, 4><<<tiles(128, 128, 512), 256, 0, stream>>>(a);

@@ -7,10 +7,15 @@
 // A row is held in registers by one wavefront, four or sixteen, so that each
 // input is read once, and v and r are computed again in the gradient instead of
 // being kept.  Bound by memory: 30011 rows of 1536 channels with a gate in bfloat16
-// take 44 us (6.3 TB/s, part of it from the last-level cache), the residual and norm
-// of 8192 rows of 768 15 us, their gradient 24.  The sums over rows stay in registers
+// take 45 us (6.2 TB/s, part of it from the last-level cache), the residual and norm
+// of 8192 rows of 768 15 us, their gradient 25.  The sums over rows stay in registers
 // over the rows that a wavefront walks, and a second kernel adds what the workgroups
 // leave, in a fixed order (4.5 us).
+//   The sixteen of a wide row have 128 registers each, which do not hold all: gradients
+// of more than 8192 channels and most results of more than 16384 keep a part of the row in
+// scratch memory.  Of 2^26 elements with a gate in bfloat16 the gradient takes 0.25 ms in
+// rows of 8192, 0.95 of 8193, 0.15 of 16384, 1.8 of 16385 and 0.53 of 32768 (its bytes:
+// 0.15), the results 0.07, 0.16, 0.08, 0.31 and 0.09.
 #pragma clang fp contract(fast)
 #include <algorithm>
 
@@ -141,6 +146,8 @@ __global__ __launch_bounds__(threads_of(W)) void k_norm(NormArgs p) {
   }
 }
 
+// Either gradient may be absent, which is looked at within the loop: 16-bit pieces of dy are
+// waited for one by one for that, and those of dsum are asked for behind the reduction.
 template <class A, class O, int MODE, int W, int PER, int COVER>
 __global__ __launch_bounds__(threads_of(W)) void k_norm_back(NormArgs p) {
   using B = std::conditional_t<MODE == ADDED || MODE == SUMMED, O, A>;

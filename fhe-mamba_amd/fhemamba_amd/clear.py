@@ -620,8 +620,9 @@ def rms_norm(x, weight, *, gate=None, groups: int = 1, eps: float = 1e-5, dtype=
 
     x [.., channels] and gate alike, weight [channels] float32.  The mean is over each of `groups`
     equal parts of the channels, of at most 32768 each.  The result is of x's type or, with dtype,
-    bfloat16.  Differentiable in x, weight and gate.  Squares are summed in 32 bits: a row with values
-    over 2^63 gives zeros; one with a value that is not finite has NaN in it."""
+    bfloat16.  Differentiable in x, weight and gate.  Squares are summed in 32 bits: a row whose
+    squares come to 2^128 or more gives zeros, one of squares below 2^-126 counts as zeros, and one with a
+    value that is not finite has NaN in it; the gradient's products with v are summed in 32 bits too."""
     _leading("x", x)
     channels = x.shape[-1]
     if groups < 1 or channels % groups or channels // groups > MAX_ROW or groups > 65535:
@@ -745,8 +746,9 @@ def int8_linear(x, weight, weight_scale, bias=None):
     """x [.., inputs] times weight [outputs, inputs] int8 and weight_scale [outputs] float32 (as
     quantize_rows gives them), plus bias [outputs] float32: [.., outputs] of x's type.
 
-    x's rows are rounded as quantize_rows does (at most 32768 inputs); the sums of products are exact, and
-    scaled in 32 bits.  A row with a value that is not finite gives NaN.  For serving: no gradient."""
+    x's rows are rounded as quantize_rows does (at most 32768 inputs; a result of fewer than 2^34 elements);
+    the sums of products are exact, and scaled in 32 bits.  A row with a value that is not finite gives NaN.
+    For serving: no gradient."""
     _leading("x", x)
     _axes("weight", weight, 2, "be [outputs, inputs]")
     inputs, outputs = x.shape[-1], weight.shape[0]
@@ -805,8 +807,8 @@ def embed(weight, ids, *, scale: float = 1.0):
     """scale * weight[ids]: weight [vocab, channels], ids [..] int64 -> [.., channels] of weight's type.
 
     An id below 0 is padding: zeros, and no gradient from it; one of vocab or more gives NaN.
-    Differentiable in weight: the gradient is dense, each row the sum in 32 bits of its tokens' in
-    their order."""
+    Differentiable in weight: the gradient is dense, each row the sum in 32 bits of its tokens', in an
+    order that the ids fix."""
     _first("weight", weight, 2)
     if min(weight.shape) < 1:
         raise ValueError("weight must have a vocabulary and channels")

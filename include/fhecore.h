@@ -502,8 +502,8 @@ typedef struct {
  * is no gate (data NULL); the mean is over each of `groups` equal parts of the
  * channels.  x and gate in dtype, y [rows][channels] in out_dtype, which is dtype
  * or FHE_BF16.  A part has at most FHE_MAX_ROW channels.  Squares are summed in 32
- * bits: values over 2^63 give zeros.  A row with a value that is not finite has
- * NaN in it. */
+ * bits: a row whose squares come to 2^128 or more gives zeros, and one of squares
+ * below 2^-126 counts as zeros.  A row with a value that is not finite has NaN in it. */
 enum { FHE_MAX_ROW = 32768 };
 typedef struct {
   uint32_t dtype, out_dtype, groups;
@@ -566,7 +566,8 @@ int fhe_quantize_rows(const fhe_quantize_args *args, int8_t *values,
 
 /* y = (q weight^T) row_scale scale + bias, q and row_scale those of x's rows as
  * above: [rows][outputs] in dtype.  weight [outputs][inputs], scale and bias
- * [outputs] (bias may be NULL).  The sums of products are exact. */
+ * [outputs] (bias may be NULL).  The sums of products are exact.  Rows in whole 64
+ * times outputs in whole 16 are fewer than 2^34. */
 typedef struct {
   uint32_t dtype, reserved;
   int64_t rows, inputs, outputs;
@@ -589,8 +590,8 @@ typedef struct {
 } fhe_embed_args;
 int fhe_embed(const fhe_embed_args *args, void *y, void *hip_stream);
 int fhe_embed_workspace(const fhe_embed_args *args, size_t *bytes);
-/* dweight [vocab][channels] in dtype: scale times the sum, in 32 bits and in the
- * tokens' order, of each id's rows of dy.  weight is not read. */
+/* dweight [vocab][channels] in dtype: scale times the sum, in 32 bits and in an order
+ * that the ids fix, of each id's rows of dy.  weight is not read. */
 int fhe_embed_backward(const fhe_embed_args *args, const fhe_rows *dy,
                        void *dweight, void *workspace, size_t bytes,
                        void *hip_stream);

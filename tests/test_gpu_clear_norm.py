@@ -383,3 +383,25 @@ def test_gates_of_16_bits_element_by_element(low, high):
     step = torch.exp2(torch.floor(torch.log2(want.abs())) - 7)
     over = ((got - want).abs() - step / 2) / want.abs()
     assert over.max().item() * 2.0 ** 24 <= 28, over.max().item() * 2.0 ** 24
+
+
+def test_squares_at_the_ends_of_32_bits():
+    """What counts is the squares' sum: beyond 2^128 a row gives zeros, and so does its gradient."""
+    from fhemamba_amd import clear
+
+    w = torch.ones(768, device="cuda")
+    x = torch.zeros(4, 768, device="cuda")
+    x[0, 5] = 2.0 ** 63.5                 # its square is 2^127
+    x[1] = 2.0 ** 60                      # 768 of 2^120
+    x[2] = 2.0 ** 59                      # 768 of 2^118, below 2^128
+    x[3] = 2.0 ** -60                     # 768 of 2^-120
+    leaf = x.requires_grad_(True)
+    y = clear.rms_norm(leaf, w, eps=0.0)
+    want = torch.zeros(4, 768, device="cuda")
+    want[0, 5], want[2:] = 768 ** 0.5, 1.0
+    torch.testing.assert_close(y, want, rtol=2.0 ** -16, atol=0)
+    dy = torch.arange(768, device="cuda") % 2 * 2.0 - 1.0
+    (g,) = torch.autograd.grad(y, leaf, dy.expand(4, 768))
+    assert bool(torch.isfinite(g).all()) and not bool(g[1].any())
+    torch.testing.assert_close(g[2], dy * 2.0 ** -59, rtol=2.0 ** -16, atol=0)
+    torch.testing.assert_close(g[3], dy * 2.0 ** 60, rtol=2.0 ** -16, atol=0)
