@@ -621,8 +621,8 @@ def rms_norm(x, weight, *, gate=None, groups: int = 1, eps: float = 1e-5, dtype=
     x [.., channels] and gate alike, weight [channels] float32.  The mean is over each of `groups`
     equal parts of the channels, of at most 32768 each.  The result is of x's type or, with dtype,
     bfloat16.  Differentiable in x, weight and gate.  Squares are summed in 32 bits: a row whose
-    squares come to 2^128 or more gives zeros, one of squares below 2^-126 counts as zeros, and one with a
-    value that is not finite has NaN in it; the gradient's products with v are summed in 32 bits too."""
+    squares come to 2^128 or more gives zeros, squares below 2^-126 lose bits, and a row with a value that is
+    not finite has NaN in it; the gradient's products with v are summed in 32 bits too."""
     _leading("x", x)
     channels = x.shape[-1]
     if groups < 1 or channels % groups or channels // groups > MAX_ROW or groups > 65535:

@@ -502,8 +502,8 @@ typedef struct {
  * is no gate (data NULL); the mean is over each of `groups` equal parts of the
  * channels.  x and gate in dtype, y [rows][channels] in out_dtype, which is dtype
  * or FHE_BF16.  A part has at most FHE_MAX_ROW channels.  Squares are summed in 32
- * bits: a row whose squares come to 2^128 or more gives zeros, and one of squares
- * below 2^-126 counts as zeros.  A row with a value that is not finite has NaN in it. */
+ * bits: a row whose squares come to 2^128 or more gives zeros, and squares below
+ * 2^-126 lose bits.  A row with a value that is not finite has NaN in it. */
 enum { FHE_MAX_ROW = 32768 };
 typedef struct {
   uint32_t dtype, out_dtype, groups;
